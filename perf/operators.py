@@ -390,8 +390,8 @@ def _own(s):
                                   cos=s["cos"], sin=s["sin"], interleaved=case["inter"])
         return _values(s)
     if "ws" not in s:   # a program's own workspace, kept from step to step
-        n = ops.attention_chunk_workspace_bytes(s["rows"], case["seqs"], mp * PAGE, case["heads"],
-                                                case["kvh"], case["hd"])
+        n = ops.attention_chunk_workspace_bytes(s["rows"], case["seqs"], case["new"], mp * PAGE,
+                                                case["heads"], case["kvh"], case["hd"])
         s["ws"] = torch.empty(max(n, 1), dtype=torch.uint8, device=DEV)
     ops.attention_chunk_batch(s["q"], s["qs"], kv, pages, s["tables"], mp, s["row0"], s["kv_len"],
                               case["seqs"], case["new"], s["o"], None, case["heads"], case["kvh"],
