@@ -31,6 +31,8 @@ extern "C" {
 
 /* MatrixView dtype codes (kernels/config.h:86-90; tools/pqwf.py:28-33). */
 enum { Q3_DT_I8 = 0, Q3_DT_U8 = 1, Q3_DT_I32 = 2, Q3_DT_U32 = 3, Q3_DT_F32 = 4 };
+/* 16-bit rows, taken by the rotary and paged-cache extensions below only. */
+enum { Q3_DT_F16 = 5, Q3_DT_BF16 = 6 };
 
 /* Status codes. */
 enum {
@@ -292,6 +294,88 @@ int q3_prefill_batch(void *blob, const q3_layout *layout, const q3_kv_pool *pool
                      uint32_t n_seqs, uint32_t T, int32_t *next_ids, void *workspace,
                      size_t workspace_bytes, void *stream);
 
+/* ---- rotary positions and paged chunks (extension) -------------------------
+ * The steps between the projections and the attention as operators of their
+ * own, for ragged batches of sequences over one page pool: rotary tables with
+ * scaled positions, rotation of rows, the append of new K/V rows to the pages,
+ * and the attention of each sequence's new rows over its pages.
+ *
+ * A ragged batch is two device arrays: row0[n_seqs + 1], ascending, and
+ * kv_len[n_seqs].  Sequence s owns rows row0[s] .. row0[s+1]-1 of the row
+ * views (none is allowed); they are its last tokens, at positions
+ * kv_len[s] - n_s + i, n_s = row0[s+1] - row0[s]: kv_len counts them.  Rows at
+ * and behind row0[n_seqs] belong to nobody and are left as they were.  What
+ * these arrays and the page tables hold is checked on the device: a row that
+ * does not fit is skipped and sets a bit of q3_device_status.
+ * Row views: head h of row r at columns h*head_dim; head_dim 64, 128 or 256
+ * (attention: 64 or 128); bases and row strides in multiples of 16 bytes. */
+enum { Q3_ROPE_NONE = 0, Q3_ROPE_LINEAR = 1, Q3_ROPE_YARN = 2 };
+typedef struct q3_rope_spec {
+  double theta;               /* base, > 1                                    */
+  double factor;              /* LINEAR, YARN: context extension, >= 1        */
+  double original_max;        /* YARN: positions the weights were trained for */
+  double beta_fast, beta_slow;/* YARN: turns within original_max above / below
+                               * which a pair keeps / divides its frequency (32, 1) */
+  double attn_factor;         /* on cos and sin; <= 0: 1, YARN 0.1 ln(factor) + 1   */
+  int32_t scaling;            /* Q3_ROPE_*                                    */
+} q3_rope_spec;
+
+/* cos[p][i], sin[p][i] (f32, cols = rot/2 <= 128 of both) = attn_factor *
+ * cos / sin((pos0 + p) * f_i): f_i = theta^(-2i/rot), LINEAR: divided by
+ * factor, YARN: blended between the two by a ramp over the pairs.  The angle
+ * is reduced exactly (integer arithmetic modulo one turn), whatever pos0. */
+int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_view *cos,
+                   const q3_view *sin, void *stream);
+
+/* Per row r and head: RMSNorm over the head with weights nw (optional;
+ * inv_hd = 1/head_dim), then rotation of the first rot = 2*cos->cols columns
+ * (a multiple of 16) by row pos[r] of the tables: pairs (i, i + rot/2), or
+ * (2i, 2i + 1) with interleaved.  x: f32, f16 or bf16.  out: f32, f16, bf16
+ * (rounded once; may be x itself), or int8 with one scale per head in `scale`
+ * (rows x heads f32), the codes of the norm-rope-quant epilogue of
+ * q3_gemm_nt_group_store bit for bit.  A row whose position is not in the tables
+ * is not written (status bit 4). */
+int q3_rope_rows(const q3_view *x, const q3_view *nw, const int32_t *pos, const q3_view *cos,
+                 const q3_view *sin, const q3_view *out, const q3_view *scale, uint32_t heads,
+                 uint32_t head_dim, int interleaved, float inv_hd, void *stream);
+
+/* Writes the batch's new K and V rows (f32, f16 or bf16, k->rows of them) to
+ * the pages of their sequences, tables[s*max_pages ...]: K through the norm
+ * (nw optional) and the rotation of q3_rope_rows at the rows' positions (cos
+ * and sin both null: none), then int8 with one scale per token and head, as
+ * q3_quant_rows_heads forms them.  kv->table is ignored; pages
+ * 0..num_pages-1.  No two sequences may share a page that is written. */
+int q3_paged_kv_append_batch(const q3_view *k, const q3_view *v, const q3_view *nw, float inv_hd,
+                             const q3_view *cos, const q3_view *sin, int interleaved,
+                             const q3_paged_kv *kv, uint32_t num_pages, const uint16_t *tables,
+                             uint32_t max_pages, const int32_t *row0, const int32_t *kv_len,
+                             uint32_t n_seqs, uint32_t kv_heads, uint32_t head_dim, void *stream);
+
+/* Attention of the batch's rows over their pages (appended before): row at
+ * position p sees keys 0..p (causal) or all kv_len[s], and of these only
+ * those after p - window where window > 0 (causal only).  For each query head
+ *   o = sum_j softmax_j(qk_scale * q.k_j) v_j,
+ * k_j and v_j being the int8 codes times their scales (scales are not
+ * negative; a V scale below 2^-100 counts as 2^-100): the softmax of the definition, in
+ * float32 with f16 weights, without the per-block requantisation of
+ * q3_attention_heads_gqa_tokscale_paged.  A row that sees no key gives zeros.
+ * q: int8 with q_scale (rows x heads f32), f16 or bf16.  o: int8 with os (one
+ * scale per head, as q3_quant_rows_heads), f16 or bf16.  heads is a multiple
+ * of kv_heads, at most 16 times it.  max_rows: no sequence has more new rows;
+ * one that has sets status bit 5 and is skipped.  The workspace of
+ * q3_attention_chunk_workspace_bytes (max_kv = max_pages * page_tokens) is written
+ * by the call; calls that may overlap on the GPU need one each. */
+size_t q3_attention_chunk_workspace_bytes(uint32_t rows, uint32_t n_seqs, uint32_t max_rows,
+                                          uint32_t max_kv, uint32_t heads, uint32_t kv_heads,
+                                          uint32_t head_dim);
+int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale, const q3_paged_kv *kv,
+                             uint32_t num_pages, const uint16_t *tables, uint32_t max_pages,
+                             const int32_t *row0, const int32_t *kv_len, uint32_t n_seqs,
+                             uint32_t max_rows, const q3_view *o, const q3_view *os,
+                             uint32_t heads, uint32_t kv_heads, uint32_t head_dim, int causal,
+                             uint32_t window, float qk_scale, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
 /* ---- host batching engine (extension; tools/engine.py:81-243) -------------
  * The reference's PagePool / Scheduler / Sampler / Engine.step in native code:
  * requests in admission order, prompts fed in chunks of up to 32 rows, one
@@ -547,9 +631,11 @@ int q3_device_check(void); /* Q3_OK on an sm_100 device, else Q3_ERR_ARCH */
 
 /* Device-side error word of the library's kernels (0 = none; bit 1: a page
  * index beyond the pool was skipped; bit 2: a sequence needs more pages than
- * its table holds; bit 3 and bits 16-19: a bounded wait in a tensor-core GEMM or
- * attention pipeline timed out and the kernel gave up; bit 20: a
- * tensor-parallel exchange wait for another rank timed out).  Reading
+ * its table holds; bit 4: a position outside the rotary tables; bit 5: row0,
+ * kv_len and max_rows of a ragged batch do not fit each other; bit 3 and bits
+ * 16-19: a bounded wait in a tensor-core GEMM or attention pipeline timed out
+ * and the kernel gave up; bit 20: a tensor-parallel exchange wait for another
+ * rank timed out).  Reading
  * synchronises with the device and clears
  * the word; -1 if it cannot be read. */
 int q3_device_status(void);

@@ -12,6 +12,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libq3b200.so"
 
 DT_I8, DT_U8, DT_I32, DT_U32, DT_F32 = 0, 1, 2, 3, 4
+DT_F16, DT_BF16 = 5, 6   # rotary and paged-chunk operators only
 
 STATUS = {0: "OK", 1: "NULL", 2: "MODE", 3: "SHAPE", 4: "DTYPE", 5: "ALIGN", 6: "CUDA",
           7: "CAPACITY", 8: "ARCH"}
@@ -50,6 +51,12 @@ class PagedKV(C.Structure):
                 ("table", C.c_void_p), ("page_tokens", C.c_uint32), ("page_bytes", C.c_uint32),
                 ("row_bytes", C.c_uint32), ("scale_page_bytes", C.c_uint32),
                 ("scale_row_bytes", C.c_uint32)]
+
+
+class RopeSpec(C.Structure):
+    _fields_ = [("theta", C.c_double), ("factor", C.c_double), ("original_max", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attn_factor", C.c_double),
+                ("scaling", C.c_int32)]
 
 
 class Layout(C.Structure):
@@ -106,6 +113,17 @@ SIGS = {
     "q3_prefill_batch": [C.c_void_p, C.POINTER(Layout), C.POINTER(KVPool), C.c_void_p, C.c_uint32,
                          C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_size_t,
                          C.c_void_p],
+    "q3_rope_tables": [C.POINTER(RopeSpec), C.c_uint32, VP, VP, C.c_void_p],
+    "q3_rope_rows": [VP, VP, C.c_void_p, VP, VP, VP, VP, C.c_uint32, C.c_uint32, C.c_int,
+                     C.c_float, C.c_void_p],
+    "q3_paged_kv_append_batch": [VP, VP, VP, C.c_float, VP, VP, C.c_int, C.POINTER(PagedKV),
+                                 C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p,
+                                 C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p],
+    "q3_attention_chunk_workspace_bytes": [C.c_uint32] * 7,
+    "q3_attention_chunk_batch": [VP, VP, C.POINTER(PagedKV), C.c_uint32, C.c_void_p, C.c_uint32,
+                                 C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, VP, VP,
+                                 C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_uint32,
+                                 C.c_float, C.c_void_p, C.c_size_t, C.c_void_p],
     "q3_sample_workspace_bytes": [C.c_uint32, C.c_uint32],
     "q3_sample_logits": [VP, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                          C.c_void_p],
@@ -128,7 +146,8 @@ SIGS = {
     "q3_timer_attach": [C.c_char_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int],
     "q3_timer_detach": [],
 }
-RESTYPE = {"q3_gemm_nt_group_argmax_workspace_bytes": C.c_size_t,
+RESTYPE = {"q3_attention_chunk_workspace_bytes": C.c_size_t,
+           "q3_gemm_nt_group_argmax_workspace_bytes": C.c_size_t,
            "q3_sample_workspace_bytes": C.c_size_t, "q3_tokenizer_eos_id": C.c_int32,
            "q3_forward_workspace_bytes": C.c_size_t, "q3_decode_workspace_bytes": C.c_size_t,
            "q3_prefill_workspace_bytes": C.c_size_t,

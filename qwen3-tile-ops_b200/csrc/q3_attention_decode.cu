@@ -472,6 +472,8 @@ int dgemm_device_status_take();
 int pattn_device_status_take();
 int tp_device_status_take();
 int dsplit_device_status_take();
+int rope_device_status_take();
+int chunk_device_status_take();
 }
 
 extern "C" int q3_device_status(void) {
@@ -495,5 +497,11 @@ extern "C" int q3_device_status(void) {
   const int ds = q3::dsplit_device_status_take();
   if (ds < 0) return -1;
   v |= static_cast<unsigned int>(ds);
+  const int ro = q3::rope_device_status_take();
+  if (ro < 0) return -1;
+  v |= static_cast<unsigned int>(ro);
+  const int ch = q3::chunk_device_status_take();
+  if (ch < 0) return -1;
+  v |= static_cast<unsigned int>(ch);
   return static_cast<int>(v) | g;
 }

@@ -409,7 +409,10 @@ enum TimerFamily { TIMER_NONE = 0, TIMER_ATTENTION = 1, TIMER_GEMM = 2, TIMER_EX
 void timer_begin(int family, cudaStream_t s);
 void timer_end(int family, cudaStream_t s);
 
-inline int dt_size(uint8_t dt) { return (dt == Q3_DT_I8 || dt == Q3_DT_U8) ? 1 : 4; }
+inline int dt_size(uint8_t dt) {
+  if (dt == Q3_DT_I8 || dt == Q3_DT_U8) return 1;
+  return (dt == Q3_DT_F16 || dt == Q3_DT_BF16) ? 2 : 4;
+}
 
 // A view usable by the kernels: non-null, dtype as expected, elements
 // contiguous within a row (col_bytes == element size), aligned to `align`

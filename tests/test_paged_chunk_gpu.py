@@ -1,0 +1,630 @@
+"""Rotary tables and rows, the append of K/V rows to the int8 pages, and the attention of a ragged
+batch over them, on the GPU against float64 formulas (float32 steps where the codes are defined by
+them).
+
+Roundings: a result rounded to type t is off by at most eps(t)/2 of its value.  The attention
+rounds its weights to f16 (2^-11 of each, and 2^-25 of the row's largest weight below f16's normal
+range); everything else is float32, allowed for as 2^-20 of the largest logit's terms."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+F = np.float32
+
+
+@pytest.fixture(scope="module")
+def ops(q3):
+    assert torch.cuda.is_available(), "GPU tests need CUDA"
+    return q3.ops
+
+
+@pytest.fixture(autouse=True)
+def clean_status(request, q3):
+    q3._lib.lib().q3_device_status()
+    yield
+    if "status" not in request.node.keywords:
+        assert q3._lib.lib().q3_device_status() == 0
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+# ------------------------------------------------------------------ tables
+def ref_freq(rot, theta, scaling, factor, orig, fast=32.0, slow=1.0):
+    f = np.array([theta ** (-2.0 * i / rot) for i in range(rot // 2)])
+    if scaling == "linear":
+        return f / factor
+    if scaling == "yarn":
+        per = rot / (2 * math.log(theta))
+        lo = max(0, math.floor(per * math.log(orig / (fast * 2 * math.pi))))
+        hi = min(rot - 1, math.ceil(per * math.log(orig / (slow * 2 * math.pi))))
+        t = np.clip((np.arange(rot // 2) - lo) / max(hi - lo, 1e-3), 0, 1)
+        return f * (1 - t) + f / factor * t
+    return f
+
+
+@pytest.mark.parametrize("rot,theta,scaling,factor,orig", [
+    (128, 1e6, "none", 1.0, 0), (64, 1e4, "linear", 2.5, 0), (128, 1e6, "yarn", 4.0, 32768),
+    (256, 5e5, "yarn", 8.0, 4096), (2, 10.0, "none", 1.0, 0), (34, 1e4, "yarn", 1.0, 64)])
+@pytest.mark.parametrize("n,pos0", [(1, 0), (1, 2 ** 31 + 12345), (77, 131071), (3000, 0)])
+def test_rope_tables(ops, rot, theta, scaling, factor, orig, n, pos0):
+    cos = torch.full((n, rot // 2), 9.0, device="cuda")
+    sin = torch.full((n, rot // 2 + 3), 9.0, device="cuda")[:, :rot // 2]   # a strided view
+    ops.rope_tables(cos, sin, theta, pos0, scaling, factor, orig)
+    a = 0.1 * math.log(factor) + 1 if scaling == "yarn" else 1.0
+    ang = np.outer(np.arange(pos0, pos0 + n, dtype=np.float64), ref_freq(rot, theta, scaling,
+                                                                         factor, orig))
+    # float32: the functions' last bit, the scaling by a; the oracle's angle: 2^-52 of itself
+    tol = a * (4 * 2.0 ** -24 + 2 * ang.max() * 2.0 ** -52)
+    assert np.abs(cos.cpu().numpy() - a * np.cos(ang)).max() <= tol
+    assert np.abs(sin.cpu().numpy() - a * np.sin(ang)).max() <= tol
+
+
+# -------------------------------------------------------------------- rows
+def tables_f32(span, rot, theta=1e6):
+    ang = torch.outer(torch.arange(span, dtype=torch.float64, device="cuda"),
+                      torch.tensor(ref_freq(rot, theta, "none", 1, 0), device="cuda"))
+    return torch.cos(ang).float(), torch.sin(ang).float()
+
+
+def ref_norm(x, w):
+    return x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w
+
+
+def ref_rotate(x, cos, sin, inter):
+    """x [rows][heads][hd]; cos, sin [rows][half], all float64."""
+    half = cos.shape[1]
+    c, s = cos[:, None], sin[:, None]
+    y = x.clone()
+    a = slice(0, 2 * half, 2) if inter else slice(0, half)
+    b = slice(1, 2 * half, 2) if inter else slice(half, 2 * half)
+    y[..., a] = x[..., a] * c - x[..., b] * s
+    y[..., b] = x[..., a] * s + x[..., b] * c
+    return y
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("rows,heads,hd,rot", [(1, 1, 64, 64), (7, 3, 128, 128), (33, 16, 128, 64),
+                                               (5, 6, 256, 256), (130, 5, 64, 16), (3, 9, 256, 80),
+                                               (2, 4, 128, 112)])
+@pytest.mark.parametrize("xt,ot,norm", [("f32", "f32", True), ("f32", "f16", False),
+                                        ("bf16", "bf16", False), ("f16", "bf16", True),
+                                        ("f16", "f32", False)])
+def test_rope_rows(ops, rows, heads, hd, rot, inter, xt, ot, norm):
+    g = gen(rows * hd + rot)
+    wide = torch.randn(rows, heads * hd + 16, device="cuda", generator=g).to(TYPES[xt])
+    x = wide[:, 8:8 + heads * hd] if xt != "f32" else wide[:, 4:4 + heads * hd]
+    pos = torch.randint(0, 999, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    cos, sin = tables_f32(999, rot)
+    nw = torch.rand(hd, device="cuda", generator=g) + 0.5 if norm else None
+    out = torch.full((rows + 2, heads * hd), 7.0, device="cuda", dtype=TYPES[ot])
+    ops.rope_rows(x, pos, cos, sin, out, heads, hd, nw=nw, interleaved=inter)
+    want = x.double().reshape(rows, heads, hd)
+    if norm:
+        want = ref_norm(want, nw.double())
+    p = pos.long()
+    want = ref_rotate(want, cos.double()[p], sin.double()[p], inter).reshape(rows, -1)
+    # float32 steps: two products and a sum (3), the norm (sum of hd squares: 2 + 5 + 8, root,
+    # quotient, two products), each 2^-24 of at most sqrt(2) of the largest value
+    tol = half_step(TYPES[ot]) * want.abs() + 20 * 2.0 ** -24 * want.abs().max() * 1.5
+    assert ((out[:rows].double() - want).abs() <= tol).all()
+    assert (out[rows:] == 7.0).all()
+
+
+def test_rope_rows_in_place_and_bad_positions(ops, q3, request):
+    request.node.keywords["status"] = True
+    g = gen(3)
+    x = torch.randn(6, 2 * 128, device="cuda", generator=g)
+    cos, sin = tables_f32(50, 128)
+    pos = torch.tensor([0, 49, 50, -1, 2 ** 31 - 1, 7], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(x)
+    ops.rope_rows(x, pos.clamp(0, 49), cos, sin, out, 2)
+    before = x.clone()
+    assert q3._lib.lib().q3_device_status() == 0
+    ops.rope_rows(x, pos, cos, sin, x, 2)
+    assert q3._lib.lib().q3_device_status() == 1 << 4
+    ok = [0, 1, 5]
+    assert torch.equal(x[ok], out[ok]) and torch.equal(x[2:5], before[2:5])
+
+
+# ------------------------------------------------------------------ the pool
+class Pool:
+    """A page pool and the ragged batch over it: lens = (new rows, tokens with them) a sequence."""
+
+    def __init__(self, ops, lens, kvh, hd, page=32, seed=0, pad_heads=0, spare=0):
+        g = gen(seed)
+        self.lens, self.kvh, self.hd, self.page = lens, kvh, hd, page
+        self.mp = max(1, max(-(-kv // page) for _, kv in lens)) + spare
+        n = self.n_pages = len(lens) * self.mp + 3
+        w = kvh + pad_heads
+        self.k = (torch.randn(n, page, w * hd, device="cuda", generator=g) * 42).round() \
+            .clamp(-127, 127).to(torch.int8)
+        self.v = (torch.randn(n, page, w * hd, device="cuda", generator=g) * 42).round() \
+            .clamp(-127, 127).to(torch.int8)
+        self.ks = torch.rand(n, page, w, device="cuda", generator=g) * 0.03 + 0.005
+        self.vs = torch.rand(n, page, w, device="cuda", generator=g) * 0.03 + 0.005
+        self.tables = torch.randperm(n, generator=torch.Generator().manual_seed(seed))[
+            :len(lens) * self.mp].to(torch.int16).cuda().view(len(lens), self.mp)
+        row0 = np.cumsum([0] + [a for a, _ in lens]).astype(np.int32)
+        self.rows = int(row0[-1])
+        self.row0 = torch.from_numpy(row0).cuda()
+        self.kv_len = torch.tensor([b for _, b in lens], dtype=torch.int32, device="cuda")
+        self.max_rows = max(a for a, _ in lens)
+        self.kv = ops.paged_kv(self.k, self.v, self.ks, self.vs, self.tables, w, hd, page)
+
+    def cached(self, s, kvlen=None):
+        """K and V of sequence s: float64 [tokens][kvh][hd]."""
+        n = self.lens[s][1] if kvlen is None else kvlen
+        pages = self.tables[s, :-(-n // self.page)].long() & 0xFFFF
+        return [(c[pages].reshape(-1, c.shape[-1] // self.hd, self.hd)[:n, :self.kvh].double(),
+                 sc[pages].reshape(-1, sc.shape[-1])[:n, :self.kvh].double())
+                for c, sc in ((self.k, self.ks), (self.v, self.vs))]
+
+
+# ------------------------------------------------------------------- append
+def int8_f32(x):
+    """Codes and scales by the float32 steps of the cache's other writers."""
+    x = x.astype(F)
+    scale = (np.abs(x).max(-1) * F(1.0 / 127.0)).astype(F)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        q = np.rint((x / scale[..., None]).astype(F))
+    return np.clip(np.nan_to_num(q), -127, 127).astype(np.int8), scale
+
+
+def norm_rope_f32(x, nw, cos, sin, inter):
+    """x [rows][heads][hd] float32 through the path's float32 steps."""
+    from oracle import q3_oracle as O
+    if nw is not None:
+        r, h, d = x.shape
+        x = O.rmsnorm(x.reshape(r * h, d), nw, F(1.0 / d)).reshape(r, h, d)
+    if cos is None:
+        return x
+    half = cos.shape[1]
+    c, s = cos[:, None].astype(F), sin[:, None].astype(F)
+    a = slice(0, 2 * half, 2) if inter else slice(0, half)
+    b = slice(1, 2 * half, 2) if inter else slice(half, 2 * half)
+    y = x.copy()
+    y[..., a] = (x[..., a] * c).astype(F) - (x[..., b] * s).astype(F)
+    y[..., b] = (x[..., a] * s).astype(F) + (x[..., b] * c).astype(F)
+    return y
+
+
+@pytest.mark.parametrize("kvh,hd,page,rot,inter,norm,t,lens", [
+    (8, 128, 32, 128, False, True, "f32", [(1, 1), (1, 32), (1, 33), (0, 5), (1, 64)]),
+    (2, 64, 16, 32, True, False, "bf16", [(40, 40), (0, 0), (3, 100), (17, 31)]),
+    (1, 128, 32, 0, False, False, "f16", [(5, 70)]),
+    (5, 256, 8, 256, False, True, "f16", [(9, 20), (1, 8), (30, 30)]),
+    (4, 64, 7, 64, False, True, "bf16", [(13, 29), (8, 9)]),
+    (3, 128, 32, 64, True, True, "f32", [(1, 1 + s % 40) for s in range(70)])])
+def test_append(ops, kvh, hd, page, rot, inter, norm, t, lens):
+    P = Pool(ops, lens, kvh, hd, page, seed=kvh + hd, pad_heads=1)
+    g = gen(11)
+    x = [(torch.randn(P.rows + 3, kvh * hd + 8, device="cuda", generator=g)).to(TYPES[t])
+         for _ in range(2)]
+    k, v = (y[:, :kvh * hd] for y in x)
+    k[0, :hd] = 0.0                                   # an all-zero head: scale 0, codes 0
+    nw = torch.rand(hd, device="cuda", generator=g) + 0.5 if norm else None
+    cos, sin = tables_f32(P.mp * page, rot) if rot else (None, None)
+    want = [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+    ops.paged_kv_append_batch(k, v, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, len(lens),
+                              kvh, hd, nw=nw, cos=cos, sin=sin, interleaved=inter)
+    host = lambda y: y.float().cpu().numpy()          # noqa: E731
+    for s, (n, kv) in enumerate(lens):
+        if not n:
+            continue
+        r = slice(int(P.row0[s]), int(P.row0[s]) + n)
+        p = torch.arange(kv - n, kv, device="cuda")
+        at = ((P.tables[s].long() & 0xFFFF)[p // page], p % page)
+        kx = norm_rope_f32(host(k[r]).reshape(n, kvh, hd), host(nw) if norm else None,
+                           host(cos[p]) if rot else None, host(sin[p]) if rot else None, inter)
+        for y, codes, scales in ((kx, want[0], want[2]),
+                                 (host(v[r]).reshape(n, kvh, hd), want[1], want[3])):
+            q, sc = int8_f32(y)
+            new = codes[at]
+            new[:, :kvh * hd] = torch.from_numpy(q.reshape(n, -1)).cuda()
+            codes[at] = new
+            new = scales[at]
+            new[:, :kvh] = torch.from_numpy(sc).cuda()
+            scales[at] = new
+    for got, exp in zip((P.k, P.v, P.ks, P.vs), want):
+        assert torch.equal(got, exp)                  # everything else as it was, too
+
+
+def test_append_refuses_on_the_device(ops, q3, request):
+    """Rows that do not fit are skipped, the others written."""
+    request.node.keywords["status"] = True
+    P = Pool(ops, [(2, 40), (2, 10), (2, 64), (2, 33)], 2, 64, seed=4)
+    P.kv_len.copy_(torch.tensor([1, 10, 65, 33]))      # fewer tokens than rows; beyond the table
+    P.tables[3, 0] = -1                                # page 65535: beyond the pool
+    k = torch.randn(P.rows, 128, device="cuda", generator=gen(1))
+    before = [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+    cos, sin = tables_f32(64, 64)
+    ops.paged_kv_append_batch(k, k, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 4, 2, 64,
+                              cos=cos, sin=sin)
+    assert q3._lib.lib().q3_device_status() == (1 << 5) | (1 << 2) | (1 << 1)
+    changed = {(int(a), int(b)) for a, b in (P.ks != before[2]).any(-1).nonzero()}
+    tab = (P.tables.long() & 0xFFFF).tolist()
+    # sequence 0: position 0 of its second row; 1: both; 2: position 63; 3: position 32
+    assert changed == {(tab[0][0], 0), (tab[1][0], 8), (tab[1][0], 9), (tab[2][1], 31),
+                       (tab[3][1], 0)}
+
+
+# ---------------------------------------------------------------- attention
+def ref_attention(P, q, heads, causal, window, scale):
+    """q float64 [rows][heads][hd] -> o, and what bounds its error: sum of weight |v|, the largest
+    logit's sum of |terms| (base 2) and the part of weights below f16's normal range."""
+    grp = heads // P.kvh
+    o = torch.zeros(P.rows, heads, P.hd, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(o)
+    for s, (n, kv) in enumerate(P.lens):
+        if not n:
+            continue
+        r = int(P.row0[s])
+        (k8, ks), (v8, vs) = P.cached(s)
+        k, v = k8 * ks[..., None], v8 * vs[..., None]
+        qq = q[r:r + n].reshape(n, P.kvh, grp, P.hd)
+        t = torch.einsum("nkgd,jkd->nkgj", qq, k) * scale
+        big = torch.einsum("nkgd,jkd->nkgj", qq.abs(), k.abs()).amax(-1, keepdim=True) * scale
+        j, p = torch.arange(kv, device="cuda"), torch.arange(kv - n, kv, device="cuda")[:, None]
+        see = (j <= p) if causal else torch.ones(n, kv, dtype=torch.bool, device="cuda")
+        if window:
+            see = see & (j > p - window)
+        t.masked_fill_(~see[:, None, None], -math.inf)
+        w = torch.softmax(t, -1)
+        o[r:r + n] = torch.einsum("nkgj,jkd->nkgd", w, v).reshape(n, heads, P.hd)
+        a = torch.einsum("nkgj,jkd->nkgd", w, v.abs())
+        rel = 2.0 ** -11 + 2 * 2.0 ** -20 * (big * 1.4427 + 8)
+        low = 2.0 ** -25 * (w * vs.T[None, :, None]).amax(-1, keepdim=True) * \
+            (v8.abs().sum(0)[None, :, None])
+        tol[r:r + n] = (rel * a + low).reshape(n, heads, P.hd)
+    return o, tol
+
+
+def make_q(P, heads, qtype, seed, rows=None, spread=1.5):
+    g = gen(seed)
+    rows = P.rows if rows is None else rows
+    x = torch.randn(rows, heads, P.hd, device="cuda", generator=g) * spread
+    if qtype == "i8":
+        qs = x.abs().amax(-1) / 127
+        c = (x / qs[..., None]).round().clamp(-127, 127).to(torch.int8)
+        return c.reshape(rows, -1), qs.contiguous(), c.double() * qs.double()[..., None]
+    x = x.to(TYPES[qtype])
+    return x.reshape(rows, -1), None, x.double()
+
+
+def check_rows(got, os, want, tol, heads, hd, rows):
+    if got.dtype == torch.int8:
+        assert got.shape[1] >= heads * hd
+        c = got[:rows, :heads * hd].reshape(rows, heads, hd).double()
+        sc = os[:rows, :heads].double()
+        top = want.abs().amax(-1)
+        assert ((sc * 127 - top).abs() <= tol.amax(-1) + 3 * 2.0 ** -24 * top).all()
+        assert c.abs().max() <= 127
+        lim = tol + sc[..., None] * (0.5 + 2.0 ** -15)
+        assert ((c * sc[..., None] - want).abs() <= lim).all()
+    else:
+        o = got[:rows].reshape(rows, heads, hd).double()
+        lim = tol + half_step(got.dtype) * (want.abs() + tol) + \
+            torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+        assert ((o - want).abs() <= lim).all(), float(((o - want).abs() / lim).max())
+
+
+def run_attention(ops, P, heads, qtype, otype, causal=True, window=0, seed=1, scale=None,
+                  workspace=None, stream=None, spread=1.5):
+    scale = P.hd ** -0.5 if scale is None else scale
+    q, qs, q64 = make_q(P, heads, qtype, seed, spread=spread)
+    dt = torch.int8 if otype == "i8" else TYPES[otype]
+    o = torch.full((P.rows + 2, heads * P.hd), 7, device="cuda", dtype=dt)
+    os = torch.full((P.rows + 2, heads), 7.0, device="cuda") if otype == "i8" else None
+    ops.attention_chunk_batch(q, qs, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len,
+                              len(P.lens), P.max_rows, o, os, heads, P.kvh, P.hd, causal, window,
+                              scale, workspace=workspace, stream=stream)
+    want, tol = ref_attention(P, q64, heads, causal, window, scale)
+    check_rows(o, os, want, tol, heads, P.hd, P.rows)
+    assert (o[P.rows:] == 7).all() and (os is None or (os[P.rows:] == 7).all())
+    return o
+
+
+SHAPES = [
+    # heads, kv heads, head_dim, page, (new rows, tokens) per sequence
+    (16, 8, 128, 32, [(1, 1), (1, 33), (1, 64), (0, 7), (1, 200), (1, 129)]),
+    (16, 8, 128, 32, [(5, 5), (3, 300), (0, 0), (8, 41)]),
+    (8, 1, 128, 32, [(1, 77), (2, 160)]),
+    (12, 4, 64, 32, [(5, 1000), (1, 3), (4, 4)]),
+    (5, 1, 64, 16, [(3, 50), (7, 100)]),
+    (16, 1, 128, 7, [(1, 30), (3, 45)]),
+    (4, 4, 64, 128, [(1, 400), (9, 129)]),
+    (2, 1, 128, 32, [(130, 130), (67, 200), (1, 64)]),
+    (4, 2, 128, 32, [(64, 1000), (257, 257), (300, 777)]),
+    (6, 2, 64, 32, [(200, 431), (45, 45), (2, 900)]),
+    (3, 3, 128, 64, [(129, 640)]),
+]
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 50), (False, 0), (True, 1)])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention_shapes(ops, shape, causal, window):
+    heads, kvh, hd, page, lens = SHAPES[shape]
+    P = Pool(ops, lens, kvh, hd, page, seed=shape)
+    qt = ("i8", "f16", "bf16")[shape % 3]
+    run_attention(ops, P, heads, qt, ("f16", "bf16", "i8")[(shape // 3 + window) % 3], causal,
+                  window, seed=shape)
+
+
+@pytest.mark.parametrize("qtype", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("otype", ["i8", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [[(1, 90), (2, 2)], [(150, 200), (40, 999)]])
+def test_attention_types(ops, qtype, otype, hd, lens):
+    run_attention(ops, Pool(ops, lens, 2, hd, seed=hd), 4, qtype, otype)
+
+
+@pytest.mark.parametrize("heads,kvh,hd,lens", [
+    (16, 8, 128, [(1, 20000)]), (8, 2, 64, [(4, 9000), (1, 31)]), (4, 1, 128, [(1, 7), (6, 30001)]),
+    (4, 2, 128, [(100, 12345)]), (2, 2, 64, [(300, 9999), (1, 50)])])
+def test_attention_long(ops, heads, kvh, hd, lens):
+    """Few rows over many keys: the key range is split and joined."""
+    P = Pool(ops, lens, kvh, hd, seed=9)
+    n = ops.attention_chunk_workspace_bytes(P.rows, len(lens), P.max_rows, P.mp * 32, heads, kvh, hd)
+    ws = torch.full((max(n, 16),), 0xFF, dtype=torch.uint8, device="cuda")       # NaN to begin with
+    a = run_attention(ops, P, heads, "bf16", "bf16", workspace=ws)
+    assert torch.equal(a, run_attention(ops, P, heads, "bf16", "bf16"))  # and repeatable
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_uneven_scales(ops, new):
+    """Scales of K and V over ten binades, zero V scales, sharp softmax: the weights stay relative
+    to each row's largest contribution."""
+    P = Pool(ops, [(new, 700), (new, 333)], 2, 128, seed=21)
+    e = torch.randint(-10, 1, P.vs.shape, device="cuda", generator=gen(2))
+    P.vs.mul_(torch.exp2(e.float()))
+    P.ks.mul_(torch.exp2(torch.randint(-5, 1, P.ks.shape, device="cuda", generator=gen(3)).float()))
+    zero = torch.rand(P.vs.shape, device="cuda", generator=gen(5)) < 0.1
+    P.vs.masked_fill_(zero, 0.0)
+    P.v.view(*P.v.shape[:2], 2, 128).masked_fill_(zero[..., None], 0)
+    run_attention(ops, P, 4, "f16", "f16", spread=6.0)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -90, 2.0 ** 70])
+def test_attention_tiny_and_huge_queries(ops, scale):
+    """bf16 queries far outside f16's range: the row's power of two brings them back."""
+    P = Pool(ops, [(3, 100), (140, 140)], 1, 64, seed=6)
+    q, _, q64 = make_q(P, 2, "bf16", 3)
+    q, q64 = (q.float() * scale).to(torch.bfloat16), q64 * scale
+    o = torch.empty(P.rows, 128, device="cuda", dtype=torch.bfloat16)
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 140, o,
+                              None, 2, 1, 64, True, 0, 0.125 / scale)
+    want, tol = ref_attention(P, q64, 2, True, 0, 0.125 / scale)
+    check_rows(o, None, want, tol, 2, 64, P.rows)
+
+
+@pytest.mark.parametrize("new", [2, 140])
+def test_attention_garbage_behind_the_mask(ops, new):
+    """NaN and infinite scales of tokens that a row does not see leave it alone; a row that sees a
+    NaN is NaN, and no other."""
+    P = Pool(ops, [(new, 150), (new, 161)], 2, 128, seed=8, spare=2)
+    tab = P.tables.long() & 0xFFFF
+    for s in range(2):
+        kv = P.lens[s][1]
+        for j in range(kv, tab.shape[1] * 32):         # behind the last token, spare pages too
+            P.ks[tab[s, j // 32], j % 32] = float("nan") if j % 2 else float("inf")
+            P.vs[tab[s, j // 32], j % 32] = float("inf") if j % 3 else float("nan")
+    P.tables[0, -1] = -1                               # a page index beyond the pool, not needed
+    o = run_attention(ops, P, 4, "i8", "f16")
+    q, qs, q64 = make_q(P, 4, "i8", 1)
+    last = P.lens[0][1] - 1                            # the last token of sequence 0
+    for arr in (P.ks, P.vs):
+        keep = arr[tab[0, last // 32], last % 32].clone()
+        arr[tab[0, last // 32], last % 32] = float("nan")
+        got = torch.empty_like(o)
+        ops.attention_chunk_batch(q, qs, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, new,
+                                  got, None, 4, 2, 128, True, 0, 128 ** -0.5)
+        arr[tab[0, last // 32], last % 32] = keep
+        assert got[new - 1].isnan().all()
+        rest = [r for r in range(P.rows) if r != new - 1]
+        assert torch.equal(got[rest], o[rest])
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_attention_refuses_on_the_device(ops, q3, request, new):
+    """Sequences whose arrays do not fit are skipped; keys in pages beyond the pool are not seen; a
+    row that sees no key gives zeros."""
+    request.node.keywords["status"] = True
+    P = Pool(ops, [(new, 150), (new, 150), (new, 160), (new, 150)], 2, 128, seed=8)
+    q, qs, q64 = make_q(P, 4, "f16", 1)
+    want, tol = ref_attention(P, q64, 4, True, 0, 128 ** -0.5)
+    P.tables[3] = -1
+    P.kv_len[0] = new - 1
+    P.kv_len[2] = P.mp * 32 + 1
+    o = torch.full((P.rows, 512), 7.0, device="cuda", dtype=torch.float16)
+    call = lambda mr: ops.attention_chunk_batch(                                   # noqa: E731
+        q, qs, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 4, mr, o, None, 4, 2, 128, True,
+        0, 128 ** -0.5)
+    call(new)
+    assert q3._lib.lib().q3_device_status() == (1 << 5) | (1 << 2) | (1 << 1)
+    assert (o[:new] == 7).all() and (o[2 * new:3 * new] == 7).all()
+    assert (o[3 * new:] == 0).all()
+    lim = tol + 2.0 ** -11 * (want.abs() + tol)
+    err = (o.double().reshape(-1, 4, 128) - want).abs()
+    assert (err[new:2 * new] <= lim[new:2 * new]).all()
+    if new > 1:                                        # more rows than max_rows
+        o.fill_(7.0)
+        call(new - 1)
+        assert q3._lib.lib().q3_device_status() & (1 << 5)
+        assert (o == 7).all()
+
+
+def test_attention_strided_views(ops):
+    P = Pool(ops, [(3, 70), (140, 300)], 2, 128, seed=5, pad_heads=3)
+    q, _, q64 = make_q(P, 4, "f16", 2)
+    wide = torch.zeros(P.rows, 3 * 512, device="cuda", dtype=torch.float16)
+    wide[:, 512:1024] = q
+    out = torch.full((P.rows, 3 * 512), 7.0, device="cuda", dtype=torch.bfloat16)
+    ops.attention_chunk_batch(wide[:, 512:1024], None, P.kv, P.n_pages, P.tables, P.mp, P.row0,
+                              P.kv_len, 2, 140, out[:, 512:1024], None, 4, 2, 128, True, 0,
+                              128 ** -0.5)
+    want, tol = ref_attention(P, q64, 4, True, 0, 128 ** -0.5)
+    check_rows(out[:, 512:1024], None, want, tol, 4, 128, P.rows)
+    assert (out[:, :512] == 7).all() and (out[:, 1024:] == 7).all()
+
+
+def test_attention_far_pages(ops):
+    """A pool over 4 GB: byte offsets of its last pages pass 32 bits."""
+    P = Pool(ops, [(1, 64), (130, 130)], 2, 128, seed=5)
+    n, page_bytes = P.n_pages, 131072                  # 8 KB of each page used
+    last = 40000 - n
+    assert last * page_bytes > 2 ** 32
+    kv2 = type(P.kv).from_buffer_copy(P.kv)
+    bufs = []
+    for src, sc in ((P.k, P.ks), (P.v, P.vs)):
+        b = torch.empty(40000 * page_bytes, dtype=torch.int8, device="cuda")
+        at = torch.as_strided(b, (n, 32 * 256), (page_bytes, 1), last * page_bytes)
+        at.copy_(src.view(n, -1))
+        s2 = torch.empty(last + n, 32, 2, device="cuda")
+        s2[last:] = sc
+        bufs.append((b, s2))
+    kv2.k, kv2.v = bufs[0][0].data_ptr(), bufs[1][0].data_ptr()
+    kv2.ks, kv2.vs = bufs[0][1].data_ptr(), bufs[1][1].data_ptr()
+    kv2.page_bytes = page_bytes
+    tables = ((P.tables.long() & 0xFFFF) + last).to(torch.int32)
+    tables = torch.where(tables > 32767, tables - 65536, tables).to(torch.int16)
+    assert last + n <= 65536
+    q, _, q64 = make_q(P, 4, "f16", 2)
+    o = torch.empty(P.rows, 512, device="cuda", dtype=torch.float16)
+    ops.attention_chunk_batch(q, None, kv2, last + n, tables, P.mp, P.row0, P.kv_len, 2, 130, o,
+                              None, 4, 2, 128, True, 0, 128 ** -0.5)
+    want, tol = ref_attention(P, q64, 4, True, 0, 128 ** -0.5)
+    check_rows(o, None, want, tol, 4, 128, P.rows)
+
+
+# ------------------------------------------------------------ used together
+def test_step_matches_the_fused_epilogues(ops):
+    """norm + rotation + codes of the separate operators are the bits of the projections' epilogue,
+    and the pages those of the scatter; then attention and the output projection on its codes."""
+    from oracle import q3_oracle as O
+    rng = np.random.default_rng(4)
+    rows, heads, kvh, hd, hid = 21, 16, 8, 128, 512
+    P = Pool(ops, [(rows, 85)], kvh, hd, seed=3)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()               # noqa: E731
+    a = dev(rng.integers(-127, 128, (rows, hid)).astype(np.int8))
+    a_s = dev(rng.uniform(1e-3, 1e-2, (rows, hid // 256)).astype(F))
+    cos, sin = tables_f32(96, 128)
+    start = 85 - rows
+    pos = torch.arange(start, 85, dtype=torch.int32, device="cuda")
+    out = {}
+    for name, n in (("q", heads), ("k", kvh), ("v", kvh)):
+        w = dev(rng.integers(-127, 128, (n * hd, hid)).astype(np.int8))
+        ws = dev(rng.uniform(1e-3, 1e-2, n * hd).astype(F))
+        nw = dev(rng.uniform(0.5, 1.5, hd).astype(F))
+        x = torch.empty(rows, n * hd, device="cuda")
+        ops.gemm_nt_group_store(a, a_s, w, ws, x, 256)
+        c8 = torch.empty(rows, n * hd, dtype=torch.int8, device="cuda")
+        cs = torch.empty(rows, n, device="cuda")
+        if name == "v":
+            ops.gemm_nt_group_store(a, a_s, w, ws, None, 256, q8=c8, qs=cs)
+        else:
+            ops.gemm_nt_group_store(a, a_s, w, ws, None, 256, q8=c8, qs=cs, nw=nw,
+                                    cos=cos[start:85], sin=sin[start:85], inv_hd=1 / 128)
+        out[name] = (x, nw, c8, cs)
+    q8 = torch.empty_like(out["q"][2])
+    qs = torch.empty_like(out["q"][3])
+    ops.rope_rows(out["q"][0], pos, cos, sin, q8, heads, hd, nw=out["q"][1], scale=qs)
+    assert torch.equal(q8, out["q"][2]) and torch.equal(qs, out["q"][3])
+    other = [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+    kv2 = ops.paged_kv(*other, P.tables, kvh, hd, 32)
+    ops.paged_kv_scatter(out["k"][2], out["v"][2], out["k"][3], out["v"][3], kv2, start, rows,
+                         kvh * hd, kvh)
+    ops.paged_kv_append_batch(out["k"][0], out["v"][0], P.kv, P.n_pages, P.tables, P.mp, P.row0,
+                              P.kv_len, 1, kvh, hd, nw=out["k"][1], cos=cos, sin=sin)
+    for x, y in zip((P.k, P.v, P.ks, P.vs), other):
+        assert torch.equal(x, y)
+    o8 = torch.empty(rows, heads * hd, dtype=torch.int8, device="cuda")
+    os = torch.empty(rows, heads, device="cuda")
+    ops.attention_chunk_batch(q8, qs, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 1, rows,
+                              o8, os, heads, kvh, hd, True, 0, hd ** -0.5)
+    q64 = q8.view(rows, heads, hd).double() * qs.double()[..., None]
+    want, tol = ref_attention(P, q64, heads, True, 0, hd ** -0.5)
+    check_rows(o8, os, want, tol, heads, hd, rows)
+    wo = dev(rng.integers(-127, 128, (hid, heads * hd)).astype(np.int8))
+    wos = dev(rng.uniform(1e-3, 1e-2, hid).astype(F))
+    y = torch.empty(rows, hid, device="cuda")
+    ops.gemm_nt_group_store(o8, os, wo, wos, y, 128)
+    ref = O.gemm_group(o8.cpu().numpy(), os.cpu().numpy(), wo.cpu().numpy(), wos.cpu().numpy(), 128)
+    assert np.array_equal(y.cpu().numpy(), ref)
+
+
+def test_captured_step_replays_with_new_lengths(ops):
+    """Tables, append and attention of a step in one graph; lengths, rows and tables change between
+    replays, on another stream than the arrays were made on."""
+    heads, kvh, hd = 4, 2, 128
+    P = Pool(ops, [(1, 40), (1, 700), (1, 9)], kvh, hd, seed=7)
+    x = {n: torch.randn(3, h * hd, device="cuda", generator=gen(h)).half()
+         for n, h in (("q", heads), ("k", kvh), ("v", kvh))}
+    cos, sin = torch.empty(704, 64, device="cuda"), torch.empty(704, 64, device="cuda")
+    pos = P.kv_len - 1
+    q, o = torch.empty_like(x["q"]), torch.empty_like(x["q"])
+    ws = torch.empty(max(16, ops.attention_chunk_workspace_bytes(3, 3, 1, P.mp * 32, heads, kvh, hd)),
+                     dtype=torch.uint8, device="cuda")
+
+    def step():
+        ops.rope_tables(cos, sin, 1e6)
+        ops.rope_rows(x["q"], pos, cos, sin, q, heads, hd)
+        ops.paged_kv_append_batch(x["k"], x["v"], P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len,
+                                  3, kvh, hd, cos=cos, sin=sin)
+        ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 3, 1,
+                                  o, None, heads, kvh, hd, True, 0, hd ** -0.5, workspace=ws)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for lens in ([40, 700, 9], [41, 640, 1], [1, 33, 704]):
+        P.kv_len.copy_(torch.tensor(lens))
+        pos.copy_(torch.tensor(lens) - 1)
+        x["k"].mul_(1.5)
+        saved = [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+        o.zero_()
+        graph.replay()
+        got, pages = o.clone(), [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+        for y, z in zip((P.k, P.v, P.ks, P.vs), saved):
+            y.copy_(z)
+        o.zero_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(o, got)
+        for y, z in zip((P.k, P.v, P.ks, P.vs), pages):
+            assert torch.equal(y, z)
+        P.lens = [(1, n) for n in lens]
+        want, tol = ref_attention(P, q.double().view(3, heads, hd), heads, True, 0, hd ** -0.5)
+        check_rows(got, None, want, tol, heads, hd, 3)
+
+
+def test_attention_stream_argument(ops):
+    P = Pool(ops, [(1, 5000), (100, 300)], 2, 64, seed=5)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    q, _, q64 = make_q(P, 4, "f16", 2)
+    s.wait_stream(torch.cuda.current_stream())
+    o = torch.empty(P.rows, 256, device="cuda", dtype=torch.float16)
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 100, o,
+                              None, 4, 2, 64, True, 0, 0.125, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    want, tol = ref_attention(P, q64, 4, True, 0, 0.125)
+    check_rows(o, None, want, tol, 4, 64, P.rows)
