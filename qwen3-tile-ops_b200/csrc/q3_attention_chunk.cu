@@ -15,6 +15,8 @@
 // bf16 queries are multiplied by a power of two per row, which brings the row's
 // maximum to [2^10, 2^11): their 8 bits then fit f16 exactly down to 2^-24 of
 // the row's maximum, and one f16 path serves all query types.
+#include <atomic>
+
 #include "q3_attention_chunk.h"
 
 namespace q3 {
@@ -69,6 +71,581 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// bf16 rows: 2^up brings the row's maximum m to [2^10, 2^11) (zero, subnormal or infinite m: the
+// nearest exponent in range); `down` is its inverse.
+__device__ __forceinline__ void bf16_scale(float m, float &up, float &down) {
+  const int ex = static_cast<int>(__float_as_uint(m) >> 23);
+  const int e = min(max(137 - ex, -120), 110);
+  up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+}
+
+// One head of a result row (whole warp, lane: columns lane*N ..) to o / os.
+template <int N>
+__device__ __forceinline__ void store_out(const Args &p, long r, int h, int lane, float (&x)[N]) {
+  constexpr int HD = 32 * N;
+  char *o = p.o + r * p.o_rb;
+  const long col = static_cast<long>(h) * HD + lane * N;
+  if (p.o_dt == Q3_DT_F16) store_row<__half, N>(x, o + col * 2);
+  else if (p.o_dt == Q3_DT_BF16) store_row<__nv_bfloat16, N>(x, o + col * 2);
+  else {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    const float scale = __fmul_rn(warp_tree_max(m), kInv127);
+    int c[N];
+    quant_n_absmax<N>(x, scale, c);
+    Elems<int8_t, N> e;
+#pragma unroll
+    for (int i = 0; i < N; ++i) e.e[i] = static_cast<int8_t>(c[i]);
+    e.store(o + col);
+    if (lane == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: sequences with at most 8 NT packed rows (packed row m is head m %
+// group of new row m / group of the sequence).  A unit of work is one 32-key block
+// of a (sequence, KV head) pair; the units of the whole batch, in order, are dealt to the
+// warps of one resident wave in equal runs, so ragged lengths and any number of
+// pairs fill the card evenly.  A warp works alone: it keeps the running maximum and
+// sums of its run of a pair and stores the result when it has the whole pair, else
+// a part (at most two a warp: its first and its last pair) that k_attn_join joins.
+//
+// Keys are the M side of the products (S^T = K8 q^T, o^T = V8^T p^T), so a decode
+// step with a group of 2 wastes 6 of 8 columns instead of 14 of 16 rows.  A warp
+// keeps STAGES blocks in shared memory or on their way there (cp.async); a fragment
+// is built from 16-byte reads of codes, since the contraction over d and the rows of
+// o^T may be permuted freely.  Reading the cache once is the bound.
+// ---------------------------------------------------------------------------
+constexpr int WARPS = 4;
+constexpr int KB = 32;                             // keys of a block
+constexpr int MIN_UNITS = 4;                       // least run of a warp
+
+template <int HD>
+struct FewStage {
+  static constexpr int STAGES = HD == 128 ? 2 : 4;
+  uint4 k[KB * HD / 16], v[KB * HD / 16];
+  float ks[KB], vs[KB];
+};
+
+// Units of a pair of sequence s (0: not this kernel's) and its first block
+__device__ __forceinline__ int pair_units(const Args &p, const Seq &s, int &b0) {
+  b0 = 0;
+  if (!s.ok || s.n * p.group > p.few_rows) return 0;
+  int lo, hi;
+  key_range(p, s, s.pos0, s.kv - 1, lo, hi);
+  b0 = lo / KB;
+  return (hi + KB - 1) / KB - b0;
+}
+
+// Where units lie (whole warp).  total: all units; with `unit` inside, s is its sequence and
+// `before` the units of the sequences before it.
+struct Place {
+  long total, before;
+  int s;
+};
+__device__ __forceinline__ long units_of(const Args &p, int s, unsigned *err) {
+  if (s >= p.n_seqs) return 0;
+  int b0;
+  return static_cast<long>(pair_units(p, load_seq(p, s, err), b0)) * p.kv_heads;
+}
+__device__ __forceinline__ long warp_sum(long x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ long count_units(const Args &p, int n, int lane, unsigned *err) {
+  long x = 0;
+  for (int s = lane; s < n; s += 32) x += units_of(p, s, err);
+  return warp_sum(x);
+}
+__device__ __forceinline__ int find_unit(const Args &p, long unit, int lane, long &before) {
+  unsigned err = 0;
+  before = 0;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const long mine = units_of(p, s0 + lane, &err);
+    long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, before + upto > unit);
+    if (m) {
+      const int l = __ffs(m) - 1;
+      before += __shfl_sync(0xffffffffu, upto - mine, l);
+      return s0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return -1;
+}
+// workers that share `total` units of a grid of `all` warps, and the first unit of worker w
+__device__ __forceinline__ long workers(long total, long all) {
+  const long n = (total + MIN_UNITS - 1) / MIN_UNITS;
+  return n < all ? n : all;
+}
+__device__ __forceinline__ long first_unit(long total, long n, long w) { return total * w / n; }
+
+// 16 (HD 64: 8) columns at g * HD/8 of one row head, a row spread over the 8 lanes of equal t4
+template <int N>
+__device__ __forceinline__ void store_part8(const Args &p, long r, int h, int g, bool ok,
+                                            float (&x)[N]) {
+  constexpr int HD = 8 * N;
+  const long col = static_cast<long>(h) * HD + g * N;
+  char *o = p.o + r * p.o_rb;
+  if (p.o_dt == Q3_DT_I8) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    const float scale = __fmul_rn(m, kInv127);
+    uint32_t c[N / 4];
+    quant_pack_absmax<N>(x, scale, c);
+    if (!ok) return;
+    Elems<int8_t, N> e;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint32_t *>(e.e)[i] = c[i];
+    e.store(o + col);
+    if (g == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
+  } else if (ok) {
+    if (p.o_dt == Q3_DT_F16) store_row<__half, N>(x, o + col * 2);
+    else store_row<__nv_bfloat16, N>(x, o + col * 2);
+  }
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0)
+               : "memory");
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const Args p) {
+  constexpr int KW = HD / 16, VW = HD / 32;   // k16 steps; words of a thread's V bytes
+  constexpr int CH = HD / 16;                 // 16-byte chunks of a row
+  using Stage = FewStage<HD>;
+  constexpr int STAGES = Stage::STAGES;
+  extern __shared__ __align__(128) char smem[];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  Stage *ring = reinterpret_cast<Stage *>(smem) + wid * STAGES;
+  const long w = static_cast<long>(blockIdx.x) * WARPS + wid;
+
+  unsigned err = 0;
+  const long total = count_units(p, p.n_seqs, lane, &err);
+  if (w == 0 && err) atomicOr(&g_chunk_error, err);
+  const long nw = workers(total, static_cast<long>(gridDim.x) * WARPS);
+  if (w < nw) {
+    long u = first_unit(total, nw, w);
+    const long u1 = first_unit(total, nw, w + 1);
+    long before;
+    int s = find_unit(p, u, lane, before);
+    while (u < u1 && s >= 0) {
+      // the pair of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
+      const Seq q = load_seq(p, s, &err);
+      int pb0;
+      const int pn = pair_units(p, q, pb0);
+      if (pn == 0) {
+        ++s;
+        continue;
+      }
+      const int kvh = static_cast<int>((u - before) / pn);
+      const int off = static_cast<int>((u - before) % pn);
+      const int b = pb0 + off;
+      const int run = static_cast<int>(u1 - u < pn - off ? u1 - u : pn - off);
+      const int be = b + run;
+      const bool whole = off == 0 && run == pn;
+      const int packed = q.n * p.group;
+
+      const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
+      const long kcol = static_cast<long>(kvh) * HD;
+      // table index and slot of key x*32 + lane; its page is requested one step before it is used
+      auto page_of = [&](int x) -> int {
+        const int j = x * KB + lane;
+        return x < be && j < q.kv ? table[page_index(p, j)] : -1;
+      };
+      auto fetch = [&](int x, int pg) {   // block x into its stage
+        const int j = x * KB + lane;
+        bool ok = pg >= 0;
+        if (ok && static_cast<uint32_t>(pg) >= p.num_pages) {
+          atomicOr(&g_chunk_error, kBadPage);
+          ok = false;
+        }
+        const uint32_t at =
+            ok ? (static_cast<uint32_t>(pg) << 16) | page_slot(p, j)
+               : 0xffffffffu;
+        Stage &st = ring[x % STAGES];
+        const uint32_t kd = static_cast<uint32_t>(__cvta_generic_to_shared(st.k)),
+                       vd = static_cast<uint32_t>(__cvta_generic_to_shared(st.v));
+        if (x < be) {
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            const int row = i * (32 / CH) + lane / CH, c = lane % CH;
+            const uint32_t ra = __shfl_sync(0xffffffffu, at, row);
+            const bool rok = ra != 0xffffffffu;
+            const size_t src = rok ? static_cast<size_t>(ra >> 16) * p.page_bytes +
+                                         static_cast<size_t>(ra & 0xffffu) * p.row_bytes + kcol +
+                                         c * 16
+                                   : 0;
+            // places that make the fragment reads conflict-free (see there)
+            const int line = HD == 128 ? row : row >> 1, lc = HD == 128 ? c : (row & 1) * 4 + c;
+            const int kc = HD == 128 ? lc ^ ((row & 1) << 2) : lc;
+            const int vc = HD == 128 ? lc ^ (row & 6) : lc ^ ((line & 3) << 1);
+            cp16(kd + (line * 8 + kc) * 16, p.k + src, rok);
+            cp16(vd + (line * 8 + vc) * 16, p.v + src, rok);
+          }
+          const size_t so = ok ? static_cast<size_t>(at >> 16) * p.scale_page_bytes +
+                                     static_cast<size_t>(at & 0xffffu) * p.scale_row_bytes + kvh * 4
+                               : 0;
+          cp4(static_cast<uint32_t>(__cvta_generic_to_shared(st.ks + lane)), p.ks + so, ok);
+          cp4(static_cast<uint32_t>(__cvta_generic_to_shared(st.vs + lane)), p.vs + so, ok);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return __ballot_sync(0xffffffffu, ok);          // keys of the block that exist
+      };
+      int pg[STAGES];
+      unsigned have[STAGES];
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) pg[i] = page_of(b + i);
+
+      // query fragments: column n*8 + g; k16 step x of thread t4 takes the 4 codes of word x of
+      // its chunks (16 bytes at t4*16, and at 64 + t4*16 when HD = 128)
+      uint32_t qf[NT][KW][2];
+      float a[NT][2], mref[NT][2], lsum[NT][2];
+      int pq[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int m = n * 8 + g;
+        float scale = 0.0f;
+#pragma unroll
+        for (int x = 0; x < KW; ++x) qf[n][x][0] = qf[n][x][1] = 0;
+        const int mm = min(m, packed - 1);
+        const long r = q.first + mm / p.group;
+        const int h = kvh * p.group + mm % p.group;
+        const char *qp = p.q + r * p.q_rb;
+        if (p.q_dt == Q3_DT_I8) {
+          if (m < packed) {
+            scale = reinterpret_cast<const float *>(p.qs + r * p.qs_rb)[h];
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {
+              Elems<uint32_t, 4> e;
+              e.load(qp + static_cast<long>(h) * HD + c * 64 + t4 * 16);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t x = e.e[i] ^ 0x80808080u;
+                qf[n][c * 4 + i][0] = f16_pair(x, 0x4140);
+                qf[n][c * 4 + i][1] = f16_pair(x, 0x4342);
+              }
+            }
+          }
+        } else {
+          scale = 1.0f;
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c) {
+            Elems<uint32_t, 8> e;
+            e.load(qp + (static_cast<long>(h) * HD + c * 64 + t4 * 16) * 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              qf[n][c * 4 + i][0] = e.e[2 * i];
+              qf[n][c * 4 + i][1] = e.e[2 * i + 1];
+            }
+          }
+          if (p.q_dt == Q3_DT_BF16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int x = 0; x < KW; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                mx = fmaxf(mx, fabsf(__uint_as_float(qf[n][x][i] << 16)));
+                mx = fmaxf(mx, fabsf(__uint_as_float(qf[n][x][i] & 0xffff0000u)));
+              }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            float up;
+            bf16_scale(mx, up, scale);
+#pragma unroll
+            for (int x = 0; x < KW; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                qf[n][x][i] = pack_f16(__fmul_rn(__uint_as_float(qf[n][x][i] << 16), up),
+                                       __fmul_rn(__uint_as_float(qf[n][x][i] & 0xffff0000u), up));
+          }
+        }
+        scale = __fmul_rn(scale, p.scale_log2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          a[n][j] = __shfl_sync(0xffffffffu, scale, (t4 * 2 + j) * 4);
+          pq[n][j] = q.pos0 + min(n * 8 + t4 * 2 + j, packed - 1) / p.group;
+          mref[n][j] = kNegInf;
+          lsum[n][j] = 0.0f;
+        }
+      }
+      float o[HD / 16][NT][4];
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[i][n][c] = 0.0f;
+
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) have[i] = fetch(b + i, pg[i]);
+      int pnext = pg[STAGES - 1];
+      for (int x = b; x < be; ++x) {
+        const unsigned newest = fetch(x + STAGES - 1, pnext);
+        pnext = page_of(x + STAGES);
+        unsigned mask = have[0];
+#pragma unroll
+        for (int i = 0; i + 2 < STAGES; ++i) have[i] = have[i + 1];
+        have[STAGES - 2] = newest;
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const Stage &st = ring[x % STAGES];
+        // S^T: rows g and g + 8 of the two 16-key tiles
+        float sc[2][NT][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t kw[2][KW];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int row = i * 16 + y * 8 + g;
+#pragma unroll
+            for (int c = 0; c < KW / 4; ++c) {
+              // a quarter warp reads 4 chunks of two rows: the odd row's lie in the other half
+              const int at = HD == 128 ? row * 8 + ((c * 4 + t4) ^ ((row & 1) << 2)) : row * 4 + t4;
+              const uint4 z = st.k[at];
+              kw[y][c * 4] = z.x ^ 0x80808080u, kw[y][c * 4 + 1] = z.y ^ 0x80808080u;
+              kw[y][c * 4 + 2] = z.z ^ 0x80808080u, kw[y][c * 4 + 3] = z.w ^ 0x80808080u;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sc[i][n][c] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < KW; ++c) {
+            const uint32_t af[4] = {f16_pair(kw[0][c], 0x4140), f16_pair(kw[1][c], 0x4140),
+                                    f16_pair(kw[0][c], 0x4342), f16_pair(kw[1][c], 0x4342)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(sc[i][n], af, qf[n][c][0], qf[n][c][1]);
+          }
+        }
+        // t = a ks S + log2 vs, masked; the block's maximum per row
+        float ks[4], lv[4], rv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ks[i] = st.ks[i * 8 + g];
+          const float v = st.vs[i * 8 + g];
+          rv[i] = rcp(fmaxf(v, kVsMin));             // (NaN: fmaxf drops it ...
+          lv[i] = v != v ? v : lg2(fmaxf(v, kVsMin));// ... and the rows that see it get NaN)
+        }
+        const bool masked = mask != 0xffffffffu || x * KB + KB - 1 > q.pos0 || p.window > 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float mx = kNegInf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float &y = sc[i >> 1][n][(i & 1) * 2 + j];
+              y = __fmaf_rn(__fmul_rn(y, ks[i]), a[n][j], lv[i]);
+              if (masked) {
+                const int key = x * KB + i * 8 + g;
+                const bool see = ((mask >> (i * 8 + g)) & 1) && !(p.causal && key > pq[n][j]) &&
+                                 !(p.window > 0 && key <= pq[n][j] - p.window);
+                y = see ? y : kNegInf;
+              }
+              mx = fmaxf(mx, y);
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            // a new reference when the maximum outgrows the old one by 2^8
+            const bool grow = mx > __fadd_rn(mref[n][j], 8.0f);
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? ex2(__fsub_rn(mref[n][j], mx)) : 1.0f;
+              mref[n][j] = grow ? mx : mref[n][j];
+              lsum[n][j] = __fmul_rn(lsum[n][j], f);
+#pragma unroll
+              for (int d = 0; d < HD / 16; ++d) {
+                o[d][n][j] = __fmul_rn(o[d][n][j], f);
+                o[d][n][2 + j] = __fmul_rn(o[d][n][2 + j], f);
+              }
+            }
+            const float base = mref[n][j] == kNegInf ? 0.0f : mref[n][j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float &y = sc[i >> 1][n][(i & 1) * 2 + j];
+              y = ex2(__fsub_rn(y, base));
+              lsum[n][j] = __fmaf_rn(y, rv[i], lsum[n][j]);
+            }
+          }
+        // o^T += V8^T p^T
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t pf[NT][2], vw[4][VW];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            pf[n][0] = transpose8(pack_f16(sc[i][n][0], sc[i][n][1]));
+            pf[n][1] = transpose8(pack_f16(sc[i][n][2], sc[i][n][3]));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // a quarter (HD 64: half) warp reads 2 chunks of rows 0, 2, 4, 6 (+ const)
+            const int row = i * 16 + (j >> 1) * 8 + t4 * 2 + (j & 1);
+            if constexpr (HD == 128) {
+              const uint4 z = st.v[row * 8 + (g ^ (row & 6))];
+              vw[j][0] = z.x, vw[j][1] = z.y, vw[j][2] = z.z, vw[j][3] = z.w;
+            } else {
+              const int line = row >> 1, c = ((row & 1) * 4 + (g >> 1)) ^ ((line & 3) << 1);
+              const uint2 z = reinterpret_cast<const uint2 *>(st.v)[(line * 8 + c) * 2 + (g & 1)];
+              vw[j][0] = z.x, vw[j][1] = z.y;
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < VW; ++c) {
+            // codes of keys (0, 1) and (2, 3) of the thread side by side, by column
+            const uint32_t l01 = __byte_perm(vw[0][c], vw[1][c], 0x5140) ^ 0x80808080u;
+            const uint32_t h01 = __byte_perm(vw[0][c], vw[1][c], 0x7362) ^ 0x80808080u;
+            const uint32_t l23 = __byte_perm(vw[2][c], vw[3][c], 0x5140) ^ 0x80808080u;
+            const uint32_t h23 = __byte_perm(vw[2][c], vw[3][c], 0x7362) ^ 0x80808080u;
+            const uint32_t fl[4] = {f16_pair(l01, 0x4140), f16_pair(l01, 0x4342),
+                                    f16_pair(l23, 0x4140), f16_pair(l23, 0x4342)};
+            const uint32_t fh[4] = {f16_pair(h01, 0x4140), f16_pair(h01, 0x4342),
+                                    f16_pair(h23, 0x4140), f16_pair(h23, 0x4342)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_16816(o[2 * c][n], fl, pf[n][0], pf[n][1]);
+              mma_16816(o[2 * c + 1][n], fh, pf[n][0], pf[n][1]);
+            }
+          }
+        }
+        __syncwarp();   // the stage is read before the next fetch overwrites it
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      // column g*(HD/8) + 2i of o^T in o[i][n][j], + 1 in o[i][n][2 + j], row n*8 + t4*2 + j
+      const long slot = 2 * w + (off == 0 ? 1 : 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float l = lsum[n][j];
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 4));
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 8));
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 16));
+          const int m = n * 8 + t4 * 2 + j;
+          const bool ok = m < packed;
+          float y[HD / 8];
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) {
+            y[2 * i] = o[i][n][j];
+            y[2 * i + 1] = o[i][n][2 + j];
+          }
+          if (whole) {
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);   // no key seen: zeros
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) y[i] = __fmul_rn(y[i], inv);
+            const int mm = min(m, packed - 1);
+            store_part8<HD / 8>(p, q.first + mm / p.group, kvh * p.group + mm % p.group, g, ok, y);
+          } else if (ok) {
+            const long at = slot * p.part_rows + m;
+            Elems<float, HD / 8> e;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) e.e[i] = y[i];
+            e.store(p.part_o + at * HD + g * (HD / 8));
+            if (g == 0) {
+              p.part_ml[at * 2] = mref[n][j];
+              p.part_ml[at * 2 + 1] = l;
+            }
+          }
+        }
+      u += run;
+      if (off + run == pn && kvh + 1 == p.kv_heads) {
+        before += static_cast<long>(pn) * p.kv_heads;
+        ++s;
+      }
+      if (s >= p.n_seqs) break;
+    }
+  }
+  pdl_trigger();
+}
+
+// The parts of one (row, head) joined by a CTA: warps take them in turn.
+template <int HD>
+__global__ void __launch_bounds__(WARPS * 32) k_attn_join(const Args p, long all_workers) {
+  constexpr int N = HD / 32;
+  __shared__ float so[WARPS][HD], sm[WARPS], sl[WARPS];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const long r = blockIdx.x;
+  const int h = blockIdx.y;
+  int first, count;
+  const int s = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
+  if (s < 0) return;
+  unsigned err = 0;
+  const Seq q = load_seq(p, s, &err);
+  int pb0;
+  const int pn = pair_units(p, q, pb0);
+  if (pn == 0) return;                             // refused, or the other kernel's
+  const long before = count_units(p, s, lane, &err);
+  const long total = count_units(p, p.n_seqs, lane, &err);
+  const long nw = workers(total, all_workers);
+  // the pair's units, and the workers that have them
+  const long a = before + static_cast<long>(h / p.group) * pn, b = a + pn;
+  long w0 = a * nw / total, w1 = (b - 1) * nw / total;
+  while (w0 + 1 < nw && first_unit(total, nw, w0 + 1) <= a) ++w0;
+  while (w1 + 1 < nw && first_unit(total, nw, w1 + 1) <= b - 1) ++w1;
+  if (w0 == w1) return;                            // stored whole
+  pdl_wait();
+  const int m = static_cast<int>(r - q.first) * p.group + h % p.group;
+  float mm = kNegInf, l = 0.0f, x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = 0.0f;
+  for (long w = w0 + wid; w <= w1; w += WARPS) {
+    const long slot = 2 * w + (first_unit(total, nw, w) <= a ? 1 : 0);
+    const long at = slot * p.part_rows + m;
+    const float pm = p.part_ml[at * 2], pl = p.part_ml[at * 2 + 1];
+    Elems<float, N> e;
+    e.load(p.part_o + at * HD + lane * N);
+    const float top = fmaxf(mm, pm), base = top == kNegInf ? 0.0f : top;
+    const float f0 = ex2(__fsub_rn(mm, base)), f1 = ex2(__fsub_rn(pm, base));
+    mm = top;
+    l = __fmaf_rn(f1, pl, __fmul_rn(f0, l));
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f1, e.e[i], __fmul_rn(f0, x[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) so[wid][lane * N + i] = x[i];
+  if (lane == 0) sm[wid] = mm, sl[wid] = l;
+  __syncthreads();
+  if (wid) return;
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, sm[i]);
+  const float base = top == kNegInf ? 0.0f : top;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < WARPS; ++k) {
+    const float f = ex2(__fsub_rn(sm[k], base));
+    l = __fmaf_rn(f, sl[k], l);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f, so[k][lane * N + i], x[i]);
+  }
+  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = __fmul_rn(x[i], inv);
+  store_out<N>(p, r, h, lane, x);
+}
+
 // One query row of a tile into shared memory as f16 (whole warp), and its a_i.
 template <int HD>
 __device__ __forceinline__ float stage_q(const Args &p, long r, int h, int lane, __half *dst) {
@@ -102,46 +679,9 @@ __device__ __forceinline__ float stage_q(const Args &p, long r, int h, int lane,
   return __fmul_rn(p.scale_log2, __uint_as_float(static_cast<uint32_t>(127 - up) << 23));
 }
 
-// One head of a result row (whole warp, lane: columns lane*N ..) to o / os.
-template <int N>
-__device__ __forceinline__ void store_out(const Args &p, long r, int h, int lane, float (&x)[N]) {
-  constexpr int HD = 32 * N;
-  char *o = p.o + r * p.o_rb;
-  const long col = static_cast<long>(h) * HD + lane * N;
-  if (p.o_dt == Q3_DT_F16) store_row<__half, N>(x, o + col * 2);
-  else if (p.o_dt == Q3_DT_BF16) store_row<__nv_bfloat16, N>(x, o + col * 2);
-  else {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
-    const float scale = __fmul_rn(warp_tree_max(m), kInv127);
-    int c[N];
-    quant_n_absmax<N>(x, scale, c);
-    Elems<int8_t, N> e;
-#pragma unroll
-    for (int i = 0; i < N; ++i) e.e[i] = static_cast<int8_t>(c[i]);
-    e.store(o + col);
-    if (lane == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Few rows.  CTA = (sequence, tile of 8 NT packed rows, KV head, part of the
-// keys); packed row m is head m % group of new row m / group.  The warps take
-// 32-key blocks in turn, each with its own running maximum and sums, merged in
-// shared memory at the end.
-//
-// Keys are the M side of the products (S^T = K8 q^T, o^T = V8^T p^T), so a decode
-// step with a group of 2 wastes 6 of 8 columns instead of 14 of 16 rows, and a
-// thread's fragment is built from 16-byte global loads without shared memory:
-// the contraction over d and the rows of o^T may be permuted freely, so a thread
-// takes the bytes it loaded.  Reading K8, V8 once is the bound.
-// ---------------------------------------------------------------------------
-constexpr int WARPS = 4;
-constexpr int KB = 32;                             // keys of a block
 
 template <int HD, int NT>
-struct FewSmem {
+struct TileSmem {
   static constexpr int Q = 8 * NT;                 // packed rows
   static constexpr int OS = HD + 4;                // row stride of the merged sums
   static constexpr int bytes =
@@ -149,10 +689,10 @@ struct FewSmem {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32) k_attn_few(const Args p) {
-  using S = FewSmem<HD, NT>;
+__global__ void __launch_bounds__(WARPS * 32) k_attn_tiles(const Args p) {
+  using S = TileSmem<HD, NT>;
   constexpr int Q = S::Q, KW = HD / 16, VW = HD / 32;   // k16 steps; words of a thread's V bytes
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];
   __half *sq = reinterpret_cast<__half *>(smem);                   // [Q][HD]
   float *sa = reinterpret_cast<float *>(smem + Q * HD * 2);        // [Q]
   float *sml = sa + Q;                                             // [WARPS][Q][2]
@@ -165,7 +705,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_attn_few(const Args p) {
   if (err && threadIdx.x == 0) atomicOr(&g_chunk_error, err);
   const int packed = sq_.n * p.group;
   const int m0 = tile * Q;
-  if (!sq_.ok || m0 >= packed) return;
+  if (!sq_.ok || m0 >= packed || packed <= p.few_rows) return;
   const int mq = min(Q, packed - m0);
   // positions of the tile's rows, its key blocks and this part's
   const int p0 = sq_.pos0 + m0 / p.group, p1 = sq_.pos0 + (m0 + mq - 1) / p.group;
@@ -431,7 +971,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_attn_few(const Args p) {
 
 // The parts of a row head joined (one warp each).
 template <int HD>
-__global__ void k_attn_join(const Args p) {
+__global__ void k_join_tiles(const Args p) {
   constexpr int N = HD / 32;
   const int lane = threadIdx.x & 31;
   const long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -442,7 +982,8 @@ __global__ void k_attn_join(const Args p) {
   const int s = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
   if (s < 0) return;
   unsigned err = 0;
-  if (!load_seq(p, s, &err).ok) return;
+  const Seq q = load_seq(p, s, &err);
+  if (!q.ok || q.n * p.group <= p.few_rows) return;
   float mm = kNegInf, l = 0.0f, x[N];
   for (int z = 0; z < p.splits; ++z)
     mm = fmaxf(mm, p.part_ml[((static_cast<long>(z) * p.rows + r) * p.heads + h) * 2]);
@@ -462,21 +1003,39 @@ __global__ void k_attn_join(const Args p) {
   store_out<N>(p, r, h, lane, x);
 }
 
-// How a call is cut: query tiles of 8*nt packed rows, parts of the key range
+// How a call is cut.  Sequences with at most few_rows packed rows go to k_attn_few (nt tiles of 8),
+// the others to the tile kernel.
 struct Plan {
-  int nt, tiles, splits;
+  int nt, few_rows, few_ctas;                      // few_ctas 0: no such sequence can be there
+  int tiles, splits;                               // tiles 0: likewise
+  size_t few_slots, bytes;                         // parts of k_attn_few; the whole workspace
 };
 static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_t max_kv,
-                      uint32_t heads, uint32_t kv_heads) {
-  Plan c;
-  const long packed = static_cast<long>(max_rows < rows ? max_rows : rows) * (heads / kv_heads);
-  c.nt = packed > 8 ? 2 : 1;
-  c.tiles = static_cast<int>((packed + 8 * c.nt - 1) / (8 * c.nt));
-  const long ctas = static_cast<long>(n_seqs) * c.tiles * kv_heads;
-  long z = (3L * q3h::sm_count() + ctas - 1) / ctas;
-  const long most = (max_kv + 511) / 512;          // 4 blocks a warp at least
-  z = z < most ? z : most;
-  c.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
+                      uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  Plan c{};
+  const long group = heads / kv_heads;
+  const long packed = static_cast<long>(max_rows < rows ? max_rows : rows) * group;
+  const int sms = q3h::sm_count();
+  c.few_rows = 16;
+  c.nt = packed > 8 && group <= c.few_rows ? 2 : 1;
+  if (group <= c.few_rows) {
+    const long units = static_cast<long>(n_seqs) * kv_heads * ((max_kv + KB - 1) / KB);
+    const long ctas = (units + MIN_UNITS * WARPS - 1) / (MIN_UNITS * WARPS);
+    const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2);
+    c.few_ctas = static_cast<int>(ctas < most ? ctas : most);
+    c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
+  }
+  c.splits = 1;
+  if (packed > c.few_rows) {
+    c.tiles = static_cast<int>((packed + 15) / 16);
+    const long ctas = static_cast<long>(n_seqs) * c.tiles * kv_heads;
+    long z = (3L * sms + ctas - 1) / ctas;
+    const long most = (max_kv + 511) / 512;        // 4 blocks a warp at least
+    z = z < most ? z : most;
+    c.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
+  }
+  const size_t parts = c.splits > 1 ? static_cast<size_t>(c.splits) * rows * heads : 0;
+  c.bytes = (c.few_slots + parts) * (head_dim + 2) * 4;
   return c;
 }
 
@@ -498,16 +1057,46 @@ extern "C" size_t q3_attention_chunk_workspace_bytes(uint32_t rows, uint32_t n_s
                                                      uint32_t heads, uint32_t kv_heads,
                                                      uint32_t head_dim) {
   if (!rows || !n_seqs || !max_rows || !max_kv || !heads || !kv_heads || heads % kv_heads) return 0;
-  const chunk::Plan c = chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads);
-  return c.splits == 1 ? 0 : static_cast<size_t>(c.splits) * rows * heads * (head_dim + 2) * 4;
+  return chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim).bytes;
+}
+
+// Dynamic shared memory above 48 KB is opted into once per kernel and device.
+template <auto kernel>
+static int opt_in(int bytes) {
+  static std::atomic<bool> done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return Q3_ERR_CUDA;
+    }
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return Q3_OK;
 }
 
 template <int HD, int NT>
-static int launch_few(const chunk::Args &p, int splits, cudaStream_t s) {
-  constexpr int smem = chunk::FewSmem<HD, NT>::bytes;
+static int launch_few(const chunk::Args &p, int ctas, cudaStream_t s) {
+  constexpr int smem = chunk::WARPS * chunk::FewStage<HD>::STAGES * (int)sizeof(chunk::FewStage<HD>);
+  Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
+  chunk::k_attn_few<HD, NT><<<ctas, chunk::WARPS * 32, smem, s>>>(p);
+  Q3_TRY(launch_status());
+  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.rows, p.heads), dim3(chunk::WARPS * 32), 0, s,
+                   p, static_cast<long>(ctas) * chunk::WARPS);
+}
+
+template <int HD>
+static int launch_tiles(const chunk::Args &p, cudaStream_t s) {
+  constexpr int smem = chunk::TileSmem<HD, 2>::bytes;
   static_assert(smem <= 48 * 1024, "no opt-in needed");
-  const dim3 grid(static_cast<unsigned>(p.n_seqs) * p.tiles, p.kv_heads, splits);
-  chunk::k_attn_few<HD, NT><<<grid, chunk::WARPS * 32, smem, s>>>(p);
+  const dim3 grid(static_cast<unsigned>(p.n_seqs) * p.tiles, p.kv_heads, p.splits);
+  chunk::k_attn_tiles<HD, 2><<<grid, chunk::WARPS * 32, smem, s>>>(p);
+  Q3_TRY(launch_status());
+  if (p.splits == 1) return Q3_OK;
+  const long warps = static_cast<long>(p.rows) * p.heads;
+  chunk::k_join_tiles<HD><<<(unsigned)((warps + 3) / 4), 128, 0, s>>>(p);
   return launch_status();
 }
 
@@ -543,17 +1132,15 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   if (rows == 0 || n_seqs == 0) return Q3_OK;
   if (max_rows == 0) return Q3_ERR_SHAPE;
   const uint32_t max_kv = max_pages * kv->page_tokens;
-  const chunk::Plan c = chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads);
-  if (static_cast<uint64_t>(n_seqs) * c.tiles > 0x7fffffffu || kv_heads > 65535) return Q3_ERR_SHAPE;
-  chunk::Args p{};
-  if (c.splits > 1) {
-    const size_t n = static_cast<size_t>(c.splits) * rows * heads;
+  const chunk::Plan c =
+      chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
+  if (static_cast<uint64_t>(n_seqs) * c.tiles > 0x7fffffffu) return Q3_ERR_SHAPE;
+  if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return Q3_ERR_ALIGN;
-    if (workspace_bytes < n * (head_dim + 2) * 4) return Q3_ERR_CAPACITY;
-    p.part_o = static_cast<float *>(workspace);
-    p.part_ml = p.part_o + n * head_dim;
+    if (workspace_bytes < c.bytes) return Q3_ERR_CAPACITY;
   }
+  chunk::Args p{};
   p.q = (const char *)q->data;
   p.q_rb = q->row_bytes;
   p.q_dt = q->dtype;
@@ -585,20 +1172,28 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   p.causal = causal;
   p.window = (int)window;
   p.scale_log2 = (float)((double)qk_scale * 1.4426950408889634);
-  p.splits = c.splits;
-  p.tiles = c.tiles;
+  p.page_shift = (p.page_tokens & (p.page_tokens - 1)) ? -1 : __builtin_ctz(p.page_tokens);
+  p.few_rows = c.few_ctas ? c.few_rows : 0;
   cudaStream_t s = (cudaStream_t)stream;
   timer_begin(TIMER_ATTENTION, s);
-  int st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, c.splits, s)
-                                        : launch_few<128, 2>(p, c.splits, s))
-                           : (c.nt == 1 ? launch_few<64, 1>(p, c.splits, s)
-                                        : launch_few<64, 2>(p, c.splits, s));
-  if (st == Q3_OK && c.splits > 1) {
-    const long warps = static_cast<long>(rows) * heads;
-    const unsigned blocks = (unsigned)((warps + 3) / 4);
-    if (head_dim == 128) chunk::k_attn_join<128><<<blocks, 128, 0, s>>>(p);
-    else chunk::k_attn_join<64><<<blocks, 128, 0, s>>>(p);
-    st = launch_status();
+  int st = Q3_OK;
+  float *ws = static_cast<float *>(workspace);
+  if (c.few_ctas) {
+    chunk::Args f = p;
+    f.part_rows = 8 * c.nt;
+    f.part_o = ws;
+    f.part_ml = ws + c.few_slots * head_dim;
+    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(f, c.few_ctas, s)
+                                      : launch_few<128, 2>(f, c.few_ctas, s))
+                         : (c.nt == 1 ? launch_few<64, 1>(f, c.few_ctas, s)
+                                      : launch_few<64, 2>(f, c.few_ctas, s));
+  }
+  if (st == Q3_OK && c.tiles) {
+    p.splits = c.splits;
+    p.tiles = c.tiles;
+    p.part_o = ws + c.few_slots * (head_dim + 2);
+    p.part_ml = p.part_o + static_cast<size_t>(c.splits) * rows * heads * head_dim;
+    st = head_dim == 128 ? launch_tiles<128>(p, s) : launch_tiles<64>(p, s);
   }
   timer_end(TIMER_ATTENTION, s);
   return st;

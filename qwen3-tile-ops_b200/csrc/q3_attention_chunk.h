@@ -21,8 +21,11 @@ struct Args {
   int causal, window;
   float scale_log2;              // qk_scale * log2(e)
   int splits;                    // parts of the key range (1: results go to o)
-  int tiles;                     // query tiles a sequence may have (few-row kernel)
-  float *part_o, *part_ml;       // [splits][rows][heads][hd], [splits][rows][heads][2]
+  int tiles;                     // query tiles a sequence may have
+  int few_rows;                  // packed rows of a sequence that k_attn_few takes
+  int part_rows;                 // rows of one of its parts
+  int page_shift;                // log2 of page_tokens, or -1
+  float *part_o, *part_ml;       // parts: sums [..][hd], and their (maximum, sum of weights)
 };
 
 // Rows of sequence s as the device sees them; ok = false: nothing to do
@@ -55,6 +58,12 @@ __device__ __forceinline__ void key_range(const Args &p, const Seq &s, int p0, i
                                           int &hi) {
   hi = p.causal ? p1 + 1 : s.kv;
   lo = p.window > 0 && p0 >= p.window ? p0 - p.window + 1 : 0;
+}
+__device__ __forceinline__ uint32_t page_index(const Args &p, uint32_t j) {
+  return p.page_shift >= 0 ? j >> p.page_shift : j / p.page_tokens;
+}
+__device__ __forceinline__ uint32_t page_slot(const Args &p, uint32_t j) {
+  return p.page_shift >= 0 ? j & (p.page_tokens - 1) : j % p.page_tokens;
 }
 // Part z of `splits` of key blocks [b0, b1): equal runs, the first ones longer
 __device__ __forceinline__ void split_range(int b0, int b1, int splits, int z, int &z0, int &z1) {

@@ -193,7 +193,6 @@ def test_attention_workspace_bytes(L):
     f = L.lib().q3_attention_chunk_workspace_bytes
     assert f(0, 1, 1, 4096, 4, 2, 128) == 0 and f(4, 0, 1, 4096, 4, 2, 128) == 0
     assert f(4, 1, 4, 4096, 5, 2, 128) == 0                    # such a call is refused
-    assert f(4096, 64, 64, 4096, 16, 8, 128) == 0              # enough work without splitting
 
 
 def test_wrappers_refuse(q3):
