@@ -74,5 +74,92 @@ __device__ __forceinline__ void split_range(int b0, int b1, int splits, int z, i
 
 constexpr float kVsMin = 7.888609052210118e-31f;   // 2^-100
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// four int8 codes, bytes xor 0x80 (u = code + 128): f16 0x6400 + u is 1024 + u
+__device__ __forceinline__ uint32_t f16_pair(uint32_t u, uint32_t sel) {
+  const uint32_t m = __byte_perm(u, 0x64646464u, sel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&m), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// bf16 rows: 2^up brings the row's maximum m to [2^10, 2^11) (zero, subnormal or infinite m: the
+// nearest exponent in range); `down` is its inverse.
+__device__ __forceinline__ void bf16_scale(float m, float &up, float &down) {
+  const int ex = static_cast<int>(__float_as_uint(m) >> 23);
+  const int e = min(max(137 - ex, -120), 110);
+  up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+}
+
+// One head of a result row (whole warp, lane: columns lane*N ..) to o / os.
+template <int N>
+__device__ __forceinline__ void store_out(const Args &p, long r, int h, int lane, float (&x)[N]) {
+  constexpr int HD = 32 * N;
+  char *o = p.o + r * p.o_rb;
+  const long col = static_cast<long>(h) * HD + lane * N;
+  if (p.o_dt == Q3_DT_F16) store_row<__half, N>(x, o + col * 2);
+  else if (p.o_dt == Q3_DT_BF16) store_row<__nv_bfloat16, N>(x, o + col * 2);
+  else {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    const float scale = __fmul_rn(warp_tree_max(m), kInv127);
+    int c[N];
+    quant_n_absmax<N>(x, scale, c);
+    Elems<int8_t, N> e;
+#pragma unroll
+    for (int i = 0; i < N; ++i) e.e[i] = static_cast<int8_t>(c[i]);
+    e.store(o + col);
+    if (lane == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
+  }
+}
+
+// Sequence of unit `unit` when sequence s has units(s) of them (whole warp); before: those of the
+// sequences before it.  -1: there is no such unit.
+template <typename F>
+__device__ __forceinline__ int find_unit(int n_seqs, long unit, int lane, long &before, F units) {
+  before = 0;
+  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+    const long mine = s0 + lane < n_seqs ? units(s0 + lane) : 0;
+    long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, before + upto > unit);
+    if (m) {
+      const int l = __ffs(m) - 1;
+      before += __shfl_sync(0xffffffffu, upto - mine, l);
+      return s0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return -1;
+}
+
+// Many rows (q3_attention_chunk_tc.cu): sequences with more than few_rows packed rows.  `tiles` is the
+// number of 256-row tiles that the batch can have.
+constexpr int TC_ROWS = 256, TC_KEYS = 128;
+int launch_tc(const Args &p, int head_dim, cudaStream_t s);
+
 }  // namespace chunk
 }  // namespace q3

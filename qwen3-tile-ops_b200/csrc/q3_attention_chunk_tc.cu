@@ -1,0 +1,704 @@
+// Attention of a ragged batch over the paged int8 cache, sequences with many new
+// rows, on the 5th-generation tensor cores (the formulas: q3_attention_chunk.cu).
+//
+// CTA = (sequence, 256 packed rows, KV head, part of the keys); packed row m is
+// head m % group of new row m / group, so a KV head is read once for its whole
+// group.  Two 128-row tiles take turns: while one tile's 128 x 128 scores
+// are exponentiated, the tensor cores work on the other's.
+//   warps 0-7    rows: four warps a tile, one TMEM lane quadrant each
+//   warps 8-13   codes of K and V from global memory, widened to f16 (exact), into a
+//                ring of four operand tiles in the 128-byte-swizzled layout
+//   warp 14      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
+//   warp 15      issues the products: S = Q K8^T (both operands in shared
+//                memory), O += P V8 (P in TMEM, over its scores)
+// The loads are plain ones because each code passes through registers on its
+// way (the tensor cores take no f16 x int8); rows of pages of any length then need
+// no tile shape of their own.
+#include <atomic>
+
+#include "q3_attention_chunk.h"
+#include "q3_tc.cuh"
+
+namespace q3 {
+
+static __device__ unsigned int g_chunk_tc_error = 0;
+
+int chunk_tc_device_status_take() {
+  unsigned int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_chunk_tc_error, sizeof v) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_chunk_tc_error, &zero, sizeof zero);
+  return static_cast<int>(v);
+}
+
+namespace chunk {
+
+using namespace tcx;
+
+constexpr unsigned kErrWait = 1u << 18;
+constexpr int TC_THREADS = 512;
+constexpr int LOADERS = 6;                         // warps 8 .. 13
+constexpr int RING = 4;                            // operand tiles K0, V0, K1, V1, ...
+constexpr int INFO = 4;                            // key tiles whose places and scales are known
+constexpr int UNIT_ROWS = 8;                       // key rows of a loader's unit
+constexpr int UNITS = TC_KEYS / UNIT_ROWS;         // of an operand tile
+constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
+
+template <int HD>
+struct TcSmem {
+  alignas(1024) uint8_t q[2][128 * HD * 2];        // [64-column half][row][128 bytes], swizzled
+  alignas(1024) uint8_t kv[RING][TC_KEYS * HD * 2];// [64-column half][key][128 bytes], swizzled
+  // scales in the order a row thread reads them: 16 keys 16k .. lie as [t4][keys 2 t4, 2 t4 + 1,
+  // 8 + 2 t4, 8 + 2 t4 + 1]
+  alignas(16) float ks[INFO][TC_KEYS], lv[INFO][TC_KEYS], rv[INFO][TC_KEYS];
+  uint32_t place[INFO][TC_KEYS];                   // page << 16 | slot, or -1
+  float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS];
+  unsigned long long full[RING], empty[RING], info_full[INFO], info_empty[INFO];
+  unsigned long long s_full[2], p_full[2], o_full;
+  uint32_t tmem;
+  int abort;
+  int seq, tile;                                   // this CTA's, from the lookup
+};
+
+__device__ __forceinline__ void wait_bar(unsigned long long *b, uint32_t par, int *abort) {
+  if (mbar_wait(b, par, abort, 100000u)) return;
+  if (!*reinterpret_cast<volatile int *>(abort)) atomicOr(&g_chunk_tc_error, kErrWait);
+  *reinterpret_cast<volatile int *>(abort) = 1;
+}
+
+// kind::f16 with float32 sums: f16 x f16, M = 128, N = n; b_mn: B is MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+// 128-byte swizzle, MN-major, two 64-column atoms side by side `lbo` bytes apart
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = (saddr & 0x3FFFFu) >> 4;
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
+  return d;
+}
+// 32 columns of 16 TMEM lanes as fragments: v[4i], v[4i+1] row lane / 4 and columns 8i + 2 (lane % 4),
+// + 1; v[4i+2], v[4i+3] row lane / 4 + 8
+__device__ __forceinline__ void tm_ld(uint32_t at, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15},"
+      " [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tm_st(uint32_t at, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          at),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+      "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
+// 32 columns of 16 lanes: v[2i] row lane / 4, column 4i + lane % 4; v[2i+1] row lane / 4 + 8
+__device__ __forceinline__ void tm_st_p(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// 32 columns of one row (lane)
+__device__ __forceinline__ void tm_ld_row(uint32_t at, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+        "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(at));
+}
+// after tcgen05.wait::ld: no use of v moves above it
+__device__ __forceinline__ void landed(float (&v)[16]) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                 "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+__device__ __forceinline__ void landed(float (&v)[32]) {
+  landed(reinterpret_cast<float(&)[16]>(v[0]));
+  landed(reinterpret_cast<float(&)[16]>(v[16]));
+}
+// two float32 at once
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void un(F2 x, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x.v));
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+__device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
+  const Seq q = load_seq(p, s, err);
+  const int packed = q.n * p.group;
+  return q.ok && packed > p.few_rows ? (packed + TC_ROWS - 1) / TC_ROWS : 0;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
+  constexpr int HALVES = HD / 64;
+  constexpr int HALF_BYTES = 128 * 128;            // 128 rows (or keys) of 64 f16
+  constexpr uint32_t ID_S = idesc_f16(TC_KEYS, false), ID_O = idesc_f16(HD, true);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  TcSmem<HD> &sm = *reinterpret_cast<TcSmem<HD> *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y;
+
+  if (warp == 0) {
+    unsigned err = 0;
+    long before;
+    const int s = find_unit(p.n_seqs, blockIdx.x, lane, before,
+                            [&](int x) { return tiles_of(p, x, &err); });
+    if (lane == 0) {
+      sm.seq = s;
+      // the last tile, which has most keys, first
+      sm.tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, &err) - 1 - (blockIdx.x - before));
+      sm.abort = 0;
+      for (int i = 0; i < RING; ++i) {
+        mbar_init(&sm.full[i], UNITS);
+        mbar_init(&sm.empty[i], 1);
+      }
+      for (int i = 0; i < INFO; ++i) {
+        mbar_init(&sm.info_full[i], 1);
+        mbar_init(&sm.info_empty[i], LOADERS + 8);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.s_full[i], 1);
+        mbar_init(&sm.p_full[i], 128);
+      }
+      mbar_init(&sm.o_full, 1);
+      mbar_init_fence();
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {   // refusals, once a launch
+      for (int x = lane; x < p.n_seqs; x += 32) load_seq(p, x, &err);
+      if (err) atomicOr(&g_chunk_tc_error, err);
+    }
+  }
+  __syncthreads();
+  const int s = sm.seq;
+  if (s < 0) return;
+  unsigned none = 0;
+  const Seq q = load_seq(p, s, &none);
+  const int packed = q.n * p.group, m0 = sm.tile * TC_ROWS;
+  const int rows = min(TC_ROWS, packed - m0);
+  // key tiles [z0, z0 + nj) of this CTA; row tile t needs the first jt[t] of them
+  int z0, nj, jt[2];
+  {
+    const int pf = q.pos0 + m0 / p.group, pl = q.pos0 + (m0 + rows - 1) / p.group;
+    int lo, hi, z1;
+    key_range(p, q, pf, pl, lo, hi);
+    split_range(lo / TC_KEYS, (hi + TC_KEYS - 1) / TC_KEYS, p.splits, blockIdx.z, z0, z1);
+    nj = z1 - z0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int last = min(rows, 128 * (t + 1)) - 1;
+      const int h = p.causal ? q.pos0 + (m0 + last) / p.group + 1 : q.kv;
+      const int n = (h + TC_KEYS - 1) / TC_KEYS - z0;
+      jt[t] = rows > 128 * t ? max(0, min(nj, n)) : 0;
+    }
+    nj = max(jt[0], jt[1]);
+  }
+  if (warp == 15) tmem_alloc<512>(&sm.tmem);
+
+  // ---- queries as f16 in the operand layout, and each row's a
+  {
+    constexpr int N = HD / 32;
+#pragma unroll 4
+    for (int i = 0; i < TC_ROWS / 16; ++i) {
+      const int m = warp * (TC_ROWS / 16) + i;
+      Elems<__half, N> e;
+#pragma unroll
+      for (int k = 0; k < N; ++k) e.e[k] = __ushort_as_half(0);
+      float scale = 0.0f;
+      if (m < rows) {
+        const long r = q.first + (m0 + m) / p.group;
+        const int h = kvh * p.group + (m0 + m) % p.group;
+        const char *qp = p.q + r * p.q_rb;
+        const long col = static_cast<long>(h) * HD + lane * N;
+        if (p.q_dt == Q3_DT_I8) {
+          Elems<int8_t, N> c;
+          c.load(qp + col);
+          scale = reinterpret_cast<const float *>(p.qs + r * p.qs_rb)[h];
+#pragma unroll
+          for (int k = 0; k < N; ++k) e.e[k] = __int2half_rn(c.e[k]);
+        } else if (p.q_dt == Q3_DT_F16) {
+          e.load(qp + col * 2);
+          scale = 1.0f;
+        } else {
+          Elems<__nv_bfloat16, N> c;
+          c.load(qp + col * 2);
+          float mx = 0.0f, up;
+#pragma unroll
+          for (int k = 0; k < N; ++k) mx = fmaxf(mx, fabsf(to_f32(c.e[k])));
+          bf16_scale(warp_tree_max(mx), up, scale);
+#pragma unroll
+          for (int k = 0; k < N; ++k) e.e[k] = __float2half_rn(__fmul_rn(to_f32(c.e[k]), up));
+        }
+      }
+      const int d = lane * N, r = m & 127;
+      e.store(sm.q[m >> 7] + (d / 64) * HALF_BYTES + r * 128 + ((((d % 64) / 8) ^ (r & 7)) * 16) +
+              (d % 8) * 2);
+      if (lane == 0) sm.a[m] = __fmul_rn(scale, p.scale_log2);
+    }
+  }
+  fence_proxy_async();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ rows
+    const int t = warp >> 2, qd = warp & 3, g = lane >> 2, t4 = lane & 3;
+    // this thread's rows, by pass (16 lanes of the quadrant) and half: t*128 + qd*32 + 16 ps + 8 e + g
+    float a[2][2], mref[2][2], l[2][2];
+    int pos[2][2];
+    const int rb = t * 128 + qd * 32;
+#pragma unroll
+    for (int ps = 0; ps < 2; ++ps)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int m = rb + 16 * ps + 8 * e + g;
+        a[ps][e] = sm.a[m];
+        pos[ps][e] = q.pos0 + min(m0 + m, packed - 1) / p.group;
+        mref[ps][e] = kNegInf;
+        l[ps][e] = 0.0f;
+      }
+    const int pmin = q.pos0 + min(m0 + rb, packed - 1) / p.group;
+    const int pmax = q.pos0 + min(m0 + rb + 31, packed - 1) / p.group;
+    for (int j = 0; j < nj; ++j) {
+      const int in = j % INFO;
+      wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
+      if (j < jt[t]) {
+        wait_bar(&sm.s_full[t], j & 1, &sm.abort);
+        fence_after();
+        const int key0 = (z0 + j) * TC_KEYS;
+        const bool masked = (p.causal && key0 + TC_KEYS - 1 > pmin) ||
+                            (p.window > 0 && key0 <= pmax - p.window);
+#pragma unroll
+        for (int ps = 0; ps < 2; ++ps) {
+          const uint32_t lanes = static_cast<uint32_t>(qd * 32 + ps * 16) << 16;
+          float x[4][16];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tm_ld(tmem + lanes + t * 128 + c * 32, x[c]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) landed(x[c]);
+          const F2 a0 = f2(a[ps][0], a[ps][0]), a1 = f2(a[ps][1], a[ps][1]);
+          float mx0 = kNegInf, mx1 = kNegInf;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {            // 16 keys: column groups 2k and 2k + 1
+              const int at = (c * 2 + k) * 16 + t4 * 4;
+              const float4 ks = *reinterpret_cast<const float4 *>(&sm.ks[in][at]);
+              const float4 lv = *reinterpret_cast<const float4 *>(&sm.lv[in][at]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float *y = &x[c][(2 * k + h) * 4];
+                const F2 kk = h ? f2(ks.z, ks.w) : f2(ks.x, ks.y);
+                const F2 ll = h ? f2(lv.z, lv.w) : f2(lv.x, lv.y);
+                un(fma2(mul2(f2(y[0], y[1]), kk), a0, ll), y[0], y[1]);
+                un(fma2(mul2(f2(y[2], y[3]), kk), a1, ll), y[2], y[3]);
+                if (masked) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + c * 32 + (2 * k + h) * 8 + t4 * 2 + (i & 1);
+                    const int at_ = pos[ps][i >> 1];
+                    const bool hide = (p.causal && key > at_) || (p.window > 0 && key <= at_ - p.window);
+                    y[i] = hide ? kNegInf : y[i];
+                  }
+                }
+                mx0 = fmaxf(mx0, fmaxf(y[0], y[1]));
+                mx1 = fmaxf(mx1, fmaxf(y[2], y[3]));
+              }
+            }
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+          // a new reference when the maximum outgrows the old one by 2^8
+          const bool g0 = mx0 > __fadd_rn(mref[ps][0], 8.0f), g1 = mx1 > __fadd_rn(mref[ps][1], 8.0f);
+          if (__any_sync(0xffffffffu, g0 || g1)) {
+            const float r0 = g0 ? ex2(__fsub_rn(mref[ps][0], mx0)) : 1.0f;
+            const float r1 = g1 ? ex2(__fsub_rn(mref[ps][1], mx1)) : 1.0f;
+            mref[ps][0] = g0 ? mx0 : mref[ps][0];
+            mref[ps][1] = g1 ? mx1 : mref[ps][1];
+            l[ps][0] = __fmul_rn(l[ps][0], r0);
+            l[ps][1] = __fmul_rn(l[ps][1], r1);
+            if (j > 0) {   // the products before this tile's have completed with its scores
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                const uint32_t at = tmem + lanes + TMEM_O + t * 128 + c * 32;
+                float o[16];
+                tm_ld(at, o);
+                tmem_wait_ld();
+                landed(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(o[i], (i & 2) ? r1 : r0);
+                tm_st(at, o);
+              }
+              tmem_wait_st();
+            }
+          }
+          const float b0 = mref[ps][0] == kNegInf ? 0.0f : -mref[ps][0];
+          const float b1 = mref[ps][1] == kNegInf ? 0.0f : -mref[ps][1];
+          const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
+          F2 s0 = f2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+          for (int c2 = 0; c2 < 2; ++c2) {           // 64 keys: 32 columns of P
+            uint32_t w[16];
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int c = c2 * 2 + cc;
+                const int at = (c * 2 + k) * 16 + t4 * 4;
+                const float4 rv = *reinterpret_cast<const float4 *>(&sm.rv[in][at]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float *y = &x[c][(2 * k + h) * 4];
+                  un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
+                  un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
+                  const F2 rr = h ? f2(rv.z, rv.w) : f2(rv.x, rv.y);
+                  s0 = fma2(f2(y[0], y[1]), rr, s0);
+                  s1 = fma2(f2(y[2], y[3]), rr, s1);
+                  w[(cc * 4 + 2 * k + h) * 2] = pack_f16(y[0], y[1]);
+                  w[(cc * 4 + 2 * k + h) * 2 + 1] = pack_f16(y[2], y[3]);
+                }
+              }
+            tm_st_p(tmem + lanes + t * 128 + c2 * 32, w);
+          }
+          float u, v;
+          un(s0, u, v);
+          l[ps][0] = __fadd_rn(l[ps][0], __fadd_rn(u, v));
+          un(s1, u, v);
+          l[ps][1] = __fadd_rn(l[ps][1], __fadd_rn(u, v));
+        }
+        tmem_wait_st();
+        fence_before();
+        mbar_arrive(&sm.p_full[t]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.info_empty[in]);
+    }
+    // ---- sums of the rows, then each thread its own row
+#pragma unroll
+    for (int ps = 0; ps < 2; ++ps)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float y = l[ps][e];
+        y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 1));
+        y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 2));
+        if (t4 == 0) {
+          sm.l[rb + 16 * ps + 8 * e + g] = y;
+          sm.m[rb + 16 * ps + 8 * e + g] = mref[ps][e];
+        }
+      }
+    __syncwarp();
+    if (nj > 0) wait_bar(&sm.o_full, 0, &sm.abort);
+    fence_after();
+    const int m = rb + lane;
+    const bool have = m < rows;
+    const int mm = min(m0 + m, packed - 1);
+    const long r = q.first + mm / p.group;
+    const int h = kvh * p.group + mm % p.group;
+    const uint32_t src = tmem + (static_cast<uint32_t>(qd * 32) << 16) + TMEM_O + t * 128;
+    const float lsum = sm.l[m];
+    if (p.splits > 1) {
+      const long at = (static_cast<long>(blockIdx.z) * p.rows + r) * p.heads + h;
+      if (jt[t] > 0) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          Elems<float, 32> o;
+          tm_ld_row(src + c * 32, o.e);
+          tmem_wait_ld();
+          landed(o.e);
+          if (have) o.store(p.part_o + at * HD + c * 32);
+          __syncwarp();
+        }
+      }
+      if (have) {
+        p.part_ml[at * 2] = jt[t] > 0 ? sm.m[m] : kNegInf;
+        p.part_ml[at * 2 + 1] = jt[t] > 0 ? lsum : 0.0f;
+      }
+    } else if (jt[t] > 0) {
+      const float inv = lsum == 0.0f ? 0.0f : __fdiv_rn(1.0f, lsum);   // no key seen: zeros
+      char *out = p.o + r * p.o_rb;
+      const long col = static_cast<long>(h) * HD;
+      float scale = 0.0f;
+      if (p.o_dt == Q3_DT_I8) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          float o[32];
+          tm_ld_row(src + c * 32, o);
+          tmem_wait_ld();
+          landed(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(__fmul_rn(o[i], inv)));
+        }
+        scale = __fmul_rn(mx, kInv127);
+        if (have) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
+      }
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        float o[32];
+        tm_ld_row(src + c * 32, o);
+        tmem_wait_ld();
+        landed(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __fmul_rn(o[i], inv);
+        if (have) {
+          if (p.o_dt == Q3_DT_I8) {
+            uint32_t w[8];
+            quant_pack_absmax<32>(o, scale, w);
+            Elems<int8_t, 32> e;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t *>(e.e)[i] = w[i];
+            e.store(out + col + c * 32);
+          } else if (p.o_dt == Q3_DT_F16) {
+            store_row<__half, 32>(o, out + (col + c * 32) * 2);
+          } else {
+            store_row<__nv_bfloat16, 32>(o, out + (col + c * 32) * 2);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8 + LOADERS) {
+    // ------------------------------------------------------------------ codes of K and V
+    // unit n of the stream: key rows 8 (n % 16) .. of operand tile n / 16 (K and V in turn)
+    constexpr int V4 = UNIT_ROWS * HD / 512;         // 16-byte loads a lane and unit
+    constexpr int D = HD == 128 ? 4 : 6;             // units in flight
+    const int lw = warp - 8, total = nj * 2 * UNITS;
+    // eight lanes take 4 chunks of two rows: their f16 chunks then lie in 8 different places of a
+    // 128-byte line
+    const int rowl = HD == 128 ? 2 * (lane >> 4) + ((lane >> 2) & 1) : lane >> 2;
+    const int c = HD == 128 ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane & 3;
+    const long kcol = static_cast<long>(kvh) * HD + c * 16;
+    uint4 buf[D][V4];
+    int tile_in = 0;                                 // key tile whose places are being read
+    auto issue = [&](int n, uint4 (&b)[V4]) {
+      if (n >= total) return;
+      const int item = n / UNITS, j = item >> 1;
+      if (j != tile_in) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.info_empty[tile_in % INFO]);
+        tile_in = j;
+      }
+      wait_bar(&sm.info_full[j % INFO], (j / INFO) & 1, &sm.abort);
+      const char *base = ((item & 1) ? p.v : p.k) + kcol;
+#pragma unroll
+      for (int i = 0; i < V4; ++i) {
+        const uint32_t at = sm.place[j % INFO][(n % UNITS) * UNIT_ROWS + i * 4 + rowl];
+        b[i] = make_uint4(0, 0, 0, 0);
+        if (at != 0xffffffffu)
+          b[i] = __ldg(reinterpret_cast<const uint4 *>(
+              base + static_cast<size_t>(at >> 16) * p.page_bytes +
+              static_cast<size_t>(at & 0xffffu) * p.row_bytes));
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d) issue(lw + d * LOADERS, buf[d]);
+    for (int n0 = lw; n0 < total; n0 += D * LOADERS) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int n = n0 + d * LOADERS;
+        if (n >= total) break;
+        const int item = n / UNITS, slot = item % RING;
+        if (item >= RING) wait_bar(&sm.empty[slot], ((item / RING) - 1) & 1, &sm.abort);
+#pragma unroll
+        for (int i = 0; i < V4; ++i) {
+          const int r = (n % UNITS) * UNIT_ROWS + i * 4 + rowl;
+          const uint32_t w[4] = {buf[d][i].x ^ 0x80808080u, buf[d][i].y ^ 0x80808080u,
+                                 buf[d][i].z ^ 0x80808080u, buf[d][i].w ^ 0x80808080u};
+          uint4 lo, hi;
+          lo.x = f16_pair(w[0], 0x4140), lo.y = f16_pair(w[0], 0x4342);
+          lo.z = f16_pair(w[1], 0x4140), lo.w = f16_pair(w[1], 0x4342);
+          hi.x = f16_pair(w[2], 0x4140), hi.y = f16_pair(w[2], 0x4342);
+          hi.z = f16_pair(w[3], 0x4140), hi.w = f16_pair(w[3], 0x4342);
+          uint8_t *row = sm.kv[slot] + (c >> 2) * HALF_BYTES + r * 128;
+          const int ch = (c & 3) * 2;
+          *reinterpret_cast<uint4 *>(row + ((ch ^ (r & 7)) * 16)) = lo;
+          *reinterpret_cast<uint4 *>(row + (((ch + 1) ^ (r & 7)) * 16)) = hi;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.full[slot]);
+        issue(n + D * LOADERS, buf[d]);
+      }
+    }
+  } else if (warp == 14) {
+    // ------------------------------------------------------------------ places and scales
+    const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
+    for (int j = 0; j < nj; ++j) {
+      const int in = j % INFO;
+      uint32_t at[4];
+      float ks[4], vs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = (z0 + j) * TC_KEYS + i * 32 + lane;
+        at[i] = 0xffffffffu;
+        if (key < q.kv) {
+          const uint32_t page = table[page_index(p, key)];
+          if (page < p.num_pages) at[i] = (page << 16) | page_slot(p, key);
+          else atomicOr(&g_chunk_tc_error, kBadPage);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ks[i] = 0.0f, vs[i] = 0.0f;
+        if (at[i] != 0xffffffffu) {
+          const size_t so = static_cast<size_t>(at[i] >> 16) * p.scale_page_bytes +
+                            static_cast<size_t>(at[i] & 0xffffu) * p.scale_row_bytes + kvh * 4;
+          ks[i] = __ldg(reinterpret_cast<const float *>(p.ks + so));
+          vs[i] = __ldg(reinterpret_cast<const float *>(p.vs + so));
+        }
+      }
+      if (j >= INFO) wait_bar(&sm.info_empty[in], ((j / INFO) - 1) & 1, &sm.abort);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = i * 32 + lane, k = key & 15;
+        const int to = (key & ~15) + ((k & 7) >> 1) * 4 + (k >> 3) * 2 + (k & 1);
+        const float v = fmaxf(vs[i], kVsMin);        // (NaN: fmaxf drops it ...
+        sm.place[in][key] = at[i];
+        sm.ks[in][to] = ks[i];
+        // ... and the rows that see it get NaN); a key that is not there: weight 0
+        sm.lv[in][to] = at[i] == 0xffffffffu ? kNegInf : vs[i] != vs[i] ? vs[i] : lg2(v);
+        sm.rv[in][to] = rcp(v);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.info_full[in]);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------------ products
+    uint32_t qa[2];
+    qa[0] = su32(sm.q[0]);
+    qa[1] = su32(sm.q[1]);
+    auto scores = [&](int t, int j) {   // S_t = Q_t K8_j^T
+      const uint32_t kb = su32(sm.kv[(2 * j) % RING]);
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint32_t at = (k / 4) * HALF_BYTES + (k % 4) * 32;
+        mma_ss(tmem + t * 128, sdesc_sw128(qa[t] + at), sdesc_sw128(kb + at), ID_S, k != 0);
+      }
+      mma_commit(&sm.s_full[t]);
+    };
+    auto values = [&](int t, int j) {   // O_t += P_t V8_j
+      const uint32_t vb = su32(sm.kv[(2 * j + 1) % RING]);
+#pragma unroll
+      for (int k = 0; k < TC_KEYS / 16; ++k)
+        mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + k * 8,
+               sdesc_mn(vb + k * 2048, HALVES == 2 ? HALF_BYTES : 16), ID_O, j > 0 || k > 0);
+    };
+    auto ready = [&](int item) {
+      wait_bar(&sm.full[item % RING], (item / RING) & 1, &sm.abort);
+      fence_after();
+    };
+    if (nj > 0) {
+      ready(0);
+      for (int t = 0; t < 2; ++t)
+        if (jt[t] > 0) scores(t, 0);
+      mma_commit(&sm.empty[0]);
+    }
+    for (int j = 0; j < nj; ++j) {
+      ready(2 * j + 1);
+      if (j + 1 < nj) ready(2 * j + 2);
+      for (int t = 0; t < 2; ++t) {
+        if (j < jt[t]) {
+          wait_bar(&sm.p_full[t], j & 1, &sm.abort);
+          fence_after();
+          values(t, j);
+          // these scores overwrite P_t: products of one thread run in order
+          if (j + 1 < jt[t]) scores(t, j + 1);
+        }
+      }
+      mma_commit(&sm.empty[(2 * j + 1) % RING]);
+      if (j + 1 < nj) mma_commit(&sm.empty[(2 * j + 2) % RING]);
+    }
+    if (nj > 0) {
+      mma_commit(&sm.o_full);
+      wait_bar(&sm.o_full, 0, &sm.abort);
+    }
+  }
+
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 15) tmem_dealloc<512>(tmem);
+}
+
+template <int HD>
+static int launch(const Args &p, cudaStream_t s) {
+  constexpr int smem = static_cast<int>(sizeof(TcSmem<HD>)) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  static std::atomic<bool> done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !done[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(k_attn_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) {
+      q3h::set_cuda_error(e);
+      return Q3_ERR_CUDA;
+    }
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  k_attn_tc<HD><<<dim3(p.tiles, p.kv_heads, p.splits), TC_THREADS, smem, s>>>(p);
+  return q3h::launch_status();
+}
+
+int launch_tc(const Args &p, int head_dim, cudaStream_t s) {
+  return head_dim == 128 ? launch<128>(p, s) : launch<64>(p, s);
+}
+
+}  // namespace chunk
+}  // namespace q3

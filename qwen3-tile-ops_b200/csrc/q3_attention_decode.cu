@@ -474,6 +474,7 @@ int tp_device_status_take();
 int dsplit_device_status_take();
 int rope_device_status_take();
 int chunk_device_status_take();
+int chunk_tc_device_status_take();
 }
 
 extern "C" int q3_device_status(void) {
@@ -503,5 +504,8 @@ extern "C" int q3_device_status(void) {
   const int ch = q3::chunk_device_status_take();
   if (ch < 0) return -1;
   v |= static_cast<unsigned int>(ch);
+  const int ct = q3::chunk_tc_device_status_take();
+  if (ct < 0) return -1;
+  v |= static_cast<unsigned int>(ct);
   return static_cast<int>(v) | g;
 }
