@@ -6,10 +6,10 @@
 // group.  Two 128-row tiles take turns: while one tile's 128 x 128 scores
 // are exponentiated, the tensor cores work on the other's.
 //   warps 0-7    rows: four warps a tile, one TMEM lane quadrant each
-//   warps 8-13   codes of K and V from global memory, widened to f16 (exact), into a
+//   warps 8-11   codes of K and V from global memory, widened to f16 (exact), into a
 //                ring of four operand tiles in the 128-byte-swizzled layout
-//   warp 14      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
-//   warp 15      issues the products: S = Q K8^T (both operands in shared
+//   warp 12      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
+//   warp 13      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
 // The loads are plain ones because each code passes through registers on its
 // way (the tensor cores take no f16 x int8); rows of pages of any length then need
@@ -36,11 +36,10 @@ using namespace tcx;
 
 constexpr unsigned kErrWait = 1u << 18;
 constexpr int TC_THREADS = 512;
-constexpr int LOADERS = 6;                         // warps 8 .. 13
+constexpr int LOADERS = 4;                         // warps 8 .. 11
+constexpr int INFO_WARP = 12, MMA_WARP = 13;
 constexpr int RING = 4;                            // operand tiles K0, V0, K1, V1, ...
 constexpr int INFO = 4;                            // key tiles whose places and scales are known
-constexpr int UNIT_ROWS = 8;                       // key rows of a loader's unit
-constexpr int UNITS = TC_KEYS / UNIT_ROWS;         // of an operand tile
 constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
 
 template <int HD>
@@ -50,7 +49,7 @@ struct TcSmem {
   // scales in the order a row thread reads them: 16 keys 16k .. lie as [t4][keys 2 t4, 2 t4 + 1,
   // 8 + 2 t4, 8 + 2 t4 + 1]
   alignas(16) float ks[INFO][TC_KEYS], lv[INFO][TC_KEYS], rv[INFO][TC_KEYS];
-  uint32_t place[INFO][TC_KEYS];                   // page << 16 | slot, or -1
+  long long place[INFO][TC_KEYS];                  // byte offset of a key's row in the pool, or -1
   float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS];
   unsigned long long full[RING], empty[RING], info_full[INFO], info_empty[INFO];
   unsigned long long s_full[2], p_full[2], o_full;
@@ -59,9 +58,27 @@ struct TcSmem {
   int seq, tile;                                   // this CTA's, from the lookup
 };
 
+// Bounded wait for the phase with parity par (about a second, or until another thread gave up)
 __device__ __forceinline__ void wait_bar(unsigned long long *b, uint32_t par, int *abort) {
-  if (mbar_wait(b, par, abort, 100000u)) return;
-  if (!*reinterpret_cast<volatile int *>(abort)) atomicOr(&g_chunk_tc_error, kErrWait);
+  const uint32_t at = su32(b);
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(at), "r"(par)
+        : "memory");
+    if (ok) return;
+    if ((it & 63) == 0) {
+      if (*reinterpret_cast<volatile int *>(abort)) return;
+      const uint64_t t = gtime();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > 1000000000ull) break;
+    }
+  }
+  atomicOr(&g_chunk_tc_error, kErrWait);
   *reinterpret_cast<volatile int *>(abort) = 1;
 }
 
@@ -172,6 +189,118 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One 128-key tile for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
+// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights in their place, sums at `ot` rescaled
+// when a row's maximum outgrows its reference by 2^8.
+template <int HD, bool MASK>
+__device__ __forceinline__ void rows16(const float *ks, const float *lv, const float *rv, uint32_t st,
+                                       uint32_t ot, bool have_o, const float (&a)[2], float (&mref)[2],
+                                       float (&l)[2], const int (&pos)[2], int key0, int causal,
+                                       int window) {
+  float x[4][16];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tm_ld(st + c * 32, x[c]);
+  tmem_wait_ld();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) landed(x[c]);
+  const F2 a0 = f2(a[0], a[0]), a1 = f2(a[1], a[1]);
+  float mx0 = kNegInf, mx1 = kNegInf;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {                    // 16 keys: column groups 2k and 2k + 1
+    const float4 kk = *reinterpret_cast<const float4 *>(ks + k * 16);
+    const float4 ll = *reinterpret_cast<const float4 *>(lv + k * 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
+      const F2 k2 = h ? f2(kk.z, kk.w) : f2(kk.x, kk.y), l2 = h ? f2(ll.z, ll.w) : f2(ll.x, ll.y);
+      un(fma2(mul2(f2(y[0], y[1]), k2), a0, l2), y[0], y[1]);
+      un(fma2(mul2(f2(y[2], y[3]), k2), a1, l2), y[2], y[3]);
+      if (MASK) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + k * 16 + h * 8 + (i & 1), at = pos[i >> 1];
+          const bool hide = (causal && key > at) || (window > 0 && key <= at - window);
+          y[i] = hide ? kNegInf : y[i];
+        }
+      }
+      mx0 = max3(mx0, y[0], y[1]);
+      mx1 = max3(mx1, y[2], y[3]);
+    }
+  }
+  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+  const bool g0 = mx0 > __fadd_rn(mref[0], 8.0f), g1 = mx1 > __fadd_rn(mref[1], 8.0f);
+  if (__any_sync(0xffffffffu, g0 || g1)) {
+    const float r0 = g0 ? ex2(__fsub_rn(mref[0], mx0)) : 1.0f;
+    const float r1 = g1 ? ex2(__fsub_rn(mref[1], mx1)) : 1.0f;
+    mref[0] = g0 ? mx0 : mref[0];
+    mref[1] = g1 ? mx1 : mref[1];
+    l[0] = __fmul_rn(l[0], r0);
+    l[1] = __fmul_rn(l[1], r1);
+    if (have_o) {   // the products before this tile's have completed with its scores
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float o[16];
+        tm_ld(ot + c * 32, o);
+        tmem_wait_ld();
+        landed(o);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(o[i], (i & 2) ? r1 : r0);
+        tm_st(ot + c * 32, o);
+      }
+      tmem_wait_st();
+    }
+  }
+  const float b0 = mref[0] == kNegInf ? 0.0f : -mref[0], b1 = mref[1] == kNegInf ? 0.0f : -mref[1];
+  const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
+  F2 s0 = f2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+  for (int c2 = 0; c2 < 2; ++c2) {                 // 64 keys: 32 columns of P
+    uint32_t w[16];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const int k = c2 * 4 + kk;
+      const float4 rr = *reinterpret_cast<const float4 *>(rv + k * 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
+        un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
+        un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
+        const F2 r2 = h ? f2(rr.z, rr.w) : f2(rr.x, rr.y);
+        s0 = fma2(f2(y[0], y[1]), r2, s0);
+        s1 = fma2(f2(y[2], y[3]), r2, s1);
+        w[(kk * 2 + h) * 2] = pack_f16(y[0], y[1]);
+        w[(kk * 2 + h) * 2 + 1] = pack_f16(y[2], y[3]);
+      }
+    }
+    tm_st_p(st + c2 * 32, w);
+  }
+  float u, v;
+  un(s0, u, v);
+  l[0] = __fadd_rn(l[0], __fadd_rn(u, v));
+  un(s1, u, v);
+  l[1] = __fadd_rn(l[1], __fadd_rn(u, v));
+}
+
+__device__ __forceinline__ bool elect_one() {   // one lane of the converged warp
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void asm_less_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+}
+
 __device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
   const Seq q = load_seq(p, s, err);
   const int packed = q.n * p.group;
@@ -200,7 +329,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       sm.tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, &err) - 1 - (blockIdx.x - before));
       sm.abort = 0;
       for (int i = 0; i < RING; ++i) {
-        mbar_init(&sm.full[i], UNITS);
+        mbar_init(&sm.full[i], LOADERS);
         mbar_init(&sm.empty[i], 1);
       }
       for (int i = 0; i < INFO; ++i) {
@@ -243,7 +372,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     }
     nj = max(jt[0], jt[1]);
   }
-  if (warp == 15) tmem_alloc<512>(&sm.tmem);
+  if (warp == MMA_WARP) tmem_alloc<512>(&sm.tmem);
 
   // ---- queries as f16 in the operand layout, and each row's a
   {
@@ -292,8 +421,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   fence_after();
   const uint32_t tmem = sm.tmem;
 
+  // registers move from the other warps to those of the rows (2 x 128 x 168 + 2 x 128 x 88 is the
+  // launch's 512 x 128)
   if (warp < 8) {
     // ------------------------------------------------------------------ rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >> 2, qd = warp & 3, g = lane >> 2, t4 = lane & 3;
     // this thread's rows, by pass (16 lanes of the quadrant) and half: t*128 + qd*32 + 16 ps + 8 e + g
     float a[2][2], mref[2][2], l[2][2];
@@ -323,104 +455,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
 #pragma unroll
         for (int ps = 0; ps < 2; ++ps) {
           const uint32_t lanes = static_cast<uint32_t>(qd * 32 + ps * 16) << 16;
-          float x[4][16];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tm_ld(tmem + lanes + t * 128 + c * 32, x[c]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) landed(x[c]);
-          const F2 a0 = f2(a[ps][0], a[ps][0]), a1 = f2(a[ps][1], a[ps][1]);
-          float mx0 = kNegInf, mx1 = kNegInf;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {            // 16 keys: column groups 2k and 2k + 1
-              const int at = (c * 2 + k) * 16 + t4 * 4;
-              const float4 ks = *reinterpret_cast<const float4 *>(&sm.ks[in][at]);
-              const float4 lv = *reinterpret_cast<const float4 *>(&sm.lv[in][at]);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float *y = &x[c][(2 * k + h) * 4];
-                const F2 kk = h ? f2(ks.z, ks.w) : f2(ks.x, ks.y);
-                const F2 ll = h ? f2(lv.z, lv.w) : f2(lv.x, lv.y);
-                un(fma2(mul2(f2(y[0], y[1]), kk), a0, ll), y[0], y[1]);
-                un(fma2(mul2(f2(y[2], y[3]), kk), a1, ll), y[2], y[3]);
-                if (masked) {
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + c * 32 + (2 * k + h) * 8 + t4 * 2 + (i & 1);
-                    const int at_ = pos[ps][i >> 1];
-                    const bool hide = (p.causal && key > at_) || (p.window > 0 && key <= at_ - p.window);
-                    y[i] = hide ? kNegInf : y[i];
-                  }
-                }
-                mx0 = fmaxf(mx0, fmaxf(y[0], y[1]));
-                mx1 = fmaxf(mx1, fmaxf(y[2], y[3]));
-              }
-            }
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-          // a new reference when the maximum outgrows the old one by 2^8
-          const bool g0 = mx0 > __fadd_rn(mref[ps][0], 8.0f), g1 = mx1 > __fadd_rn(mref[ps][1], 8.0f);
-          if (__any_sync(0xffffffffu, g0 || g1)) {
-            const float r0 = g0 ? ex2(__fsub_rn(mref[ps][0], mx0)) : 1.0f;
-            const float r1 = g1 ? ex2(__fsub_rn(mref[ps][1], mx1)) : 1.0f;
-            mref[ps][0] = g0 ? mx0 : mref[ps][0];
-            mref[ps][1] = g1 ? mx1 : mref[ps][1];
-            l[ps][0] = __fmul_rn(l[ps][0], r0);
-            l[ps][1] = __fmul_rn(l[ps][1], r1);
-            if (j > 0) {   // the products before this tile's have completed with its scores
-#pragma unroll
-              for (int c = 0; c < HD / 32; ++c) {
-                const uint32_t at = tmem + lanes + TMEM_O + t * 128 + c * 32;
-                float o[16];
-                tm_ld(at, o);
-                tmem_wait_ld();
-                landed(o);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(o[i], (i & 2) ? r1 : r0);
-                tm_st(at, o);
-              }
-              tmem_wait_st();
-            }
-          }
-          const float b0 = mref[ps][0] == kNegInf ? 0.0f : -mref[ps][0];
-          const float b1 = mref[ps][1] == kNegInf ? 0.0f : -mref[ps][1];
-          const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
-          F2 s0 = f2(0.0f, 0.0f), s1 = s0;
-#pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2) {           // 64 keys: 32 columns of P
-            uint32_t w[16];
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int c = c2 * 2 + cc;
-                const int at = (c * 2 + k) * 16 + t4 * 4;
-                const float4 rv = *reinterpret_cast<const float4 *>(&sm.rv[in][at]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float *y = &x[c][(2 * k + h) * 4];
-                  un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
-                  un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
-                  const F2 rr = h ? f2(rv.z, rv.w) : f2(rv.x, rv.y);
-                  s0 = fma2(f2(y[0], y[1]), rr, s0);
-                  s1 = fma2(f2(y[2], y[3]), rr, s1);
-                  w[(cc * 4 + 2 * k + h) * 2] = pack_f16(y[0], y[1]);
-                  w[(cc * 4 + 2 * k + h) * 2 + 1] = pack_f16(y[2], y[3]);
-                }
-              }
-            tm_st_p(tmem + lanes + t * 128 + c2 * 32, w);
-          }
-          float u, v;
-          un(s0, u, v);
-          l[ps][0] = __fadd_rn(l[ps][0], __fadd_rn(u, v));
-          un(s1, u, v);
-          l[ps][1] = __fadd_rn(l[ps][1], __fadd_rn(u, v));
+          const uint32_t st = tmem + lanes + t * 128, ot = tmem + lanes + TMEM_O + t * 128;
+          if (masked)
+            rows16<HD, true>(sm.ks[in] + t4 * 4, sm.lv[in] + t4 * 4, sm.rv[in] + t4 * 4, st, ot, j > 0,
+                             a[ps], mref[ps], l[ps], pos[ps], key0 + t4 * 2, p.causal, p.window);
+          else
+            rows16<HD, false>(sm.ks[in] + t4 * 4, sm.lv[in] + t4 * 4, sm.rv[in] + t4 * 4, st, ot, j > 0,
+                              a[ps], mref[ps], l[ps], pos[ps], key0 + t4 * 2, p.causal, p.window);
         }
         tmem_wait_st();
         fence_before();
@@ -514,131 +555,146 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       }
     }
     __syncwarp();
-  } else if (warp < 8 + LOADERS) {
+  } else if (asm_less_registers(), warp < 8 + LOADERS) {
     // ------------------------------------------------------------------ codes of K and V
-    // unit n of the stream: key rows 8 (n % 16) .. of operand tile n / 16 (K and V in turn)
-    constexpr int V4 = UNIT_ROWS * HD / 512;         // 16-byte loads a lane and unit
-    constexpr int D = HD == 128 ? 4 : 6;             // units in flight
-    const int lw = warp - 8, total = nj * 2 * UNITS;
+    // Operand tile `item` (K and V in turn): a warp takes 32 key rows in chunks of CR rows, one
+    // 16-byte load a lane; a chunk of the next item is requested as soon as this item's is stored.
+    constexpr int CR = HD == 128 ? 4 : 8, CHUNKS = 32 / CR;
+    const int lw = warp - 8, items = 2 * nj;
     // eight lanes take 4 chunks of two rows: their f16 chunks then lie in 8 different places of a
     // 128-byte line
     const int rowl = HD == 128 ? 2 * (lane >> 4) + ((lane >> 2) & 1) : lane >> 2;
     const int c = HD == 128 ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane & 3;
-    const long kcol = static_cast<long>(kvh) * HD + c * 16;
-    uint4 buf[D][V4];
-    int tile_in = 0;                                 // key tile whose places are being read
-    auto issue = [&](int n, uint4 (&b)[V4]) {
-      if (n >= total) return;
-      const int item = n / UNITS, j = item >> 1;
-      if (j != tile_in) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.info_empty[tile_in % INFO]);
-        tile_in = j;
-      }
-      wait_bar(&sm.info_full[j % INFO], (j / INFO) & 1, &sm.abort);
-      const char *base = ((item & 1) ? p.v : p.k) + kcol;
-#pragma unroll
-      for (int i = 0; i < V4; ++i) {
-        const uint32_t at = sm.place[j % INFO][(n % UNITS) * UNIT_ROWS + i * 4 + rowl];
-        b[i] = make_uint4(0, 0, 0, 0);
-        if (at != 0xffffffffu)
-          b[i] = __ldg(reinterpret_cast<const uint4 *>(
-              base + static_cast<size_t>(at >> 16) * p.page_bytes +
-              static_cast<size_t>(at & 0xffffu) * p.row_bytes));
-      }
+    const char *base[2] = {p.k + static_cast<long>(kvh) * HD + c * 16,
+                           p.v + static_cast<long>(kvh) * HD + c * 16};
+    const int row0 = lw * 32 + rowl;
+    const uint32_t to = static_cast<uint32_t>((c >> 2) * HALF_BYTES + row0 * 128);
+    const int ch = (c & 3) * 2;
+    uint4 buf[CHUNKS];
+    auto load = [&](const long long *place, const char *from, int i) {
+      const long long at = place[row0 + i * CR];
+      buf[i] = make_uint4(0, 0, 0, 0);
+      if (at >= 0) buf[i] = __ldg(reinterpret_cast<const uint4 *>(from + at));
     };
+    if (nj > 0) {
+      wait_bar(&sm.info_full[0], 0, &sm.abort);
 #pragma unroll
-    for (int d = 0; d < D; ++d) issue(lw + d * LOADERS, buf[d]);
-    for (int n0 = lw; n0 < total; n0 += D * LOADERS) {
+      for (int i = 0; i < CHUNKS; ++i) load(sm.place[0], base[0], i);
+    }
+    for (int item = 0; item < items; ++item) {
+      const int slot = item % RING, next = item + 1, jn = next >> 1;
+      const bool more = next < items;
+      if (more && !(next & 1)) wait_bar(&sm.info_full[jn % INFO], (jn / INFO) & 1, &sm.abort);
+      if (item >= RING) wait_bar(&sm.empty[slot], ((item / RING) - 1) & 1, &sm.abort);
+      uint8_t *dst = sm.kv[slot] + to;
+      const long long *place = sm.place[jn % INFO];
+      const char *from = (next & 1) ? base[1] : base[0];
 #pragma unroll
-      for (int d = 0; d < D; ++d) {
-        const int n = n0 + d * LOADERS;
-        if (n >= total) break;
-        const int item = n / UNITS, slot = item % RING;
-        if (item >= RING) wait_bar(&sm.empty[slot], ((item / RING) - 1) & 1, &sm.abort);
-#pragma unroll
-        for (int i = 0; i < V4; ++i) {
-          const int r = (n % UNITS) * UNIT_ROWS + i * 4 + rowl;
-          const uint32_t w[4] = {buf[d][i].x ^ 0x80808080u, buf[d][i].y ^ 0x80808080u,
-                                 buf[d][i].z ^ 0x80808080u, buf[d][i].w ^ 0x80808080u};
-          uint4 lo, hi;
-          lo.x = f16_pair(w[0], 0x4140), lo.y = f16_pair(w[0], 0x4342);
-          lo.z = f16_pair(w[1], 0x4140), lo.w = f16_pair(w[1], 0x4342);
-          hi.x = f16_pair(w[2], 0x4140), hi.y = f16_pair(w[2], 0x4342);
-          hi.z = f16_pair(w[3], 0x4140), hi.w = f16_pair(w[3], 0x4342);
-          uint8_t *row = sm.kv[slot] + (c >> 2) * HALF_BYTES + r * 128;
-          const int ch = (c & 3) * 2;
-          *reinterpret_cast<uint4 *>(row + ((ch ^ (r & 7)) * 16)) = lo;
-          *reinterpret_cast<uint4 *>(row + (((ch + 1) ^ (r & 7)) * 16)) = hi;
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.full[slot]);
-        issue(n + D * LOADERS, buf[d]);
+      for (int i = 0; i < CHUNKS; ++i) {
+        const uint32_t w[4] = {buf[i].x ^ 0x80808080u, buf[i].y ^ 0x80808080u,
+                               buf[i].z ^ 0x80808080u, buf[i].w ^ 0x80808080u};
+        uint4 lo, hi;
+        lo.x = f16_pair(w[0], 0x4140), lo.y = f16_pair(w[0], 0x4342);
+        lo.z = f16_pair(w[1], 0x4140), lo.w = f16_pair(w[1], 0x4342);
+        hi.x = f16_pair(w[2], 0x4140), hi.y = f16_pair(w[2], 0x4342);
+        hi.z = f16_pair(w[3], 0x4140), hi.w = f16_pair(w[3], 0x4342);
+        const int r = row0 + i * CR;
+        *reinterpret_cast<uint4 *>(dst + i * CR * 128 + ((ch ^ (r & 7)) * 16)) = lo;
+        *reinterpret_cast<uint4 *>(dst + i * CR * 128 + (((ch + 1) ^ (r & 7)) * 16)) = hi;
+        if (more) load(place, from, i);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.full[slot]);
+        if (next & 1) mbar_arrive(&sm.info_empty[(item >> 1) % INFO]);   // V's places are read
       }
     }
-  } else if (warp == 14) {
+  } else if (warp == INFO_WARP) {
     // ------------------------------------------------------------------ places and scales
+    // A lane has keys i*32 + lane of a tile.  Pages are looked up two tiles ahead, scales
+    // requested one tile ahead.
     const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
-    for (int j = 0; j < nj; ++j) {
-      const int in = j % INFO;
-      uint32_t at[4];
-      float ks[4], vs[4];
+    auto page_of = [&](int j, int (&pg)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = (z0 + j) * TC_KEYS + i * 32 + lane;
-        at[i] = 0xffffffffu;
-        if (key < q.kv) {
-          const uint32_t page = table[page_index(p, key)];
-          if (page < p.num_pages) at[i] = (page << 16) | page_slot(p, key);
-          else atomicOr(&g_chunk_tc_error, kBadPage);
-        }
+        pg[i] = j < nj && key < q.kv ? table[page_index(p, key)] : -1;
       }
+    };
+    struct Keys {
+      long long at[4];
+      float ks[4], vs[4];
+    };
+    auto request = [&](int j, const int (&pg)[4], Keys &k) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ks[i] = 0.0f, vs[i] = 0.0f;
-        if (at[i] != 0xffffffffu) {
-          const size_t so = static_cast<size_t>(at[i] >> 16) * p.scale_page_bytes +
-                            static_cast<size_t>(at[i] & 0xffffu) * p.scale_row_bytes + kvh * 4;
-          ks[i] = __ldg(reinterpret_cast<const float *>(p.ks + so));
-          vs[i] = __ldg(reinterpret_cast<const float *>(p.vs + so));
+        const int key = (z0 + j) * TC_KEYS + i * 32 + lane;
+        k.at[i] = -1;
+        k.ks[i] = k.vs[i] = 0.0f;
+        if (pg[i] >= 0) {
+          if (static_cast<uint32_t>(pg[i]) < p.num_pages) {
+            const uint32_t slot = page_slot(p, key);
+            k.at[i] = static_cast<long long>(pg[i]) * p.page_bytes +
+                      static_cast<long long>(slot) * p.row_bytes;
+            const size_t so = static_cast<size_t>(pg[i]) * p.scale_page_bytes +
+                              static_cast<size_t>(slot) * p.scale_row_bytes + kvh * 4;
+            k.ks[i] = __ldg(reinterpret_cast<const float *>(p.ks + so));
+            k.vs[i] = __ldg(reinterpret_cast<const float *>(p.vs + so));
+          } else {
+            atomicOr(&g_chunk_tc_error, kBadPage);
+          }
         }
       }
+    };
+    int pg[4];
+    Keys now;
+    page_of(0, pg);
+    request(0, pg, now);
+    page_of(1, pg);
+    for (int j = 0; j < nj; ++j) {
+      const int in = j % INFO;
+      Keys next;
+      request(j + 1, pg, next);
+      page_of(j + 2, pg);
       if (j >= INFO) wait_bar(&sm.info_empty[in], ((j / INFO) - 1) & 1, &sm.abort);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = i * 32 + lane, k = key & 15;
         const int to = (key & ~15) + ((k & 7) >> 1) * 4 + (k >> 3) * 2 + (k & 1);
-        const float v = fmaxf(vs[i], kVsMin);        // (NaN: fmaxf drops it ...
-        sm.place[in][key] = at[i];
-        sm.ks[in][to] = ks[i];
+        const float v = fmaxf(now.vs[i], kVsMin);    // (NaN: fmaxf drops it ...
+        sm.place[in][key] = now.at[i];
+        sm.ks[in][to] = now.ks[i];
         // ... and the rows that see it get NaN); a key that is not there: weight 0
-        sm.lv[in][to] = at[i] == 0xffffffffu ? kNegInf : vs[i] != vs[i] ? vs[i] : lg2(v);
+        sm.lv[in][to] = now.at[i] < 0 ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
         sm.rv[in][to] = rcp(v);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_full[in]);
+      now = next;
     }
-  } else if (lane == 0) {
+  } else if (warp == MMA_WARP && elect_one()) {
     // ------------------------------------------------------------------ products
-    uint32_t qa[2];
-    qa[0] = su32(sm.q[0]);
-    qa[1] = su32(sm.q[1]);
-    auto scores = [&](int t, int j) {   // S_t = Q_t K8_j^T
-      const uint32_t kb = su32(sm.kv[(2 * j) % RING]);
+    // descriptors: constant but for the start address (in 16-byte units) in the low bits
+    const uint64_t qd[2] = {sdesc_sw128(su32(sm.q[0])), sdesc_sw128(su32(sm.q[1]))};
+    const uint64_t kd = sdesc_sw128(su32(sm.kv[0]));
+    const uint64_t vd = sdesc_mn(su32(sm.kv[0]), HALVES == 2 ? HALF_BYTES : 16);
+    constexpr uint32_t SLOT = TC_KEYS * HD * 2 / 16;
+    auto scores = [&](const int t, int j) {   // S_t = Q_t K8_j^T
+      const uint64_t b = kd + static_cast<uint32_t>((2 * j) % RING) * SLOT;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
-        const uint32_t at = (k / 4) * HALF_BYTES + (k % 4) * 32;
-        mma_ss(tmem + t * 128, sdesc_sw128(qa[t] + at), sdesc_sw128(kb + at), ID_S, k != 0);
+        const uint32_t at = ((k / 4) * HALF_BYTES + (k % 4) * 32) / 16;
+        mma_ss(tmem + t * 128, qd[t] + at, b + at, ID_S, k != 0);
       }
       mma_commit(&sm.s_full[t]);
     };
-    auto values = [&](int t, int j) {   // O_t += P_t V8_j
-      const uint32_t vb = su32(sm.kv[(2 * j + 1) % RING]);
+    auto values = [&](const int t, int j) {   // O_t += P_t V8_j
+      const uint64_t b = vd + static_cast<uint32_t>((2 * j + 1) % RING) * SLOT;
 #pragma unroll
       for (int k = 0; k < TC_KEYS / 16; ++k)
-        mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + k * 8,
-               sdesc_mn(vb + k * 2048, HALVES == 2 ? HALF_BYTES : 16), ID_O, j > 0 || k > 0);
+        mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + k * 8, b + k * (2048 / 16), ID_O,
+               j > 0 || k > 0);
     };
     auto ready = [&](int item) {
       wait_bar(&sm.full[item % RING], (item / RING) & 1, &sm.abort);
@@ -646,23 +702,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     };
     if (nj > 0) {
       ready(0);
+#pragma unroll
       for (int t = 0; t < 2; ++t)
         if (jt[t] > 0) scores(t, 0);
       mma_commit(&sm.empty[0]);
     }
     for (int j = 0; j < nj; ++j) {
       ready(2 * j + 1);
-      if (j + 1 < nj) ready(2 * j + 2);
+#pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (j < jt[t]) {
           wait_bar(&sm.p_full[t], j & 1, &sm.abort);
           fence_after();
           values(t, j);
-          // these scores overwrite P_t: products of one thread run in order
-          if (j + 1 < jt[t]) scores(t, j + 1);
         }
+        if (t == 1) mma_commit(&sm.empty[(2 * j + 1) % RING]);
+        if (t == 0 && j + 1 < nj) ready(2 * j + 2);
+        // these scores overwrite P_t: products of one thread run in order
+        if (j + 1 < jt[t]) scores(t, j + 1);
       }
-      mma_commit(&sm.empty[(2 * j + 1) % RING]);
       if (j + 1 < nj) mma_commit(&sm.empty[(2 * j + 2) % RING]);
     }
     if (nj > 0) {
@@ -674,7 +732,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 15) tmem_dealloc<512>(tmem);
+  if (warp == MMA_WARP) tmem_dealloc<512>(tmem);
 }
 
 template <int HD>
