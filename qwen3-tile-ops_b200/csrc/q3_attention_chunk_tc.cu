@@ -5,11 +5,11 @@
 // head m % group of new row m / group, so a KV head is read once for its whole
 // group.  Two 128-row tiles take turns: while one tile's 128 x 128 scores
 // are exponentiated, the tensor cores work on the other's.
-//   warps 0-7    rows: four warps a tile, one TMEM lane quadrant each
-//   warps 8-11   codes of K and V from global memory, widened to f16 (exact), into a
+//   warps 0-15   rows: eight warps a tile, two a TMEM lane quadrant, 16 rows each
+//   warps 16-19  codes of K and V from global memory, widened to f16 (exact), into a
 //                ring of four operand tiles in the 128-byte-swizzled layout
-//   warp 12      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
-//   warp 13      issues the products: S = Q K8^T (both operands in shared
+//   warp 20      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
+//   warp 21      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
 // The loads are plain ones because each code passes through registers on its
 // way (the tensor cores take no f16 x int8); rows of pages of any length then need
@@ -35,9 +35,9 @@ namespace chunk {
 using namespace tcx;
 
 constexpr unsigned kErrWait = 1u << 18;
-constexpr int TC_THREADS = 512;
-constexpr int LOADERS = 4;                         // warps 8 .. 11
-constexpr int INFO_WARP = 12, MMA_WARP = 13;
+constexpr int ROW_WARPS = 16, LOADERS = 4;
+constexpr int INFO_WARP = ROW_WARPS + LOADERS, MMA_WARP = INFO_WARP + 1;
+constexpr int TC_THREADS = 768;                    // whole warpgroups: two warps idle
 constexpr int RING = 4;                            // operand tiles K0, V0, K1, V1, ...
 constexpr int INFO = 4;                            // key tiles whose places and scales are known
 constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
@@ -138,6 +138,15 @@ __device__ __forceinline__ void tm_st_p(uint32_t at, const uint32_t (&v)[16]) {
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tm_ld_p(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15},"
+      " [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(at));
+}
 // 32 columns of one row (lane)
 __device__ __forceinline__ void tm_ld_row(uint32_t at, float (&v)[32]) {
   asm volatile(
@@ -156,6 +165,12 @@ __device__ __forceinline__ void landed(float (&v)[16]) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
                  "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
                  "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+__device__ __forceinline__ void landed(uint32_t (&v)[16]) {
+  asm volatile(""
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
+                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
 }
 __device__ __forceinline__ void landed(float (&v)[32]) {
   landed(reinterpret_cast<float(&)[16]>(v[0]));
@@ -195,24 +210,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// One 128-key tile for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
-// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights in their place, sums at `ot` rescaled
-// when a row's maximum outgrows its reference by 2^8.
+// Half a key tile (64 keys) for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
+// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights at `pt`.  The reference of a row's
+// weights is a whole number and moves only when the maximum outgrows it by 2^8; then the sums at
+// `ot` (have_o) and the weights of the tile's first half (`first`) are multiplied by the power of
+// two between the references.
 template <int HD, bool MASK>
 __device__ __forceinline__ void rows16(const float *ks, const float *lv, const float *rv, uint32_t st,
-                                       uint32_t ot, bool have_o, const float (&a)[2], float (&mref)[2],
-                                       float (&l)[2], const int (&pos)[2], int key0, int causal,
-                                       int window) {
-  float x[4][16];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tm_ld(st + c * 32, x[c]);
+                                       uint32_t pt, uint32_t first, uint32_t ot, bool have_o,
+                                       const float (&a)[2], float (&mref)[2], float (&l)[2],
+                                       const int (&pos)[2], int key0, int causal, int window) {
+  float x[2][16];
+  tm_ld(st, x[0]);
+  tm_ld(st + 32, x[1]);
   tmem_wait_ld();
-#pragma unroll
-  for (int c = 0; c < 4; ++c) landed(x[c]);
+  landed(x[0]);
+  landed(x[1]);
   const F2 a0 = f2(a[0], a[0]), a1 = f2(a[1], a[1]);
   float mx0 = kNegInf, mx1 = kNegInf;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {                    // 16 keys: column groups 2k and 2k + 1
+  for (int k = 0; k < 4; ++k) {                    // 16 keys: column groups 2k and 2k + 1
     const float4 kk = *reinterpret_cast<const float4 *>(ks + k * 16);
     const float4 ll = *reinterpret_cast<const float4 *>(lv + k * 16);
 #pragma unroll
@@ -239,10 +256,11 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
   mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
   const bool g0 = mx0 > __fadd_rn(mref[0], 8.0f), g1 = mx1 > __fadd_rn(mref[1], 8.0f);
   if (__any_sync(0xffffffffu, g0 || g1)) {
-    const float r0 = g0 ? ex2(__fsub_rn(mref[0], mx0)) : 1.0f;
-    const float r1 = g1 ? ex2(__fsub_rn(mref[1], mx1)) : 1.0f;
-    mref[0] = g0 ? mx0 : mref[0];
-    mref[1] = g1 ? mx1 : mref[1];
+    const float m0 = ceilf(mx0), m1 = ceilf(mx1);
+    const float r0 = g0 ? ex2(__fsub_rn(mref[0], m0)) : 1.0f;
+    const float r1 = g1 ? ex2(__fsub_rn(mref[1], m1)) : 1.0f;
+    mref[0] = g0 ? m0 : mref[0];
+    mref[1] = g1 ? m1 : mref[1];
     l[0] = __fmul_rn(l[0], r0);
     l[1] = __fmul_rn(l[1], r1);
     if (have_o) {   // the products before this tile's have completed with its scores
@@ -256,35 +274,44 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
         for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(o[i], (i & 2) ? r1 : r0);
         tm_st(ot + c * 32, o);
       }
+    }
+    if (pt != first) {
       tmem_wait_st();
+      uint32_t w[16];
+      tm_ld_p(first, w);
+      tmem_wait_ld();
+      landed(w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        const float r = (i & 1) ? r1 : r0;
+        w[i] = pack_f16(__fmul_rn(y.x, r), __fmul_rn(y.y, r));
+      }
+      tm_st_p(first, w);
     }
   }
   const float b0 = mref[0] == kNegInf ? 0.0f : -mref[0], b1 = mref[1] == kNegInf ? 0.0f : -mref[1];
   const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
   F2 s0 = f2(0.0f, 0.0f), s1 = s0;
+  uint32_t w[16];
 #pragma unroll
-  for (int c2 = 0; c2 < 2; ++c2) {                 // 64 keys: 32 columns of P
-    uint32_t w[16];
+  for (int k = 0; k < 4; ++k) {
+    const float4 rr = *reinterpret_cast<const float4 *>(rv + k * 16);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int k = c2 * 4 + kk;
-      const float4 rr = *reinterpret_cast<const float4 *>(rv + k * 16);
+    for (int h = 0; h < 2; ++h) {
+      float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
+      un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
+      un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
-        un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
-        un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
-        const F2 r2 = h ? f2(rr.z, rr.w) : f2(rr.x, rr.y);
-        s0 = fma2(f2(y[0], y[1]), r2, s0);
-        s1 = fma2(f2(y[2], y[3]), r2, s1);
-        w[(kk * 2 + h) * 2] = pack_f16(y[0], y[1]);
-        w[(kk * 2 + h) * 2 + 1] = pack_f16(y[2], y[3]);
-      }
+      for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
+      const F2 r2 = h ? f2(rr.z, rr.w) : f2(rr.x, rr.y);
+      s0 = fma2(f2(y[0], y[1]), r2, s0);
+      s1 = fma2(f2(y[2], y[3]), r2, s1);
+      w[(k * 2 + h) * 2] = pack_f16(y[0], y[1]);
+      w[(k * 2 + h) * 2 + 1] = pack_f16(y[2], y[3]);
     }
-    tm_st_p(st + c2 * 32, w);
   }
+  tm_st_p(pt, w);
   float u, v;
   un(s0, u, v);
   l[0] = __fadd_rn(l[0], __fadd_rn(u, v));
@@ -298,7 +325,7 @@ __device__ __forceinline__ bool elect_one() {   // one lane of the converged war
   return r != 0;
 }
 __device__ __forceinline__ void asm_less_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 }
 
 __device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
@@ -334,11 +361,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       }
       for (int i = 0; i < INFO; ++i) {
         mbar_init(&sm.info_full[i], 1);
-        mbar_init(&sm.info_empty[i], LOADERS + 8);
+        mbar_init(&sm.info_empty[i], LOADERS + ROW_WARPS);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], 128);
+        mbar_init(&sm.p_full[i], ROW_WARPS / 2);
       }
       mbar_init(&sm.o_full, 1);
       mbar_init_fence();
@@ -378,8 +405,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   {
     constexpr int N = HD / 32;
 #pragma unroll 4
-    for (int i = 0; i < TC_ROWS / 16; ++i) {
-      const int m = warp * (TC_ROWS / 16) + i;
+    for (int m = warp; m < TC_ROWS; m += TC_THREADS / 32) {
       Elems<__half, N> e;
 #pragma unroll
       for (int k = 0; k < N; ++k) e.e[k] = __ushort_as_half(0);
@@ -421,83 +447,86 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   fence_after();
   const uint32_t tmem = sm.tmem;
 
-  // registers move from the other warps to those of the rows (2 x 128 x 168 + 2 x 128 x 88 is the
-  // launch's 512 x 128)
-  if (warp < 8) {
+  // registers move from the other warps to those of the rows: 4 x 128 x 88 + 2 x 128 x 64 is the
+  // launch's 768 x 80
+  if (warp < ROW_WARPS) {
     // ------------------------------------------------------------------ rows
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    const int t = warp >> 2, qd = warp & 3, g = lane >> 2, t4 = lane & 3;
-    // this thread's rows, by pass (16 lanes of the quadrant) and half: t*128 + qd*32 + 16 ps + 8 e + g
-    float a[2][2], mref[2][2], l[2][2];
-    int pos[2][2];
-    const int rb = t * 128 + qd * 32;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    // warp: tile t, lane quadrant qd, its 16 rows ps; thread: rows rb + 8 e + g
+    const int t = warp >> 3, ps = (warp >> 2) & 1, qd = warp & 3, g = lane >> 2, t4 = lane & 3;
+    float a[2], mref[2], l[2];
+    int pos[2];
+    const int rb = t * 128 + qd * 32 + ps * 16;
 #pragma unroll
-    for (int ps = 0; ps < 2; ++ps)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int m = rb + 16 * ps + 8 * e + g;
-        a[ps][e] = sm.a[m];
-        pos[ps][e] = q.pos0 + min(m0 + m, packed - 1) / p.group;
-        mref[ps][e] = kNegInf;
-        l[ps][e] = 0.0f;
-      }
+    for (int e = 0; e < 2; ++e) {
+      const int m = rb + 8 * e + g;
+      a[e] = sm.a[m];
+      pos[e] = q.pos0 + min(m0 + m, packed - 1) / p.group;
+      mref[e] = kNegInf;
+      l[e] = 0.0f;
+    }
     const int pmin = q.pos0 + min(m0 + rb, packed - 1) / p.group;
-    const int pmax = q.pos0 + min(m0 + rb + 31, packed - 1) / p.group;
+    const int pmax = q.pos0 + min(m0 + rb + 15, packed - 1) / p.group;
+    const int mine = t ? jt[1] : jt[0];
+    const uint32_t st = tmem + (static_cast<uint32_t>(qd * 32 + ps * 16) << 16) + t * 128;
     for (int j = 0; j < nj; ++j) {
       const int in = j % INFO;
       wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
-      if (j < jt[t]) {
+      if (j < mine) {
         wait_bar(&sm.s_full[t], j & 1, &sm.abort);
         fence_after();
         const int key0 = (z0 + j) * TC_KEYS;
         const bool masked = (p.causal && key0 + TC_KEYS - 1 > pmin) ||
                             (p.window > 0 && key0 <= pmax - p.window);
-#pragma unroll
-        for (int ps = 0; ps < 2; ++ps) {
-          const uint32_t lanes = static_cast<uint32_t>(qd * 32 + ps * 16) << 16;
-          const uint32_t st = tmem + lanes + t * 128, ot = tmem + lanes + TMEM_O + t * 128;
-          if (masked)
-            rows16<HD, true>(sm.ks[in] + t4 * 4, sm.lv[in] + t4 * 4, sm.rv[in] + t4 * 4, st, ot, j > 0,
-                             a[ps], mref[ps], l[ps], pos[ps], key0 + t4 * 2, p.causal, p.window);
-          else
-            rows16<HD, false>(sm.ks[in] + t4 * 4, sm.lv[in] + t4 * 4, sm.rv[in] + t4 * 4, st, ot, j > 0,
-                              a[ps], mref[ps], l[ps], pos[ps], key0 + t4 * 2, p.causal, p.window);
+        const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
+        if (masked) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h)
+            rows16<HD, true>(ks + h * 64, lv + h * 64, rv + h * 64, st + h * 64, st + h * 32, st,
+                             st + TMEM_O, j > 0, a, mref, l, pos, key0 + h * 64 + t4 * 2, p.causal,
+                             p.window);
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h)
+            rows16<HD, false>(ks + h * 64, lv + h * 64, rv + h * 64, st + h * 64, st + h * 32, st,
+                              st + TMEM_O, j > 0, a, mref, l, pos, key0 + h * 64 + t4 * 2, p.causal,
+                              p.window);
         }
         tmem_wait_st();
         fence_before();
-        mbar_arrive(&sm.p_full[t]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[t]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[in]);
     }
-    // ---- sums of the rows, then each thread its own row
+    // ---- sums of the rows; then each thread half the columns of its own row
 #pragma unroll
-    for (int ps = 0; ps < 2; ++ps)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float y = l[ps][e];
-        y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 1));
-        y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 2));
-        if (t4 == 0) {
-          sm.l[rb + 16 * ps + 8 * e + g] = y;
-          sm.m[rb + 16 * ps + 8 * e + g] = mref[ps][e];
-        }
+    for (int e = 0; e < 2; ++e) {
+      float y = l[e];
+      y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 1));
+      y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 2));
+      if (t4 == 0) {
+        sm.l[rb + 8 * e + g] = y;
+        sm.m[rb + 8 * e + g] = mref[e];
       }
-    __syncwarp();
+    }
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");   // the eight warps of the tile
     if (nj > 0) wait_bar(&sm.o_full, 0, &sm.abort);
     fence_after();
-    const int m = rb + lane;
+    const int m = t * 128 + qd * 32 + lane;
     const bool have = m < rows;
     const int mm = min(m0 + m, packed - 1);
     const long r = q.first + mm / p.group;
     const int h = kvh * p.group + mm % p.group;
     const uint32_t src = tmem + (static_cast<uint32_t>(qd * 32) << 16) + TMEM_O + t * 128;
     const float lsum = sm.l[m];
+    constexpr int OC = HD / 64;                    // 32-column chunks a thread stores, from ps * OC
     if (p.splits > 1) {
       const long at = (static_cast<long>(blockIdx.z) * p.rows + r) * p.heads + h;
-      if (jt[t] > 0) {
+      if (mine > 0) {
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = ps * OC; c < ps * OC + OC; ++c) {
           Elems<float, 32> o;
           tm_ld_row(src + c * 32, o.e);
           tmem_wait_ld();
@@ -506,18 +535,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
           __syncwarp();
         }
       }
-      if (have) {
-        p.part_ml[at * 2] = jt[t] > 0 ? sm.m[m] : kNegInf;
-        p.part_ml[at * 2 + 1] = jt[t] > 0 ? lsum : 0.0f;
+      if (have && ps == 0) {
+        p.part_ml[at * 2] = mine > 0 ? sm.m[m] : kNegInf;
+        p.part_ml[at * 2 + 1] = mine > 0 ? lsum : 0.0f;
       }
-    } else if (jt[t] > 0) {
+    } else if (mine > 0) {
       const float inv = lsum == 0.0f ? 0.0f : __fdiv_rn(1.0f, lsum);   // no key seen: zeros
       char *out = p.o + r * p.o_rb;
       const long col = static_cast<long>(h) * HD;
       float scale = 0.0f;
       if (p.o_dt == Q3_DT_I8) {
         float mx = 0.0f;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           float o[32];
           tm_ld_row(src + c * 32, o);
@@ -527,10 +556,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
           for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(__fmul_rn(o[i], inv)));
         }
         scale = __fmul_rn(mx, kInv127);
-        if (have) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
+        if (have && ps == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
       }
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
+#pragma unroll 1
+      for (int c = ps * OC; c < ps * OC + OC; ++c) {
         float o[32];
         tm_ld_row(src + c * 32, o);
         tmem_wait_ld();
@@ -554,13 +583,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         __syncwarp();
       }
     }
-    __syncwarp();
-  } else if (asm_less_registers(), warp < 8 + LOADERS) {
+  } else if (asm_less_registers(), warp < INFO_WARP) {
     // ------------------------------------------------------------------ codes of K and V
     // Operand tile `item` (K and V in turn): a warp takes 32 key rows in chunks of CR rows, one
     // 16-byte load a lane; a chunk of the next item is requested as soon as this item's is stored.
     constexpr int CR = HD == 128 ? 4 : 8, CHUNKS = 32 / CR;
-    const int lw = warp - 8, items = 2 * nj;
+    const int lw = warp - ROW_WARPS, items = 2 * nj;
     // eight lanes take 4 chunks of two rows: their f16 chunks then lie in 8 different places of a
     // 128-byte line
     const int rowl = HD == 128 ? 2 * (lane >> 4) + ((lane >> 2) & 1) : lane >> 2;
