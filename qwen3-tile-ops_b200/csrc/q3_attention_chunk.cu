@@ -95,6 +95,11 @@ __device__ __forceinline__ long count_units(const Args &p, int n, int lane, unsi
   for (int s = lane; s < n; s += 32) x += units_of(p, s, err);
   return warp_sum(x);
 }
+__device__ __forceinline__ long count_units_from(const Args &p, int s0, int lane, unsigned *err) {
+  long x = 0;
+  for (int s = s0 + lane; s < p.n_seqs; s += 32) x += units_of(p, s, err);
+  return warp_sum(x);
+}
 // workers that share `total` units of a grid of `all` warps, and the first unit of worker w
 __device__ __forceinline__ long workers(long total, long all) {
   const long n = (total + MIN_UNITS - 1) / MIN_UNITS;
@@ -492,33 +497,31 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
   pdl_trigger();
 }
 
-// The parts of one (row, head) joined by a CTA: warps take them in turn.
+// The parts of a (sequence, KV head) pair joined by a CTA; its warps take the parts of a row in turn.
 template <int HD>
 __global__ void __launch_bounds__(WARPS * 32) k_attn_join(const Args p, long all_workers) {
   constexpr int N = HD / 32;
   __shared__ float so[WARPS][HD], sm[WARPS], sl[WARPS];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long r = blockIdx.x;
-  const int h = blockIdx.y;
-  int first, count;
-  const int s = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
-  if (s < 0) return;
+  const int s = blockIdx.x, kvh = blockIdx.y;
   unsigned err = 0;
   const Seq q = load_seq(p, s, &err);
   int pb0;
   const int pn = pair_units(p, q, pb0);
-  if (pn == 0) return;                             // refused, or the other kernel's
+  const int m = blockIdx.z;                        // packed row
+  if (pn == 0 || m >= q.n * p.group) return;       // refused, or the other kernel's
+  const long r = q.first + m / p.group;
+  const int h = kvh * p.group + m % p.group;
   const long before = count_units(p, s, lane, &err);
-  const long total = count_units(p, p.n_seqs, lane, &err);
+  const long total = before + count_units_from(p, s, lane, &err);
   const long nw = workers(total, all_workers);
   // the pair's units, and the workers that have them
-  const long a = before + static_cast<long>(h / p.group) * pn, b = a + pn;
+  const long a = before + static_cast<long>(kvh) * pn, b = a + pn;
   long w0 = a * nw / total, w1 = (b - 1) * nw / total;
   while (w0 + 1 < nw && first_unit(total, nw, w0 + 1) <= a) ++w0;
   while (w1 + 1 < nw && first_unit(total, nw, w1 + 1) <= b - 1) ++w1;
   if (w0 == w1) return;                            // stored whole
   pdl_wait();
-  const int m = static_cast<int>(r - q.first) * p.group + h % p.group;
   float mm = kNegInf, l = 0.0f, x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
@@ -677,7 +680,7 @@ static int launch_few(const chunk::Args &p, int ctas, cudaStream_t s) {
   Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
   chunk::k_attn_few<HD, NT><<<ctas, chunk::WARPS * 32, smem, s>>>(p);
   Q3_TRY(launch_status());
-  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.rows, p.heads), dim3(chunk::WARPS * 32), 0, s,
+  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, p.part_rows), dim3(chunk::WARPS * 32), 0, s,
                    p, static_cast<long>(ctas) * chunk::WARPS);
 }
 

@@ -6,10 +6,10 @@
 // group.  Two 128-row tiles take turns: while one tile's 128 x 128 scores
 // are exponentiated, the tensor cores work on the other's.
 //   warps 0-15   rows: eight warps a tile, two a TMEM lane quadrant, 16 rows each
-//   warps 16-19  codes of K and V from global memory, widened to f16 (exact), into a
+//   warps 16-23  codes of K and V from global memory, widened to f16 (exact), into a
 //                ring of four operand tiles in the 128-byte-swizzled layout
-//   warp 20      page lookups, and the keys' scales as ks, log2 vs and 1 / vs
-//   warp 21      issues the products: S = Q K8^T (both operands in shared
+//   warp 24      page lookups, and the keys' scales as ks qk_scale log2 e, log2 vs, 1 / vs
+//   warp 25      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
 // The loads are plain ones because each code passes through registers on its
 // way (the tensor cores take no f16 x int8); rows of pages of any length then need
@@ -35,9 +35,9 @@ namespace chunk {
 using namespace tcx;
 
 constexpr unsigned kErrWait = 1u << 18;
-constexpr int ROW_WARPS = 16, LOADERS = 4;
+constexpr int ROW_WARPS = 16, LOADERS = 8;
 constexpr int INFO_WARP = ROW_WARPS + LOADERS, MMA_WARP = INFO_WARP + 1;
-constexpr int TC_THREADS = 768;                    // whole warpgroups: two warps idle
+constexpr int TC_THREADS = 896;                    // whole warpgroups: two warps idle
 constexpr int RING = 4;                            // operand tiles K0, V0, K1, V1, ...
 constexpr int INFO = 4;                            // key tiles whose places and scales are known
 constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
@@ -211,11 +211,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Half a key tile (64 keys) for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
-// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights at `pt`.  The reference of a row's
-// weights is a whole number and moves only when the maximum outgrows it by 2^8; then the sums at
-// `ot` (have_o) and the weights of the tile's first half (`first`) are multiplied by the power of
-// two between the references.
-template <int HD, bool MASK>
+// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights at `pt`.  ks holds ks qk_scale log2 e;
+// UNIT: a = 1 in all rows.  The reference of a row's weights is a whole number and moves only when
+// a weight outgrows it by 2^8, which a vote tells, so no row maximum is formed otherwise; then the
+// sums at `ot` (have_o) and the weights of the tile's first half (`first`) are multiplied by the
+// power of two between the references.
+template <int HD, bool MASK, bool UNIT>
 __device__ __forceinline__ void rows16(const float *ks, const float *lv, const float *rv, uint32_t st,
                                        uint32_t pt, uint32_t first, uint32_t ot, bool have_o,
                                        const float (&a)[2], float (&mref)[2], float (&l)[2],
@@ -227,6 +228,8 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
   landed(x[0]);
   landed(x[1]);
   const F2 a0 = f2(a[0], a[0]), a1 = f2(a[1], a[1]);
+  float b0 = mref[0] == kNegInf ? 0.0f : -mref[0], b1 = mref[1] == kNegInf ? 0.0f : -mref[1];
+  const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
   float mx0 = kNegInf, mx1 = kNegInf;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {                    // 16 keys: column groups 2k and 2k + 1
@@ -236,8 +239,13 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
     for (int h = 0; h < 2; ++h) {
       float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
       const F2 k2 = h ? f2(kk.z, kk.w) : f2(kk.x, kk.y), l2 = h ? f2(ll.z, ll.w) : f2(ll.x, ll.y);
-      un(fma2(mul2(f2(y[0], y[1]), k2), a0, l2), y[0], y[1]);
-      un(fma2(mul2(f2(y[2], y[3]), k2), a1, l2), y[2], y[3]);
+      if (UNIT) {
+        un(add2(fma2(f2(y[0], y[1]), k2, l2), n0), y[0], y[1]);
+        un(add2(fma2(f2(y[2], y[3]), k2, l2), n1), y[2], y[3]);
+      } else {
+        un(add2(fma2(mul2(f2(y[0], y[1]), k2), a0, l2), n0), y[0], y[1]);
+        un(add2(fma2(mul2(f2(y[2], y[3]), k2), a1, l2), n1), y[2], y[3]);
+      }
       if (MASK) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -250,17 +258,24 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
       mx1 = max3(mx1, y[2], y[3]);
     }
   }
-  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-  const bool g0 = mx0 > __fadd_rn(mref[0], 8.0f), g1 = mx1 > __fadd_rn(mref[1], 8.0f);
-  if (__any_sync(0xffffffffu, g0 || g1)) {
-    const float m0 = ceilf(mx0), m1 = ceilf(mx1);
-    const float r0 = g0 ? ex2(__fsub_rn(mref[0], m0)) : 1.0f;
-    const float r1 = g1 ? ex2(__fsub_rn(mref[1], m1)) : 1.0f;
-    mref[0] = g0 ? m0 : mref[0];
-    mref[1] = g1 ? m1 : mref[1];
+  const bool grow = fmaxf(mx0, mx1) > 8.0f || mref[0] == kNegInf || mref[1] == kNegInf;
+  if (__any_sync(0xffffffffu, grow)) {
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    // maxima relative to the old references (0 where there was none yet)
+    const bool g0 = mx0 > (mref[0] == kNegInf ? kNegInf : 8.0f);
+    const bool g1 = mx1 > (mref[1] == kNegInf ? kNegInf : 8.0f);
+    const float u0 = g0 ? -ceilf(mx0) : 0.0f, u1 = g1 ? -ceilf(mx1) : 0.0f;
+    // powers of two; without a reference all sums are still zero
+    const float r0 = mref[0] == kNegInf ? 1.0f : ex2(u0), r1 = mref[1] == kNegInf ? 1.0f : ex2(u1);
+    b0 = __fadd_rn(b0, u0);
+    b1 = __fadd_rn(b1, u1);
+    mref[0] = g0 ? -b0 : mref[0];
+    mref[1] = g1 ? -b1 : mref[1];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = __fadd_rn(x[i >> 4][i & 15], (i & 2) ? u1 : u0);
     l[0] = __fmul_rn(l[0], r0);
     l[1] = __fmul_rn(l[1], r1);
     if (have_o) {   // the products before this tile's have completed with its scores
@@ -290,8 +305,6 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
       tm_st_p(first, w);
     }
   }
-  const float b0 = mref[0] == kNegInf ? 0.0f : -mref[0], b1 = mref[1] == kNegInf ? 0.0f : -mref[1];
-  const F2 n0 = f2(b0, b0), n1 = f2(b1, b1);
   F2 s0 = f2(0.0f, 0.0f), s1 = s0;
   uint32_t w[16];
 #pragma unroll
@@ -300,8 +313,6 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float *y = &x[k >> 1][((k & 1) * 2 + h) * 4];
-      un(add2(f2(y[0], y[1]), n0), y[0], y[1]);
-      un(add2(f2(y[2], y[3]), n1), y[2], y[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = ex2(y[i]);
       const F2 r2 = h ? f2(rr.z, rr.w) : f2(rr.x, rr.y);
@@ -324,8 +335,12 @@ __device__ __forceinline__ bool elect_one() {   // one lane of the converged war
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
   return r != 0;
 }
+// the row warps and the MMA warp: queries staged, TMEM allocated
+__device__ __forceinline__ void start_sync() {
+  asm volatile("bar.sync 3, %0;" ::"n"((ROW_WARPS + 1) * 32) : "memory");
+}
 __device__ __forceinline__ void asm_less_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
 }
 
 __device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
@@ -340,8 +355,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   constexpr int HALF_BYTES = 128 * 128;            // 128 rows (or keys) of 64 f16
   constexpr uint32_t ID_S = idesc_f16(TC_KEYS, false), ID_O = idesc_f16(HD, true);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TcSmem<HD> &sm = *reinterpret_cast<TcSmem<HD> *>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // (an offset, not a rounded address: accesses stay shared-memory accesses)
+  TcSmem<HD> &sm = *reinterpret_cast<TcSmem<HD> *>(smem_raw + ((0u - su32(smem_raw)) & 1023u));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y;
 
@@ -399,59 +414,70 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     }
     nj = max(jt[0], jt[1]);
   }
-  if (warp == MMA_WARP) tmem_alloc<512>(&sm.tmem);
-
-  // ---- queries as f16 in the operand layout, and each row's a
-  {
-    constexpr int N = HD / 32;
-#pragma unroll 4
-    for (int m = warp; m < TC_ROWS; m += TC_THREADS / 32) {
-      Elems<__half, N> e;
-#pragma unroll
-      for (int k = 0; k < N; ++k) e.e[k] = __ushort_as_half(0);
-      float scale = 0.0f;
-      if (m < rows) {
-        const long r = q.first + (m0 + m) / p.group;
-        const int h = kvh * p.group + (m0 + m) % p.group;
-        const char *qp = p.q + r * p.q_rb;
-        const long col = static_cast<long>(h) * HD + lane * N;
-        if (p.q_dt == Q3_DT_I8) {
-          Elems<int8_t, N> c;
-          c.load(qp + col);
-          scale = reinterpret_cast<const float *>(p.qs + r * p.qs_rb)[h];
-#pragma unroll
-          for (int k = 0; k < N; ++k) e.e[k] = __int2half_rn(c.e[k]);
-        } else if (p.q_dt == Q3_DT_F16) {
-          e.load(qp + col * 2);
-          scale = 1.0f;
-        } else {
-          Elems<__nv_bfloat16, N> c;
-          c.load(qp + col * 2);
-          float mx = 0.0f, up;
-#pragma unroll
-          for (int k = 0; k < N; ++k) mx = fmaxf(mx, fabsf(to_f32(c.e[k])));
-          bf16_scale(warp_tree_max(mx), up, scale);
-#pragma unroll
-          for (int k = 0; k < N; ++k) e.e[k] = __float2half_rn(__fmul_rn(to_f32(c.e[k]), up));
-        }
-      }
-      const int d = lane * N, r = m & 127;
-      e.store(sm.q[m >> 7] + (d / 64) * HALF_BYTES + r * 128 + ((((d % 64) / 8) ^ (r & 7)) * 16) +
-              (d % 8) * 2);
-      if (lane == 0) sm.a[m] = __fmul_rn(scale, p.scale_log2);
-    }
-  }
-  fence_proxy_async();
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const uint32_t tmem = sm.tmem;
-
-  // registers move from the other warps to those of the rows: 4 x 128 x 88 + 2 x 128 x 64 is the
-  // launch's 768 x 80
+  // registers move from the other warps to those of the rows: 4 x 128 x 88 + 3 x 128 x 48 is
+  // within the launch's 896 x 72
   if (warp < ROW_WARPS) {
     // ------------------------------------------------------------------ rows
     asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    // ---- queries as f16 in the operand layout and each row's a: 8 columns a thread at a time
+    {
+      constexpr int G8 = HD / 8, EACH = TC_ROWS * G8 / (ROW_WARPS * 32);
+      uint4 raw[EACH];
+      float qs[EACH];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int id = i * ROW_WARPS * 32 + threadIdx.x, m = id / G8;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        qs[i] = 0.0f;
+        if (m < rows) {
+          const int mm = m0 + m;
+          const long r = q.first + mm / p.group;
+          const int h = kvh * p.group + mm % p.group;
+          const char *qp = p.q + r * p.q_rb;
+          const long col = static_cast<long>(h) * HD + (id % G8) * 8;
+          qs[i] = 1.0f;
+          if (p.q_dt == Q3_DT_I8) {
+            *reinterpret_cast<uint2 *>(&raw[i]) = *reinterpret_cast<const uint2 *>(qp + col);
+            qs[i] = reinterpret_cast<const float *>(p.qs + r * p.qs_rb)[h];
+          } else {
+            raw[i] = *reinterpret_cast<const uint4 *>(qp + col * 2);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int id = i * ROW_WARPS * 32 + threadIdx.x, m = id / G8, d8 = id % G8;
+        uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        if (p.q_dt == Q3_DT_I8) {
+          const uint32_t lo = w[0] ^ 0x80808080u, hi = w[1] ^ 0x80808080u;
+          w[0] = f16_pair(lo, 0x4140), w[1] = f16_pair(lo, 0x4342);
+          w[2] = f16_pair(hi, 0x4140), w[3] = f16_pair(hi, 0x4342);
+        } else if (p.q_dt == Q3_DT_BF16) {
+          float mx = 0.0f, up = 1.0f, down = 1.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[k] << 16)),
+                                 fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+#pragma unroll
+          for (int o = 1; o < G8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          // within [2^-6, 2^15) f16 holds the row as it is (to 2^-19 of its maximum)
+          if (mx != 0.0f && !(mx >= 0.015625f && mx < 32768.0f)) bf16_scale(mx, up, down);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = pack_f16(__fmul_rn(__uint_as_float(w[k] << 16), up),
+                            __fmul_rn(__uint_as_float(w[k] & 0xffff0000u), up));
+          qs[i] = __fmul_rn(qs[i], down);
+        }
+        const int r = m & 127;
+        *reinterpret_cast<uint4 *>(sm.q[m >> 7] + (d8 / 8) * HALF_BYTES + r * 128 +
+                                   (((d8 % 8) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (d8 == 0) sm.a[m] = qs[i];
+      }
+    }
+    fence_proxy_async();
+    start_sync();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
     // warp: tile t, lane quadrant qd, its 16 rows ps; thread: rows rb + 8 e + g
     const int t = warp >> 3, ps = (warp >> 2) & 1, qd = warp & 3, g = lane >> 2, t4 = lane & 3;
     float a[2], mref[2], l[2];
@@ -465,6 +491,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       mref[e] = kNegInf;
       l[e] = 0.0f;
     }
+    const bool unit = __all_sync(0xffffffffu, a[0] == 1.0f && a[1] == 1.0f);
     const int pmin = q.pos0 + min(m0 + rb, packed - 1) / p.group;
     const int pmax = q.pos0 + min(m0 + rb + 15, packed - 1) / p.group;
     const int mine = t ? jt[1] : jt[0];
@@ -479,18 +506,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         const bool masked = (p.causal && key0 + TC_KEYS - 1 > pmin) ||
                             (p.window > 0 && key0 <= pmax - p.window);
         const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
-        if (masked) {
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-            rows16<HD, true>(ks + h * 64, lv + h * 64, rv + h * 64, st + h * 64, st + h * 32, st,
-                             st + TMEM_O, j > 0, a, mref, l, pos, key0 + h * 64 + t4 * 2, p.causal,
-                             p.window);
-        } else {
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-            rows16<HD, false>(ks + h * 64, lv + h * 64, rv + h * 64, st + h * 64, st + h * 32, st,
-                              st + TMEM_O, j > 0, a, mref, l, pos, key0 + h * 64 + t4 * 2, p.causal,
-                              p.window);
+        for (int h = 0; h < 2; ++h) {
+          const int at = h * 64, k0 = key0 + at + t4 * 2;
+          if (masked)
+            rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
+                                    j > 0, a, mref, l, pos, k0, p.causal, p.window);
+          else if (unit)
+            rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
+                                    j > 0, a, mref, l, pos, k0, p.causal, p.window);
+          else
+            rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
+                                     j > 0, a, mref, l, pos, k0, p.causal, p.window);
         }
         tmem_wait_st();
         fence_before();
@@ -585,9 +612,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     }
   } else if (asm_less_registers(), warp < INFO_WARP) {
     // ------------------------------------------------------------------ codes of K and V
-    // Operand tile `item` (K and V in turn): a warp takes 32 key rows in chunks of CR rows, one
+    // Operand tile `item` (K and V in turn): a warp takes WR key rows in chunks of CR rows, one
     // 16-byte load a lane; a chunk of the next item is requested as soon as this item's is stored.
-    constexpr int CR = HD == 128 ? 4 : 8, CHUNKS = 32 / CR;
+    constexpr int WR = TC_KEYS / LOADERS, CR = HD == 128 ? 4 : 8, CHUNKS = WR / CR;
     const int lw = warp - ROW_WARPS, items = 2 * nj;
     // eight lanes take 4 chunks of two rows: their f16 chunks then lie in 8 different places of a
     // 128-byte line
@@ -595,7 +622,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     const int c = HD == 128 ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane & 3;
     const char *base[2] = {p.k + static_cast<long>(kvh) * HD + c * 16,
                            p.v + static_cast<long>(kvh) * HD + c * 16};
-    const int row0 = lw * 32 + rowl;
+    const int row0 = lw * WR + rowl;
     const uint32_t to = static_cast<uint32_t>((c >> 2) * HALF_BYTES + row0 * 128);
     const int ch = (c & 3) * 2;
     uint4 buf[CHUNKS];
@@ -692,7 +719,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         const int to = (key & ~15) + ((k & 7) >> 1) * 4 + (k >> 3) * 2 + (k & 1);
         const float v = fmaxf(now.vs[i], kVsMin);    // (NaN: fmaxf drops it ...
         sm.place[in][key] = now.at[i];
-        sm.ks[in][to] = now.ks[i];
+        sm.ks[in][to] = __fmul_rn(now.ks[i], p.scale_log2);
         // ... and the rows that see it get NaN); a key that is not there: weight 0
         sm.lv[in][to] = now.at[i] < 0 ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
         sm.rv[in][to] = rcp(v);
@@ -701,8 +728,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       if (lane == 0) mbar_arrive(&sm.info_full[in]);
       now = next;
     }
-  } else if (warp == MMA_WARP && elect_one()) {
+  } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------------ products
+    tmem_alloc<512>(&sm.tmem);
+    fence_before();
+    start_sync();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+    if (elect_one()) {
     // descriptors: constant but for the start address (in 16-byte units) in the low bits
     const uint64_t qd[2] = {sdesc_sw128(su32(sm.q[0])), sdesc_sw128(su32(sm.q[1]))};
     const uint64_t kd = sdesc_sw128(su32(sm.kv[0]));
@@ -755,12 +788,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       mma_commit(&sm.o_full);
       wait_bar(&sm.o_full, 0, &sm.abort);
     }
+    }
+    __syncwarp();
   }
 
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == MMA_WARP) tmem_dealloc<512>(tmem);
+  if (warp == MMA_WARP) tmem_dealloc<512>(sm.tmem);
 }
 
 template <int HD>
