@@ -136,10 +136,6 @@ __device__ __forceinline__ void store_part8(const Args &p, long r, int h, int g,
   }
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool ok) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0)
                : "memory");

@@ -132,6 +132,10 @@ __device__ __forceinline__ void store_out(const Args &p, long r, int h, int lane
   }
 }
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+               : "memory");
+}
 // Sequence of unit `unit` when sequence s has units(s) of them (whole warp); before: those of the
 // sequences before it.  -1: there is no such unit.
 template <typename F>

@@ -3,11 +3,12 @@
 //
 // CTA = (sequence, 256 packed rows, KV head, part of the keys); packed row m is
 // head m % group of new row m / group, so a KV head is read once for its whole
-// group.  Two 128-row tiles take turns: while one tile's 128 x 128 scores
-// are exponentiated, the tensor cores work on the other's.
+// group.  Two 128-row tiles of scores by halves of a key tile (128 rows x 64 keys), two
+// halves each in TMEM: while the rows turn one into weights, the tensor cores use
+// the weights of another and form the scores after it.
 //   warps 0-15   rows: eight warps a tile, two a TMEM lane quadrant, 16 rows each
 //   warps 16-23  codes of K and V from global memory, widened to f16 (exact), into a
-//                ring of four operand tiles in the 128-byte-swizzled layout
+//                ring of three operand tiles in the 128-byte-swizzled layout
 //   warp 24      page lookups, and the keys' scales as ks qk_scale log2 e, log2 vs, 1 / vs
 //   warp 25      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
@@ -38,7 +39,8 @@ constexpr unsigned kErrWait = 1u << 18;
 constexpr int ROW_WARPS = 16, LOADERS = 8;
 constexpr int INFO_WARP = ROW_WARPS + LOADERS, MMA_WARP = INFO_WARP + 1;
 constexpr int TC_THREADS = 896;                    // whole warpgroups: two warps idle
-constexpr int RING = 4;                            // operand tiles K0, V0, K1, V1, ...
+constexpr int RING = 3;                            // operand tiles K0, V0, K1, V1, ...
+constexpr int RAW = 3;                             // their codes, loaded or on the way
 constexpr int INFO = 4;                            // key tiles whose places and scales are known
 constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
 
@@ -46,13 +48,14 @@ template <int HD>
 struct TcSmem {
   alignas(1024) uint8_t q[2][128 * HD * 2];        // [64-column half][row][128 bytes], swizzled
   alignas(1024) uint8_t kv[RING][TC_KEYS * HD * 2];// [64-column half][key][128 bytes], swizzled
+  alignas(16) uint4 raw[RAW][TC_KEYS * HD / 16];   // in the order of the code threads
   // scales in the order a row thread reads them: 16 keys 16k .. lie as [t4][keys 2 t4, 2 t4 + 1,
   // 8 + 2 t4, 8 + 2 t4 + 1]
   alignas(16) float ks[INFO][TC_KEYS], lv[INFO][TC_KEYS], rv[INFO][TC_KEYS];
   long long place[INFO][TC_KEYS];                  // byte offset of a key's row in the pool, or -1
   float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS];
   unsigned long long full[RING], empty[RING], info_full[INFO], info_empty[INFO];
-  unsigned long long s_full[2], p_full[2], o_full;
+  unsigned long long s_full[2][2], p_full[2][2], o_full;   // [row tile][half & 1]
   uint32_t tmem;
   int abort;
   int seq, tile;                                   // this CTA's, from the lookup
@@ -138,15 +141,6 @@ __device__ __forceinline__ void tm_st_p(uint32_t at, const uint32_t (&v)[16]) {
       "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tm_ld_p(uint32_t at, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15},"
-      " [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(at));
-}
 // 32 columns of one row (lane)
 __device__ __forceinline__ void tm_ld_row(uint32_t at, float (&v)[32]) {
   asm volatile(
@@ -165,12 +159,6 @@ __device__ __forceinline__ void landed(float (&v)[16]) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
                  "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
                  "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
-}
-__device__ __forceinline__ void landed(uint32_t (&v)[16]) {
-  asm volatile(""
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
-                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
-                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
 }
 __device__ __forceinline__ void landed(float (&v)[32]) {
   landed(reinterpret_cast<float(&)[16]>(v[0]));
@@ -211,14 +199,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Half a key tile (64 keys) for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
-// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights at `pt`.  ks holds ks qk_scale log2 e;
-// UNIT: a = 1 in all rows.  The reference of a row's weights is a whole number and moves only when
-// a weight outgrows it by 2^8, which a vote tells, so no row maximum is formed otherwise; then the
-// sums at `ot` (have_o) and the weights of the tile's first half (`first`) are multiplied by the
-// power of two between the references.
+// columns 8i + 2 (lane % 4), + 1: scores at `st` to weights in their place.  ks holds ks qk_scale
+// log2 e; UNIT: a = 1 in all rows.  The reference of a row's weights moves only when a weight
+// outgrows it by 2^8, which a vote tells, so no row maximum is formed otherwise; then the sums at
+// `ot` are rescaled, once the products before this half's are in (`next`, the barrier of the next
+// half's scores, which follow them, with parity par; par < 0: there are none).
 template <int HD, bool MASK, bool UNIT>
 __device__ __forceinline__ void rows16(const float *ks, const float *lv, const float *rv, uint32_t st,
-                                       uint32_t pt, uint32_t first, uint32_t ot, bool have_o,
+                                       uint32_t ot, unsigned long long *next, int par, int *abort,
                                        const float (&a)[2], float (&mref)[2], float (&l)[2],
                                        const int (&pos)[2], int key0, int causal, int window) {
   float x[2][16];
@@ -267,8 +255,8 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
     // maxima relative to the old references (0 where there was none yet)
     const bool g0 = mx0 > (mref[0] == kNegInf ? kNegInf : 8.0f);
     const bool g1 = mx1 > (mref[1] == kNegInf ? kNegInf : 8.0f);
-    const float u0 = g0 ? -ceilf(mx0) : 0.0f, u1 = g1 ? -ceilf(mx1) : 0.0f;
-    // powers of two; without a reference all sums are still zero
+    const float u0 = g0 ? -mx0 : 0.0f, u1 = g1 ? -mx1 : 0.0f;
+    // (without a reference all sums are still zero)
     const float r0 = mref[0] == kNegInf ? 1.0f : ex2(u0), r1 = mref[1] == kNegInf ? 1.0f : ex2(u1);
     b0 = __fadd_rn(b0, u0);
     b1 = __fadd_rn(b1, u1);
@@ -278,7 +266,10 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
     for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = __fadd_rn(x[i >> 4][i & 15], (i & 2) ? u1 : u0);
     l[0] = __fmul_rn(l[0], r0);
     l[1] = __fmul_rn(l[1], r1);
-    if (have_o) {   // the products before this tile's have completed with its scores
+    if (par >= 0) {
+      wait_bar(next, par, abort);
+      __syncwarp();
+      fence_after();
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         float o[16];
@@ -289,20 +280,6 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
         for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(o[i], (i & 2) ? r1 : r0);
         tm_st(ot + c * 32, o);
       }
-    }
-    if (pt != first) {
-      tmem_wait_st();
-      uint32_t w[16];
-      tm_ld_p(first, w);
-      tmem_wait_ld();
-      landed(w);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        const float r = (i & 1) ? r1 : r0;
-        w[i] = pack_f16(__fmul_rn(y.x, r), __fmul_rn(y.y, r));
-      }
-      tm_st_p(first, w);
     }
   }
   F2 s0 = f2(0.0f, 0.0f), s1 = s0;
@@ -322,7 +299,7 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
       w[(k * 2 + h) * 2 + 1] = pack_f16(y[2], y[3]);
     }
   }
-  tm_st_p(pt, w);
+  tm_st_p(st, w);
   float u, v;
   un(s0, u, v);
   l[0] = __fadd_rn(l[0], __fadd_rn(u, v));
@@ -353,7 +330,7 @@ template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   constexpr int HALVES = HD / 64;
   constexpr int HALF_BYTES = 128 * 128;            // 128 rows (or keys) of 64 f16
-  constexpr uint32_t ID_S = idesc_f16(TC_KEYS, false), ID_O = idesc_f16(HD, true);
+  constexpr uint32_t ID_S = idesc_f16(64, false), ID_O = idesc_f16(HD, true);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // (an offset, not a rounded address: accesses stay shared-memory accesses)
   TcSmem<HD> &sm = *reinterpret_cast<TcSmem<HD> *>(smem_raw + ((0u - su32(smem_raw)) & 1023u));
@@ -379,8 +356,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         mbar_init(&sm.info_empty[i], LOADERS + ROW_WARPS);
       }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], ROW_WARPS / 2);
+        for (int b = 0; b < 2; ++b) {
+          mbar_init(&sm.s_full[i][b], 1);
+          mbar_init(&sm.p_full[i][b], ROW_WARPS / 2);
+        }
       }
       mbar_init(&sm.o_full, 1);
       mbar_init_fence();
@@ -397,23 +376,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   const Seq q = load_seq(p, s, &none);
   const int packed = q.n * p.group, m0 = sm.tile * TC_ROWS;
   const int rows = min(TC_ROWS, packed - m0);
-  // key tiles [z0, z0 + nj) of this CTA; row tile t needs the first jt[t] of them
-  int z0, nj, jt[2];
+  // key tiles [z0, z0 + nj) of this CTA; row tile t needs the first ht[t] of their halves
+  int z0, nj, ht[2];
   {
     const int pf = q.pos0 + m0 / p.group, pl = q.pos0 + (m0 + rows - 1) / p.group;
     int lo, hi, z1;
     key_range(p, q, pf, pl, lo, hi);
     split_range(lo / TC_KEYS, (hi + TC_KEYS - 1) / TC_KEYS, p.splits, blockIdx.z, z0, z1);
-    nj = z1 - z0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int last = min(rows, 128 * (t + 1)) - 1;
       const int h = p.causal ? q.pos0 + (m0 + last) / p.group + 1 : q.kv;
-      const int n = (h + TC_KEYS - 1) / TC_KEYS - z0;
-      jt[t] = rows > 128 * t ? max(0, min(nj, n)) : 0;
+      const int n = (h + 63) / 64 - 2 * z0;
+      ht[t] = rows > 128 * t ? max(0, min(2 * (z1 - z0), n)) : 0;
     }
-    nj = max(jt[0], jt[1]);
+    nj = (max(ht[0], ht[1]) + 1) / 2;
   }
+
   // registers move from the other warps to those of the rows: 4 x 128 x 88 + 3 x 128 x 48 is
   // within the launch's 896 x 72
   if (warp < ROW_WARPS) {
@@ -494,35 +473,35 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     const bool unit = __all_sync(0xffffffffu, a[0] == 1.0f && a[1] == 1.0f);
     const int pmin = q.pos0 + min(m0 + rb, packed - 1) / p.group;
     const int pmax = q.pos0 + min(m0 + rb + 15, packed - 1) / p.group;
-    const int mine = t ? jt[1] : jt[0];
+    const int mine = t ? ht[1] : ht[0];
     const uint32_t st = tmem + (static_cast<uint32_t>(qd * 32 + ps * 16) << 16) + t * 128;
     for (int j = 0; j < nj; ++j) {
       const int in = j % INFO;
       wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
-      if (j < mine) {
-        wait_bar(&sm.s_full[t], j & 1, &sm.abort);
-        fence_after();
-        const int key0 = (z0 + j) * TC_KEYS;
-        const bool masked = (p.causal && key0 + TC_KEYS - 1 > pmin) ||
-                            (p.window > 0 && key0 <= pmax - p.window);
-        const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int at = h * 64, k0 = key0 + at + t4 * 2;
+      const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int h = 2 * j + b;
+        if (h < mine) {
+          wait_bar(&sm.s_full[t][b], j & 1, &sm.abort);
+          __syncwarp();
+          fence_after();
+          const int key0 = z0 * TC_KEYS + h * 64, at = b * 64, par = h ? ((h + 1) >> 1) & 1 : -1;
+          const bool masked = (p.causal && key0 + 63 > pmin) || (p.window > 0 && key0 <= pmax - p.window);
           if (masked)
-            rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
-                                    j > 0, a, mref, l, pos, k0, p.causal, p.window);
+            rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                    &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
           else if (unit)
-            rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
-                                    j > 0, a, mref, l, pos, k0, p.causal, p.window);
+            rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                    &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
           else
-            rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + h * 32, st, st + TMEM_O,
-                                     j > 0, a, mref, l, pos, k0, p.causal, p.window);
+            rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                     &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[t][b]);
         }
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[t]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[in]);
@@ -612,42 +591,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     }
   } else if (asm_less_registers(), warp < INFO_WARP) {
     // ------------------------------------------------------------------ codes of K and V
-    // Operand tile `item` (K and V in turn): a warp takes WR key rows in chunks of CR rows, one
-    // 16-byte load a lane; a chunk of the next item is requested as soon as this item's is stored.
+    // Operand tile `item` (K and V in turn): a warp takes WR key rows in chunks of CR rows, 16 bytes
+    // a lane, copied into places of its own (cp.async, RAW items ahead: the latency of L2 is
+    // longer than an item takes), then widened into the operand layout.
     constexpr int WR = TC_KEYS / LOADERS, CR = HD == 128 ? 4 : 8, CHUNKS = WR / CR;
     const int lw = warp - ROW_WARPS, items = 2 * nj;
     // eight lanes take 4 chunks of two rows: their f16 chunks then lie in 8 different places of a
     // 128-byte line
     const int rowl = HD == 128 ? 2 * (lane >> 4) + ((lane >> 2) & 1) : lane >> 2;
     const int c = HD == 128 ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane & 3;
-    const char *base[2] = {p.k + static_cast<long>(kvh) * HD + c * 16,
-                           p.v + static_cast<long>(kvh) * HD + c * 16};
+    const long kcol = static_cast<long>(kvh) * HD + c * 16;
     const int row0 = lw * WR + rowl;
     const uint32_t to = static_cast<uint32_t>((c >> 2) * HALF_BYTES + row0 * 128);
     const int ch = (c & 3) * 2;
-    uint4 buf[CHUNKS];
-    auto load = [&](const long long *place, const char *from, int i) {
-      const long long at = place[row0 + i * CR];
-      buf[i] = make_uint4(0, 0, 0, 0);
-      if (at >= 0) buf[i] = __ldg(reinterpret_cast<const uint4 *>(from + at));
-    };
-    if (nj > 0) {
-      wait_bar(&sm.info_full[0], 0, &sm.abort);
+    uint4 *raw = sm.raw[0] + lw * 32 + lane;
+    auto request = [&](int item) {
+      if (item < items) {
+        const int j = item >> 1, in = j % INFO;
+        wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
+        const char *from = ((item & 1) ? p.v : p.k) + kcol;
+        const uint32_t dst = su32(raw + (item % RAW) * (TC_KEYS * HD / 16));
 #pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) load(sm.place[0], base[0], i);
-    }
+        for (int i = 0; i < CHUNKS; ++i) {
+          const long long at = sm.place[in][row0 + i * CR];
+          cp16(dst + i * LOADERS * 512, at >= 0 ? from + at : p.k, at >= 0);
+        }
+        __syncwarp();
+        if (lane == 0 && (item & 1)) mbar_arrive(&sm.info_empty[in]);   // its places are read
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < RAW; ++i) request(i);
     for (int item = 0; item < items; ++item) {
-      const int slot = item % RING, next = item + 1, jn = next >> 1;
-      const bool more = next < items;
-      if (more && !(next & 1)) wait_bar(&sm.info_full[jn % INFO], (jn / INFO) & 1, &sm.abort);
+      const int slot = item % RING;
       if (item >= RING) wait_bar(&sm.empty[slot], ((item / RING) - 1) & 1, &sm.abort);
+      asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");
       uint8_t *dst = sm.kv[slot] + to;
-      const long long *place = sm.place[jn % INFO];
-      const char *from = (next & 1) ? base[1] : base[0];
+      const uint4 *src = raw + (item % RAW) * (TC_KEYS * HD / 16);
 #pragma unroll
       for (int i = 0; i < CHUNKS; ++i) {
-        const uint32_t w[4] = {buf[i].x ^ 0x80808080u, buf[i].y ^ 0x80808080u,
-                               buf[i].z ^ 0x80808080u, buf[i].w ^ 0x80808080u};
+        const uint4 x = src[i * LOADERS * 32];
+        const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u,
+                               x.w ^ 0x80808080u};
         uint4 lo, hi;
         lo.x = f16_pair(w[0], 0x4140), lo.y = f16_pair(w[0], 0x4342);
         lo.z = f16_pair(w[1], 0x4140), lo.w = f16_pair(w[1], 0x4342);
@@ -656,15 +642,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         const int r = row0 + i * CR;
         *reinterpret_cast<uint4 *>(dst + i * CR * 128 + ((ch ^ (r & 7)) * 16)) = lo;
         *reinterpret_cast<uint4 *>(dst + i * CR * 128 + (((ch + 1) ^ (r & 7)) * 16)) = hi;
-        if (more) load(place, from, i);
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.full[slot]);
-        if (next & 1) mbar_arrive(&sm.info_empty[(item >> 1) % INFO]);   // V's places are read
-      }
+      if (lane == 0) mbar_arrive(&sm.full[slot]);
+      request(item + RAW);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == INFO_WARP) {
     // ------------------------------------------------------------------ places and scales
     // A lane has keys i*32 + lane of a tile.  Pages are looked up two tiles ahead, scales
@@ -734,60 +718,70 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     fence_before();
     start_sync();
     fence_after();
-    const uint32_t tmem = sm.tmem;
     if (elect_one()) {
-    // descriptors: constant but for the start address (in 16-byte units) in the low bits
-    const uint64_t qd[2] = {sdesc_sw128(su32(sm.q[0])), sdesc_sw128(su32(sm.q[1]))};
-    const uint64_t kd = sdesc_sw128(su32(sm.kv[0]));
-    const uint64_t vd = sdesc_mn(su32(sm.kv[0]), HALVES == 2 ? HALF_BYTES : 16);
-    constexpr uint32_t SLOT = TC_KEYS * HD * 2 / 16;
-    auto scores = [&](const int t, int j) {   // S_t = Q_t K8_j^T
-      const uint64_t b = kd + static_cast<uint32_t>((2 * j) % RING) * SLOT;
+      // descriptors: constant but for the start address (in 16-byte units) in the low bits
+      const uint64_t qd[2] = {sdesc_sw128(su32(sm.q[0])), sdesc_sw128(su32(sm.q[1]))};
+      const uint64_t kd = sdesc_sw128(su32(sm.kv[0]));
+      const uint64_t vd = sdesc_mn(su32(sm.kv[0]), HALVES == 2 ? HALF_BYTES : 16);
+      constexpr uint32_t SLOT = TC_KEYS * HD * 2 / 16, KEYS64 = 64 * 128 / 16;
+      const uint32_t tmem = sm.tmem;
+      auto scores = [&](const int t, int h) {   // S of half h = Q K8^T
+        const uint64_t b = kd + static_cast<uint32_t>((h & ~1) % RING) * SLOT + (h & 1) * KEYS64;
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint32_t at = ((k / 4) * HALF_BYTES + (k % 4) * 32) / 16;
-        mma_ss(tmem + t * 128, qd[t] + at, b + at, ID_S, k != 0);
-      }
-      mma_commit(&sm.s_full[t]);
-    };
-    auto values = [&](const int t, int j) {   // O_t += P_t V8_j
-      const uint64_t b = vd + static_cast<uint32_t>((2 * j + 1) % RING) * SLOT;
-#pragma unroll
-      for (int k = 0; k < TC_KEYS / 16; ++k)
-        mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + k * 8, b + k * (2048 / 16), ID_O,
-               j > 0 || k > 0);
-    };
-    auto ready = [&](int item) {
-      wait_bar(&sm.full[item % RING], (item / RING) & 1, &sm.abort);
-      fence_after();
-    };
-    if (nj > 0) {
-      ready(0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (jt[t] > 0) scores(t, 0);
-      mma_commit(&sm.empty[0]);
-    }
-    for (int j = 0; j < nj; ++j) {
-      ready(2 * j + 1);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (j < jt[t]) {
-          wait_bar(&sm.p_full[t], j & 1, &sm.abort);
-          fence_after();
-          values(t, j);
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t at = ((k / 4) * HALF_BYTES + (k % 4) * 32) / 16;
+          mma_ss(tmem + t * 128 + (h & 1) * 64, qd[t] + at, b + at, ID_S, k != 0);
         }
-        if (t == 1) mma_commit(&sm.empty[(2 * j + 1) % RING]);
-        if (t == 0 && j + 1 < nj) ready(2 * j + 2);
-        // these scores overwrite P_t: products of one thread run in order
-        if (j + 1 < jt[t]) scores(t, j + 1);
+      };
+      auto values = [&](const int t, int h) {   // O += P V8 of half h
+        const uint64_t b = vd + static_cast<uint32_t>((h | 1) % RING) * SLOT + (h & 1) * KEYS64;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + (h & 1) * 64 + k * 8, b + k * (2048 / 16),
+                 ID_O, h > 0 || k > 0);
+      };
+      auto ready = [&](int item) {
+        wait_bar(&sm.full[item % RING], (item / RING) & 1, &sm.abort);
+        fence_after();
+      };
+      if (nj > 0) {
+        ready(0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (h < ht[t]) {
+              scores(t, h);
+              mma_commit(&sm.s_full[t][h]);
+            }
+        mma_commit(&sm.empty[0]);
       }
-      if (j + 1 < nj) mma_commit(&sm.empty[(2 * j + 2) % RING]);
-    }
-    if (nj > 0) {
-      mma_commit(&sm.o_full);
-      wait_bar(&sm.o_full, 0, &sm.abort);
-    }
+      for (int h = 0; h < 2 * nj; ++h) {
+        const int j = h >> 1;                      // V of tile j, then K of tile j + 1
+        if (!(h & 1)) ready(2 * j + 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (h < ht[t]) {
+            wait_bar(&sm.p_full[t][h & 1], j & 1, &sm.abort);
+            fence_after();
+            values(t, h);
+          }
+          if (t == 0 && !(h & 1) && j + 1 < nj) ready(2 * j + 2);
+          if (h < ht[t]) {
+            // these scores overwrite the weights of half h: products of one thread run in order
+            if (h + 2 < ht[t]) scores(t, h + 2);
+            mma_commit(&sm.s_full[t][h & 1]);      // (after the last halves: their products are in)
+          }
+        }
+        if (h & 1) {
+          mma_commit(&sm.empty[(2 * j + 1) % RING]);
+          if (j + 1 < nj) mma_commit(&sm.empty[(2 * j + 2) % RING]);
+        }
+      }
+      if (nj > 0) {
+        mma_commit(&sm.o_full);
+        wait_bar(&sm.o_full, 0, &sm.abort);
+      }
     }
     __syncwarp();
   }
