@@ -723,7 +723,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   const uint32_t max_kv = max_pages * kv->page_tokens;
   const chunk::Plan c =
       chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
-  if (c.tiles > 0x7fffffff) return Q3_ERR_SHAPE;
+  if (c.tiles * kv_heads > 0x7fffffff) return Q3_ERR_SHAPE;
   if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return Q3_ERR_ALIGN;

@@ -335,17 +335,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   // (an offset, not a rounded address: accesses stay shared-memory accesses)
   TcSmem<HD> &sm = *reinterpret_cast<TcSmem<HD> *>(smem_raw + ((0u - su32(smem_raw)) & 1023u));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y;
+  // KV heads first: they share the tile's row arrays, and heavy tiles of a sequence start together
+  const int kvh = blockIdx.x % p.kv_heads, tile_id = blockIdx.x / p.kv_heads;
 
   if (warp == 0) {
     unsigned err = 0;
     long before;
-    const int s = find_unit(p.n_seqs, blockIdx.x, lane, before,
+    const int s = find_unit(p.n_seqs, tile_id, lane, before,
                             [&](int x) { return tiles_of(p, x, &err); });
     if (lane == 0) {
       sm.seq = s;
       // the last tile, which has most keys, first
-      sm.tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, &err) - 1 - (blockIdx.x - before));
+      sm.tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, &err) - 1 - (tile_id - before));
       sm.abort = 0;
       for (int i = 0; i < RING; ++i) {
         mbar_init(&sm.full[i], LOADERS);
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       mbar_init(&sm.o_full, 1);
       mbar_init_fence();
     }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {   // refusals, once a launch
+    if (blockIdx.x == 0 && blockIdx.z == 0) {   // refusals, once a launch
       for (int x = lane; x < p.n_seqs; x += 32) load_seq(p, x, &err);
       if (err) atomicOr(&g_chunk_tc_error, err);
     }
@@ -376,6 +377,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   const Seq q = load_seq(p, s, &none);
   const int packed = q.n * p.group, m0 = sm.tile * TC_ROWS;
   const int rows = min(TC_ROWS, packed - m0);
+  // packed row m0 + m: token t0 + (o0 + m) / group, head (o0 + m) % group; the quotient by a 16-bit
+  // reciprocal is exact for o0 + m < 272 and group <= 16
+  const int t0 = m0 / p.group, o0 = m0 - t0 * p.group;
+  const uint32_t magic = (65535u + p.group) / p.group;
+  auto token = [&](int m, int &g) {
+    const int x = o0 + m, y = static_cast<int>((x * magic) >> 16);
+    g = x - y * p.group;
+    return t0 + y;
+  };
   // key tiles [z0, z0 + nj) of this CTA; row tile t needs the first ht[t] of their halves
   int z0, nj, ht[2];
   {
@@ -409,9 +419,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         raw[i] = make_uint4(0, 0, 0, 0);
         qs[i] = 0.0f;
         if (m < rows) {
-          const int mm = m0 + m;
-          const long r = q.first + mm / p.group;
-          const int h = kvh * p.group + mm % p.group;
+          int hg;
+          const long r = q.first + token(m, hg);
+          const int h = kvh * p.group + hg;
           const char *qp = p.q + r * p.q_rb;
           const long col = static_cast<long>(h) * HD + (id % G8) * 8;
           qs[i] = 1.0f;
@@ -466,13 +476,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     for (int e = 0; e < 2; ++e) {
       const int m = rb + 8 * e + g;
       a[e] = sm.a[m];
-      pos[e] = q.pos0 + min(m0 + m, packed - 1) / p.group;
+      int hg;
+      pos[e] = q.pos0 + token(min(m, rows - 1), hg);
       mref[e] = kNegInf;
       l[e] = 0.0f;
     }
     const bool unit = __all_sync(0xffffffffu, a[0] == 1.0f && a[1] == 1.0f);
-    const int pmin = q.pos0 + min(m0 + rb, packed - 1) / p.group;
-    const int pmax = q.pos0 + min(m0 + rb + 15, packed - 1) / p.group;
+    int unused;
+    const int pmin = q.pos0 + token(min(rb, rows - 1), unused);
+    const int pmax = q.pos0 + token(min(rb + 15, rows - 1), unused);
     const int mine = t ? ht[1] : ht[0];
     const uint32_t st = tmem + (static_cast<uint32_t>(qd * 32 + ps * 16) << 16) + t * 128;
     for (int j = 0; j < nj; ++j) {
@@ -522,23 +534,45 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     fence_after();
     const int m = t * 128 + qd * 32 + lane;
     const bool have = m < rows;
-    const int mm = min(m0 + m, packed - 1);
-    const long r = q.first + mm / p.group;
-    const int h = kvh * p.group + mm % p.group;
+    int hg;
+    const long r = q.first + token(min(m, rows - 1), hg);
+    const int h = kvh * p.group + hg;
     const uint32_t src = tmem + (static_cast<uint32_t>(qd * 32) << 16) + TMEM_O + t * 128;
     const float lsum = sm.l[m];
-    constexpr int OC = HD / 64;                    // 32-column chunks a thread stores, from ps * OC
+    // this warp's columns, 32 at a time (its chunks ps * OC ..), go through its part of the query
+    // tile, which the products no longer read: a row's pieces then leave as whole lines
+    constexpr int OC = HD / 64;
+    uint8_t *stage = sm.q[0] + warp * 4096;        // (HD = 64: on into the ring, which is idle too)
+    const int nr = min(32, rows - (t * 128 + qd * 32));
+    auto flush = [&](const int bytes, char *to) {   // `bytes` a row; `to`: where this lane's row goes
+      __syncwarp();
+      const int per = bytes / 16;
+      const unsigned long long mine_ = reinterpret_cast<unsigned long long>(to);
+#pragma unroll 4
+      for (int k = lane; k < 32 * per; k += 32) {
+        const int row = k / per, c = k % per;
+        const unsigned long long at = __shfl_sync(0xffffffffu, mine_, row);
+        if (row < nr)
+          *reinterpret_cast<uint4 *>(at + c * 16) =
+              *reinterpret_cast<const uint4 *>(stage + row * bytes + ((c ^ (row & (per - 1))) * 16));
+      }
+      __syncwarp();
+    };
+    auto put = [&](const int bytes, const int c, const uint4 x) {   // 16-byte piece c of this lane's row
+      *reinterpret_cast<uint4 *>(stage + lane * bytes + ((c ^ (lane & (bytes / 16 - 1))) * 16)) = x;
+    };
     if (p.splits > 1) {
       const long at = (static_cast<long>(blockIdx.z) * p.rows + r) * p.heads + h;
       if (mine > 0) {
-#pragma unroll
+#pragma unroll 1
         for (int c = ps * OC; c < ps * OC + OC; ++c) {
           Elems<float, 32> o;
           tm_ld_row(src + c * 32, o.e);
           tmem_wait_ld();
           landed(o.e);
-          if (have) o.store(p.part_o + at * HD + c * 32);
-          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) put(128, i, o.v[i]);
+          flush(128, reinterpret_cast<char *>(p.part_o + at * HD + c * 32));
         }
       }
       if (have && ps == 0) {
@@ -547,10 +581,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       }
     } else if (mine > 0) {
       const float inv = lsum == 0.0f ? 0.0f : __fdiv_rn(1.0f, lsum);   // no key seen: zeros
-      char *out = p.o + r * p.o_rb;
-      const long col = static_cast<long>(h) * HD;
+      const bool i8 = p.o_dt == Q3_DT_I8;
+      const int es = i8 ? 1 : 2;
+      char *out = p.o + r * p.o_rb + (static_cast<long>(h) * HD + ps * OC * 32) * es;
       float scale = 0.0f;
-      if (p.o_dt == Q3_DT_I8) {
+      if (i8) {
         float mx = 0.0f;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
@@ -565,29 +600,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         if (have && ps == 0) reinterpret_cast<float *>(p.os + r * p.os_rb)[h] = scale;
       }
 #pragma unroll 1
-      for (int c = ps * OC; c < ps * OC + OC; ++c) {
+      for (int c = 0; c < OC; ++c) {
         float o[32];
-        tm_ld_row(src + c * 32, o);
+        tm_ld_row(src + (ps * OC + c) * 32, o);
         tmem_wait_ld();
         landed(o);
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = __fmul_rn(o[i], inv);
-        if (have) {
-          if (p.o_dt == Q3_DT_I8) {
-            uint32_t w[8];
-            quant_pack_absmax<32>(o, scale, w);
-            Elems<int8_t, 32> e;
+        if (i8) {
+          uint32_t w[8];
+          quant_pack_absmax<32>(o, scale, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t *>(e.e)[i] = w[i];
-            e.store(out + col + c * 32);
-          } else if (p.o_dt == Q3_DT_F16) {
-            store_row<__half, 32>(o, out + (col + c * 32) * 2);
-          } else {
-            store_row<__nv_bfloat16, 32>(o, out + (col + c * 32) * 2);
+          for (int i = 0; i < 2; ++i)
+            put(32 * OC, c * 2 + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (p.o_dt == Q3_DT_F16) {
+              w[i] = pack_f16(o[2 * i], o[2 * i + 1]);
+            } else {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+              w[i] = *reinterpret_cast<const uint32_t *>(&v);
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            put(64 * OC, c * 4 + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
         }
-        __syncwarp();
       }
+      flush(32 * OC * es, out);
     }
   } else if (asm_less_registers(), warp < INFO_WARP) {
     // ------------------------------------------------------------------ codes of K and V
@@ -807,7 +849,7 @@ static int launch(const Args &p, cudaStream_t s) {
     }
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  k_attn_tc<HD><<<dim3(p.tiles, p.kv_heads, p.splits), TC_THREADS, smem, s>>>(p);
+  k_attn_tc<HD><<<dim3(p.tiles * p.kv_heads, 1, p.splits), TC_THREADS, smem, s>>>(p);
   return q3h::launch_status();
 }
 
