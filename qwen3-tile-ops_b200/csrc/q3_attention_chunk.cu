@@ -48,11 +48,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // ---------------------------------------------------------------------------
 // Few rows: sequences with at most 8 NT packed rows (packed row m is head m %
 // group of new row m / group of the sequence).  A unit of work is one 32-key block
-// of a (sequence, KV head) pair; the units of the whole batch, in order, are dealt to the
-// warps of one resident wave in equal runs, so ragged lengths and any number of
-// pairs fill the card evenly.  A warp works alone: it keeps the running maximum and
-// sums of its run of a pair and stores the result when it has the whole pair, else
-// a part (at most two a warp: its first and its last pair) that k_attn_join joins.
+// of a sequence; the units of the whole batch, in order, are cut into equal slices,
+// and a warp takes one KV head of a slice, so ragged lengths and any number of
+// sequences fill one resident wave evenly, and the heads of a token, which lie side
+// by side in memory, are read at about the same time.  A warp works alone: it keeps
+// the running maximum and sums of its run of a sequence and stores the result when
+// it has the whole sequence, else a part (at most two a warp: its first and its last
+// sequence) that k_attn_join joins.
 //
 // Keys are the M side of the products (S^T = K8 q^T, o^T = V8^T p^T), so a decode
 // step with a group of 2 wastes 6 of 8 columns instead of 14 of 16 rows.  A warp
@@ -71,8 +73,8 @@ struct FewStage {
   float ks[KB], vs[KB];
 };
 
-// Units of a pair of sequence s (0: not this kernel's) and its first block
-__device__ __forceinline__ int pair_units(const Args &p, const Seq &s, int &b0) {
+// Units of sequence s (0: not this kernel's) and its first block
+__device__ __forceinline__ int seq_units(const Args &p, const Seq &s, int &b0) {
   b0 = 0;
   if (!s.ok || s.n * p.group > p.few_rows) return 0;
   int lo, hi;
@@ -80,32 +82,38 @@ __device__ __forceinline__ int pair_units(const Args &p, const Seq &s, int &b0) 
   b0 = lo / KB;
   return (hi + KB - 1) / KB - b0;
 }
-
-__device__ __forceinline__ long units_of(const Args &p, int s, unsigned *err) {
+__device__ __forceinline__ int units_of(const Args &p, int s, unsigned *err) {
   int b0;
-  return static_cast<long>(pair_units(p, load_seq(p, s, err), b0)) * p.kv_heads;
+  return seq_units(p, load_seq(p, s, err), b0);
 }
-__device__ __forceinline__ long warp_sum(long x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+// All units, and those of the sequences before s0 (whole warp; the host bounds them below 2^31)
+__device__ __forceinline__ uint32_t count_units(const Args &p, int s0, int lane, unsigned *err,
+                                                uint32_t &before) {
+  uint32_t x = 0, y = 0;
+  for (int s = lane; s < p.n_seqs; s += 32) {
+    const uint32_t n = units_of(p, s, err);
+    x += n;
+    y += s < s0 ? n : 0;
+  }
+  before = __reduce_add_sync(0xffffffffu, y);
+  return __reduce_add_sync(0xffffffffu, x);
 }
-__device__ __forceinline__ long count_units(const Args &p, int n, int lane, unsigned *err) {
-  long x = 0;
-  for (int s = lane; s < n; s += 32) x += units_of(p, s, err);
-  return warp_sum(x);
-}
-__device__ __forceinline__ long count_units_from(const Args &p, int s0, int lane, unsigned *err) {
-  long x = 0;
-  for (int s = s0 + lane; s < p.n_seqs; s += 32) x += units_of(p, s, err);
-  return warp_sum(x);
-}
-// workers that share `total` units of a grid of `all` warps, and the first unit of worker w
-__device__ __forceinline__ long workers(long total, long all) {
-  const long n = (total + MIN_UNITS - 1) / MIN_UNITS;
-  return n < all ? n : all;
-}
-__device__ __forceinline__ long first_unit(long total, long n, long w) { return total * w / n; }
+// The slices of `total` units: the first `more` have each + 1 of them
+struct Slices {
+  uint32_t n, each, more;
+  __device__ __forceinline__ Slices(uint32_t total, uint32_t most) {
+    n = (total + MIN_UNITS - 1) / MIN_UNITS;
+    n = n < most ? n : most;
+    n = n ? n : 1;
+    each = total / n;
+    more = total - each * n;
+  }
+  __device__ __forceinline__ uint32_t first(uint32_t w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t unit) const {
+    const uint32_t big = more * (each + 1);
+    return unit < big ? unit / (each + 1) : more + (unit - big) / each;
+  }
+};
 
 // 16 (HD 64: 8) columns at g * HD/8 of one row head, a row spread over the 8 lanes of equal t4
 template <int N>
@@ -151,30 +159,31 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   Stage *ring = reinterpret_cast<Stage *>(smem) + wid * STAGES;
-  const long w = static_cast<long>(blockIdx.x) * WARPS + wid;
+  const uint32_t w = blockIdx.x * WARPS + wid, slice = w / p.kv_heads;
+  const int kvh = w - slice * p.kv_heads;
 
   unsigned err = 0;
-  const long total = count_units(p, p.n_seqs, lane, &err);
+  uint32_t none;
+  const uint32_t total = count_units(p, 0, lane, &err, none);
   if (w == 0 && err) atomicOr(&g_chunk_error, err);
-  const long nw = workers(total, static_cast<long>(gridDim.x) * WARPS);
-  if (w < nw) {
-    long u = first_unit(total, nw, w);
-    const long u1 = first_unit(total, nw, w + 1);
+  const Slices cut(total, gridDim.x * WARPS / p.kv_heads);
+  if (total && slice < cut.n) {
+    uint32_t u = cut.first(slice);
+    const uint32_t u1 = cut.first(slice + 1);
     long before;
     int s = find_unit(p.n_seqs, u, lane, before, [&](int x) { return units_of(p, x, &err); });
-    while (u < u1 && s >= 0) {
-      // the pair of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
+    while (u < u1 && s >= 0 && s < p.n_seqs) {
+      // the sequence of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
       const Seq q = load_seq(p, s, &err);
       int pb0;
-      const int pn = pair_units(p, q, pb0);
+      const int pn = seq_units(p, q, pb0);
       if (pn == 0) {
         ++s;
         continue;
       }
-      const int kvh = static_cast<int>((u - before) / pn);
-      const int off = static_cast<int>((u - before) % pn);
+      const int off = static_cast<int>(u - static_cast<uint32_t>(before));
       const int b = pb0 + off;
-      const int run = static_cast<int>(u1 - u < pn - off ? u1 - u : pn - off);
+      const int run = static_cast<int>(u1 - u) < pn - off ? static_cast<int>(u1 - u) : pn - off;
       const int be = b + run;
       const bool whole = off == 0 && run == pn;
       const int packed = q.n * p.group;
@@ -186,44 +195,59 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
         const int j = x * KB + lane;
         return x < be && j < q.kv ? table[page_index(p, j)] : -1;
       };
-      auto fetch = [&](int x, int pg) {   // block x into its stage
-        const int j = x * KB + lane;
-        bool ok = pg >= 0;
-        if (ok && static_cast<uint32_t>(pg) >= p.num_pages) {
-          atomicOr(&g_chunk_error, kBadPage);
-          ok = false;
-        }
-        const uint32_t at =
-            ok ? (static_cast<uint32_t>(pg) << 16) | page_slot(p, j)
-               : 0xffffffffu;
+      // this lane's part of a block: chunk lane % CH of rows lane / CH, + 32 / CH, ...; in places
+      // that make the fragment reads conflict-free (see there)
+      const int fr = lane / CH, fc = lane % CH;
+      const long from = kcol + static_cast<long>(fr) * p.row_bytes + fc * 16;
+      const uint32_t step = (32 / CH) * p.row_bytes;
+      const int kto = HD == 128 ? fr * 8 + (fc ^ ((fr & 1) << 2)) : (fr >> 1) * 8 + (fr & 1) * 4 + fc;
+      const int vto = HD == 128 ? fr * 8 + (fc ^ (fr & 2)) : kto ^ (((fr >> 1) & 3) << 1);
+      auto fetch = [&](int x, int pg) -> unsigned {   // block x into its stage; its keys that exist
         Stage &st = ring[x % STAGES];
-        const uint32_t kd = static_cast<uint32_t>(__cvta_generic_to_shared(st.k)),
-                       vd = static_cast<uint32_t>(__cvta_generic_to_shared(st.v));
+        const uint32_t kd = static_cast<uint32_t>(__cvta_generic_to_shared(st.k + kto)),
+                       vd = static_cast<uint32_t>(__cvta_generic_to_shared(st.v + vto)),
+                       sd = static_cast<uint32_t>(__cvta_generic_to_shared(st.ks + lane));
+        unsigned have = 0;
         if (x < be) {
+          const int j = x * KB + lane;
+          const bool ok = pg >= 0 && static_cast<uint32_t>(pg) < p.num_pages;
+          if (pg >= 0 && !ok) atomicOr(&g_chunk_error, kBadPage);
+          have = __ballot_sync(0xffffffffu, ok);
+          const uint32_t slot = page_slot(p, j);
+          if (p.whole_blocks && have == 0xffffffffu) {
+            // one page, all of its keys: rows at equal steps
+            const size_t at = static_cast<size_t>(pg) * p.page_bytes +
+                              static_cast<size_t>(slot - lane) * p.row_bytes + from;
+            const char *k = p.k + at, *v = p.v + at;
 #pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            const int row = i * (32 / CH) + lane / CH, c = lane % CH;
-            const uint32_t ra = __shfl_sync(0xffffffffu, at, row);
-            const bool rok = ra != 0xffffffffu;
-            const size_t src = rok ? static_cast<size_t>(ra >> 16) * p.page_bytes +
-                                         static_cast<size_t>(ra & 0xffffu) * p.row_bytes + kcol +
-                                         c * 16
-                                   : 0;
-            // places that make the fragment reads conflict-free (see there)
-            const int line = HD == 128 ? row : row >> 1, lc = HD == 128 ? c : (row & 1) * 4 + c;
-            const int kc = HD == 128 ? lc ^ ((row & 1) << 2) : lc;
-            const int vc = HD == 128 ? lc ^ (row & 6) : lc ^ ((line & 3) << 1);
-            cp16(kd + (line * 8 + kc) * 16, p.k + src, rok);
-            cp16(vd + (line * 8 + vc) * 16, p.v + src, rok);
+            for (int i = 0; i < CH; ++i) {
+              cp16(kd + i * 512, k, true);
+              cp16((HD == 128 && (i & 1) ? vd ^ 64 : vd) + i * 512, v, true);
+              k += step;
+              v += step;
+            }
+          } else {
+            const uint32_t mine = ok ? (static_cast<uint32_t>(pg) << 16) | slot : 0xffffffffu;
+#pragma unroll 2
+            for (int i = 0; i < CH; ++i) {
+              const uint32_t ra = __shfl_sync(0xffffffffu, mine, i * (32 / CH) + fr);
+              const bool rok = ra != 0xffffffffu;
+              const size_t at = rok ? static_cast<size_t>(ra >> 16) * p.page_bytes +
+                                          static_cast<size_t>(ra & 0xffffu) * p.row_bytes + kcol +
+                                          fc * 16
+                                    : 0;
+              cp16(kd + i * 512, p.k + at, rok);
+              cp16((HD == 128 && (i & 1) ? vd ^ 64 : vd) + i * 512, p.v + at, rok);
+            }
           }
-          const size_t so = ok ? static_cast<size_t>(at >> 16) * p.scale_page_bytes +
-                                     static_cast<size_t>(at & 0xffffu) * p.scale_row_bytes + kvh * 4
+          const size_t so = ok ? static_cast<size_t>(pg) * p.scale_page_bytes +
+                                     static_cast<size_t>(slot) * p.scale_row_bytes + kvh * 4
                                : 0;
-          cp4(static_cast<uint32_t>(__cvta_generic_to_shared(st.ks + lane)), p.ks + so, ok);
-          cp4(static_cast<uint32_t>(__cvta_generic_to_shared(st.vs + lane)), p.vs + so, ok);
+          cp4(sd, p.ks + so, ok);
+          cp4(sd + KB * 4, p.vs + so, ok);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return __ballot_sync(0xffffffffu, ok);          // keys of the block that exist
+        return have;
       };
       int pg[STAGES];
       unsigned have[STAGES];
@@ -362,15 +386,19 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
           lv[i] = v != v ? v : lg2(fmaxf(v, kVsMin));// ... and the rows that see it get NaN)
         }
         const bool masked = mask != 0xffffffffu || x * KB + KB - 1 > q.pos0 || p.window > 0;
+        // relative to the reference of the row's weights, which moves when one outgrows it by 2^8
+        float top[NT][2];
+        bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            const float base = mref[n][j] == kNegInf ? 0.0f : mref[n][j];
             float mx = kNegInf;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float &y = sc[i >> 1][n][(i & 1) * 2 + j];
-              y = __fmaf_rn(__fmul_rn(y, ks[i]), a[n][j], lv[i]);
+              y = __fsub_rn(__fmaf_rn(__fmul_rn(y, ks[i]), a[n][j], lv[i]), base);
               if (masked) {
                 const int key = x * KB + i * 8 + g;
                 const bool see = ((mask >> (i * 8 + g)) & 1) && !(p.causal && key > pq[n][j]) &&
@@ -379,29 +407,45 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
               }
               mx = fmaxf(mx, y);
             }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            // a new reference when the maximum outgrows the old one by 2^8
-            const bool grow = mx > __fadd_rn(mref[n][j], 8.0f);
-            if (__any_sync(0xffffffffu, grow)) {
-              const float f = grow ? ex2(__fsub_rn(mref[n][j], mx)) : 1.0f;
-              mref[n][j] = grow ? mx : mref[n][j];
+            top[n][j] = mx;
+            grow = grow || mx > 8.0f || mref[n][j] == kNegInf;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float mx = top[n][j];
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const bool none = mref[n][j] == kNegInf;
+              const float up = mx > (none ? kNegInf : 8.0f) ? mx : 0.0f;
+              const float f = none ? 1.0f : ex2(-up);    // (without a reference the sums are zero)
+              if (mx > (none ? kNegInf : 8.0f)) mref[n][j] = none ? up : __fadd_rn(mref[n][j], up);
               lsum[n][j] = __fmul_rn(lsum[n][j], f);
 #pragma unroll
               for (int d = 0; d < HD / 16; ++d) {
                 o[d][n][j] = __fmul_rn(o[d][n][j], f);
                 o[d][n][2 + j] = __fmul_rn(o[d][n][2 + j], f);
               }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float &y = sc[i >> 1][n][(i & 1) * 2 + j];
+                y = __fsub_rn(y, up);
+              }
             }
-            const float base = mref[n][j] == kNegInf ? 0.0f : mref[n][j];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float &y = sc[i >> 1][n][(i & 1) * 2 + j];
-              y = ex2(__fsub_rn(y, base));
+              y = ex2(y);
               lsum[n][j] = __fmaf_rn(y, rv[i], lsum[n][j]);
             }
-          }
         // o^T += V8^T p^T
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -447,7 +491,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
       // column g*(HD/8) + 2i of o^T in o[i][n][j], + 1 in o[i][n][2 + j], row n*8 + t4*2 + j
-      const long slot = 2 * w + (off == 0 ? 1 : 0);
+      const long slot = 2 * static_cast<long>(w) + (off == 0 ? 1 : 0);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -483,56 +527,73 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
           }
         }
       u += run;
-      if (off + run == pn && kvh + 1 == p.kv_heads) {
-        before += static_cast<long>(pn) * p.kv_heads;
-        ++s;
-      }
-      if (s >= p.n_seqs) break;
+      before += pn;
+      ++s;
     }
   }
   pdl_trigger();
 }
 
-// The parts of a (sequence, KV head) pair joined by a CTA; its warps take the parts of a row in turn.
+// The parts of one packed row of a (sequence, KV head) pair joined by a CTA: its warps take them in
+// turn, JOIN_AT loads at once.
+constexpr int JOIN_WARPS = 8, JOIN_AT = 4;
 template <int HD>
-__global__ void __launch_bounds__(WARPS * 32) k_attn_join(const Args p, long all_workers) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uint32_t most) {
   constexpr int N = HD / 32;
-  __shared__ float so[WARPS][HD], sm[WARPS], sl[WARPS];
+  __shared__ float so[JOIN_WARPS][HD], sm[JOIN_WARPS], sl[JOIN_WARPS];
+  __shared__ uint32_t range[2];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int s = blockIdx.x, kvh = blockIdx.y;
   unsigned err = 0;
   const Seq q = load_seq(p, s, &err);
   int pb0;
-  const int pn = pair_units(p, q, pb0);
+  const int pn = seq_units(p, q, pb0);
   const int m = blockIdx.z;                        // packed row
   if (pn == 0 || m >= q.n * p.group) return;       // refused, or the other kernel's
+  if (wid == 0) {   // the slices that have units of the sequence
+    uint32_t before;
+    const Slices cut(count_units(p, s, lane, &err, before), most);
+    if (lane == 0) {
+      range[0] = cut.of(before);
+      range[1] = cut.of(before + pn - 1);
+    }
+  }
+  __syncthreads();
+  const uint32_t w0 = range[0], w1 = range[1];
+  if (w0 == w1) return;                            // stored whole
   const long r = q.first + m / p.group;
   const int h = kvh * p.group + m % p.group;
-  const long before = count_units(p, s, lane, &err);
-  const long total = before + count_units_from(p, s, lane, &err);
-  const long nw = workers(total, all_workers);
-  // the pair's units, and the workers that have them
-  const long a = before + static_cast<long>(kvh) * pn, b = a + pn;
-  long w0 = a * nw / total, w1 = (b - 1) * nw / total;
-  while (w0 + 1 < nw && first_unit(total, nw, w0 + 1) <= a) ++w0;
-  while (w1 + 1 < nw && first_unit(total, nw, w1 + 1) <= b - 1) ++w1;
-  if (w0 == w1) return;                            // stored whole
   pdl_wait();
   float mm = kNegInf, l = 0.0f, x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
-  for (long w = w0 + wid; w <= w1; w += WARPS) {
-    const long slot = 2 * w + (first_unit(total, nw, w) <= a ? 1 : 0);
-    const long at = slot * p.part_rows + m;
-    const float pm = p.part_ml[at * 2], pl = p.part_ml[at * 2 + 1];
-    Elems<float, N> e;
-    e.load(p.part_o + at * HD + lane * N);
-    const float top = fmaxf(mm, pm), base = top == kNegInf ? 0.0f : top;
-    const float f0 = ex2(__fsub_rn(mm, base)), f1 = ex2(__fsub_rn(pm, base));
-    mm = top;
-    l = __fmaf_rn(f1, pl, __fmul_rn(f0, l));
+  for (uint32_t w = w0 + wid; w <= w1; w += JOIN_WARPS * JOIN_AT) {
+    float pm[JOIN_AT], pl[JOIN_AT];
+    Elems<float, N> e[JOIN_AT];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f1, e.e[i], __fmul_rn(f0, x[i]));
+    for (int k = 0; k < JOIN_AT; ++k) {
+      const uint32_t wk = w + k * JOIN_WARPS;
+      pm[k] = kNegInf;
+      pl[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[k].e[i] = 0.0f;
+      if (wk <= w1) {   // the warp's part: of its last sequence if this one begins with it
+        const long at = (2 * (static_cast<long>(wk) * p.kv_heads + kvh) + (wk == w0 ? 1 : 0)) *
+                            p.part_rows + m;
+        pm[k] = p.part_ml[at * 2];
+        pl[k] = p.part_ml[at * 2 + 1];
+        e[k].load(p.part_o + at * HD + lane * N);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < JOIN_AT; ++k) {
+      const float top = fmaxf(mm, pm[k]), base = top == kNegInf ? 0.0f : top;
+      const float f0 = ex2(__fsub_rn(mm, base)), f1 = ex2(__fsub_rn(pm[k], base));
+      mm = top;
+      l = __fmaf_rn(f1, pl[k], __fmul_rn(f0, l));
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f1, e[k].e[i], __fmul_rn(f0, x[i]));
+    }
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) so[wid][lane * N + i] = x[i];
@@ -541,13 +602,13 @@ __global__ void __launch_bounds__(WARPS * 32) k_attn_join(const Args p, long all
   if (wid) return;
   float top = kNegInf;
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, sm[i]);
+  for (int i = 0; i < JOIN_WARPS; ++i) top = fmaxf(top, sm[i]);
   const float base = top == kNegInf ? 0.0f : top;
   l = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < WARPS; ++k) {
+  for (int k = 0; k < JOIN_WARPS; ++k) {
     const float f = ex2(__fsub_rn(sm[k], base));
     l = __fmaf_rn(f, sl[k], l);
 #pragma unroll
@@ -610,10 +671,12 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
   c.few_rows = 16;
   c.nt = packed > 8 && group <= c.few_rows ? 2 : 1;
   if (group <= c.few_rows) {
-    const long units = static_cast<long>(n_seqs) * kv_heads * ((max_kv + KB - 1) / KB);
-    const long ctas = (units + MIN_UNITS * WARPS - 1) / (MIN_UNITS * WARPS);
-    const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2);
-    c.few_ctas = static_cast<int>(ctas < most ? ctas : most);
+    const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB);
+    const long slices = (units + MIN_UNITS - 1) / MIN_UNITS;
+    const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2), least = (kv_heads + WARPS - 1) / WARPS;
+    long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
+    ctas = ctas < most ? ctas : most;
+    c.few_ctas = static_cast<int>(ctas > least ? ctas : least);   // a slice at least
     c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
   }
   c.splits = 1;
@@ -676,8 +739,11 @@ static int launch_few(const chunk::Args &p, int ctas, cudaStream_t s) {
   Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
   chunk::k_attn_few<HD, NT><<<ctas, chunk::WARPS * 32, smem, s>>>(p);
   Q3_TRY(launch_status());
-  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, p.part_rows), dim3(chunk::WARPS * 32), 0, s,
-                   p, static_cast<long>(ctas) * chunk::WARPS);
+  const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
+  const unsigned z = static_cast<unsigned>(packed < p.part_rows ? packed : p.part_rows);
+  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, z),
+                   dim3(chunk::JOIN_WARPS * 32), 0, s, p,
+                   static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads);
 }
 
 template <int HD>
@@ -723,7 +789,8 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   const uint32_t max_kv = max_pages * kv->page_tokens;
   const chunk::Plan c =
       chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
-  if (c.tiles * kv_heads > 0x7fffffff) return Q3_ERR_SHAPE;
+  if (c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
+    return Q3_ERR_SHAPE;
   if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return Q3_ERR_ALIGN;
@@ -762,6 +829,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   p.window = (int)window;
   p.scale_log2 = (float)((double)qk_scale * 1.4426950408889634);
   p.page_shift = (p.page_tokens & (p.page_tokens - 1)) ? -1 : __builtin_ctz(p.page_tokens);
+  p.whole_blocks = p.page_tokens % chunk::KB == 0;
   p.few_rows = c.few_ctas ? c.few_rows : 0;
   cudaStream_t s = (cudaStream_t)stream;
   timer_begin(TIMER_ATTENTION, s);
