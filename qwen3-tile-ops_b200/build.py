@@ -1,4 +1,6 @@
-"""Build ``libq3b200.so`` (every CUDA/C++ source under ``csrc/``) for sm_100a.
+"""Build ``libq3b200.so`` (every CUDA/C++ source under ``csrc/``) for sm_100a, and
+``_native.so``, the Python side of its rotary and paged-chunk operators
+(``csrc/python/``, against the torch that this interpreter imports).
 
     python qwen3-tile-ops_b200/build.py          # incremental
     python qwen3-tile-ops_b200/build.py --clean
@@ -21,6 +23,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libq3b200.so"
+NATIVE = PKG / "_native.so"
 INCLUDE = PKG.parent / "include"
 
 NVCC = os.environ.get("NVCC", "nvcc")
@@ -49,6 +52,29 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _native(lib: Path) -> None:
+    """``_native.so`` next to the library, which it finds by its own place."""
+    import sysconfig
+
+    import torch
+    src = CSRC / "python" / "q3_native.cpp"
+    newest = max(f.stat().st_mtime for f in (src, INCLUDE / "q3_ops.h", Path(torch.__file__)))
+    if NATIVE.exists() and NATIVE.stat().st_mtime >= newest:
+        return
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(shutil.which(NVCC) or "/usr/local/cuda/bin/nvcc").resolve().parent.parent
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{INCLUDE}", f"-I{root}/include",
+           f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{cuda}/include", str(src), "-o", str(NATIVE), f"-L{root}/lib", f"-L{lib.parent}",
+           "-l:" + lib.name, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{root}/lib"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building {NATIVE.name} failed:\n{res.stdout}\n{res.stderr}")
+
+
 def build(verbose: bool = False, clean: bool = False) -> Path:
     if clean and BUILD.exists():
         shutil.rmtree(BUILD)
@@ -57,12 +83,14 @@ def build(verbose: bool = False, clean: bool = False) -> Path:
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
     if LIB.exists() and all(LIB.stat().st_mtime >= o.stat().st_mtime for o in objs):
+        _native(LIB)
         return LIB
     cmd = [NVCC, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(LIB), *map(str, objs),
            "-lcudart", "-lcuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _native(LIB)
     return LIB
 
 

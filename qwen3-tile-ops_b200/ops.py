@@ -10,11 +10,12 @@ shape, these raise ``Q3Error``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 from dataclasses import dataclass, replace
 
 import torch
 
-from ._lib import (DT_BF16, DT_F16, DT_F32, DT_I8, DT_I32, DT_U32, DT_U8, PagedKV, RopeSpec,
+from ._lib import (DT_BF16, DT_F16, DT_F32, DT_I8, DT_I32, DT_U32, DT_U8, PagedKV,
                    SampleRow, View, check, lib)
 
 _TORCH_DT = {torch.int8: DT_I8, torch.uint8: DT_U8, torch.int32: DT_I32, torch.float32: DT_F32,
@@ -209,59 +210,22 @@ def exp2_rows(x, out, stream=None) -> None:
 
 # ---- rotary positions and paged chunks (extension) ---------------------------
 # The operators below run on the device of their tensors (made current for the
-# call) and on that device's current stream unless ``stream=`` is given.
+# call) and on that device's current stream unless ``stream=`` is given.  Their
+# views are built in ``_native.so`` (csrc/python/), imported on first use.
 
 _SCALING = {"none": 0, "linear": 1, "yarn": 2}
+_native = None
 
 
-def _on(dev, x):
-    """View of a tensor (or MatrixView) for a call on device ``dev``."""
-    if x is None:
-        return None
-    if isinstance(x, MatrixView):
-        return C.byref(x.c())
-    if x.get_device() != dev:
-        raise ValueError(f"operands on different devices: {x.device} and cuda:{dev}")
-    es = x.element_size()
-    shape, stride = x.shape, x.stride()
-    if len(shape) == 2:
-        return C.byref(View(x.data_ptr(), stride[0] * es, stride[1] * es, shape[0], shape[1],
-                            _TORCH_DT[x.dtype]))
-    if len(shape) != 1:
-        raise ValueError("MatrixView needs a 1-D or 2-D tensor")
-    return C.byref(View(x.data_ptr(), stride[0] * es, es, shape[0], 1, _TORCH_DT[x.dtype]))
-
-
-def _device(x) -> int:
-    """CUDA device of an operand (a MatrixView without a tensor: the current one)."""
-    if isinstance(x, MatrixView):
-        x = x.owner
-    if not isinstance(x, torch.Tensor):
-        return torch.cuda.current_device()
-    dev = x.get_device()
-    if dev < 0:
-        raise ValueError("MatrixView needs CUDA memory")
-    return dev
-
-
-def _array(dev, x, dtypes, n, what) -> int:
-    """Address of a contiguous device array of at least n elements."""
-    if x.get_device() != dev or x.dtype not in dtypes or not x.is_contiguous() or x.numel() < n:
-        raise ValueError(f"{what}: a contiguous array of at least {n} {dtypes[0]} on cuda:{dev} "
-                         f"is needed, got {tuple(x.shape)} {x.dtype} on {x.device}")
-    return x.data_ptr()
-
-
-def _run(fn: str, dev: int, stream, *args) -> None:
-    s = torch._C._cuda_getCurrentRawStream(dev) if stream is None else _s(stream)
-    if dev == torch.cuda.current_device():
-        check(fn, getattr(lib(), fn)(*args, s))
-    else:
-        with torch.cuda.device(dev):
-            check(fn, getattr(lib(), fn)(*args, s))
-
-
-_I32, _U16 = (torch.int32,), (torch.uint16, torch.int16)
+def _load_native():
+    global _native
+    if _native is None:
+        lib()   # the library that it calls
+        try:
+            _native = importlib.import_module("._native", __package__)
+        except ImportError as e:
+            raise ImportError(f"{e}: run qwen3-tile-ops_b200/build.py") from e
+    return _native
 
 
 def rope_tables(cos, sin, theta: float, pos0: int = 0, scaling: str = "none", factor: float = 1.0,
@@ -272,10 +236,11 @@ def rope_tables(cos, sin, theta: float, pos0: int = 0, scaling: str = "none", fa
     factor).  attn_factor <= 0: 1, or 0.1 ln(factor) + 1 with yarn."""
     if scaling not in _SCALING:
         raise ValueError(f"scaling: one of {', '.join(_SCALING)}, got {scaling!r}")
-    dev = _device(cos)
-    spec = RopeSpec(theta, factor, original_max, beta_fast, beta_slow, attn_factor,
-                    _SCALING[scaling])
-    _run("q3_rope_tables", dev, stream, C.byref(spec), pos0, _on(dev, cos), _on(dev, sin))
+    code = (_native or _load_native()).rope_tables(
+        theta, pos0, _SCALING[scaling], factor, original_max, beta_fast, beta_slow, attn_factor, cos,
+        sin, stream)
+    if code:
+        check("q3_rope_tables", code)
 
 
 def rope_rows(x, pos: torch.Tensor, cos, sin, out, heads: int, head_dim: int = 128, nw=None,
@@ -284,12 +249,11 @@ def rope_rows(x, pos: torch.Tensor, cos, sin, out, heads: int, head_dim: int = 1
     """Each head of each row: RMSNorm with ``nw`` (optional), then rotation by row pos[r] of the
     tables (rot = 2 * columns of cos).  ``out``: float32, float16, bfloat16 (may be x), or int8
     with one scale per head in ``scale``."""
-    dev = _device(x)
-    rows = x.rows if isinstance(x, MatrixView) else x.shape[0]
-    _run("q3_rope_rows", dev, stream, _on(dev, x), _on(dev, nw),
-         _array(dev, pos, _I32, rows, "pos"), _on(dev, cos), _on(dev, sin), _on(dev, out),
-         _on(dev, scale), heads, head_dim, 1 if interleaved else 0,
-         1.0 / head_dim if inv_hd is None else inv_hd)
+    code = (_native or _load_native()).rope_rows(
+        x, nw, pos, cos, sin, out, scale, heads, head_dim, interleaved,
+        1.0 / head_dim if inv_hd is None else inv_hd, stream)
+    if code:
+        check("q3_rope_rows", code)
 
 
 def paged_kv_append_batch(k, v, kv: PagedKV, num_pages: int, tables: torch.Tensor, max_pages: int,
@@ -299,13 +263,11 @@ def paged_kv_append_batch(k, v, kv: PagedKV, num_pages: int, tables: torch.Tenso
     """New K/V rows of a ragged batch (sequence s: rows row0[s] .. row0[s+1]-1, its last tokens
     of kv_len[s]) into their int8 pages: K normed (``nw``) and rotated (``cos``, ``sin``) on the
     way, one scale per token and head."""
-    dev = _device(k)
-    _run("q3_paged_kv_append_batch", dev, stream, _on(dev, k), _on(dev, v), _on(dev, nw),
-         1.0 / head_dim if inv_hd is None else inv_hd, _on(dev, cos), _on(dev, sin),
-         1 if interleaved else 0, C.byref(kv), num_pages,
-         _array(dev, tables, _U16, n_seqs * max_pages, "tables"), max_pages,
-         _array(dev, row0, _I32, n_seqs + 1, "row0"), _array(dev, kv_len, _I32, n_seqs, "kv_len"),
-         n_seqs, kv_heads, head_dim)
+    code = (_native or _load_native()).paged_kv_append(
+        k, v, nw, 1.0 / head_dim if inv_hd is None else inv_hd, cos, sin, interleaved, kv, num_pages,
+        tables, max_pages, row0, kv_len, n_seqs, kv_heads, head_dim, stream)
+    if code:
+        check("q3_paged_kv_append_batch", code)
 
 
 def attention_chunk_workspace_bytes(rows: int, n_seqs: int, max_rows: int, max_kv: int, heads: int,
@@ -322,20 +284,8 @@ def attention_chunk_batch(q, q_scale, kv: PagedKV, num_pages: int, tables: torch
     """Attention of a ragged batch's rows (at most ``max_rows`` a sequence) over their int8 pages,
     the new tokens' own included.  q: int8 with q_scale, float16 or bfloat16; o: int8 with os,
     float16 or bfloat16.  ``window`` > 0: a row sees its last ``window`` positions only."""
-    dev = _device(q)
-    rows = q.rows if isinstance(q, MatrixView) else q.shape[0]
-    if workspace is None:
-        n = attention_chunk_workspace_bytes(rows, n_seqs, max_rows, max_pages * kv.page_tokens,
-                                            heads, kv_heads, head_dim)
-        workspace = torch.empty(n, dtype=torch.uint8, device=f"cuda:{dev}") if n else None
-        if n and stream is not None:   # the allocator's stream is another one
-            workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else
-                                    torch.cuda.ExternalStream(int(stream), device=dev))
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace: a contiguous tensor on cuda:{dev} is needed")
-    _run("q3_attention_chunk_batch", dev, stream, _on(dev, q), _on(dev, q_scale), C.byref(kv),
-         num_pages, _array(dev, tables, _U16, n_seqs * max_pages, "tables"), max_pages,
-         _array(dev, row0, _I32, n_seqs + 1, "row0"), _array(dev, kv_len, _I32, n_seqs, "kv_len"),
-         n_seqs, max_rows, _on(dev, o), _on(dev, os), heads, kv_heads, head_dim,
-         1 if causal else 0, window, qk_scale, workspace.data_ptr() if workspace is not None else 0,
-         workspace.numel() * workspace.element_size() if workspace is not None else 0)
+    code = (_native or _load_native()).attention_chunk(
+        q, q_scale, kv, num_pages, tables, max_pages, row0, kv_len, n_seqs, max_rows, o, os, heads,
+        kv_heads, head_dim, causal, window, qk_scale, workspace, stream)
+    if code:
+        check("q3_attention_chunk_batch", code)
