@@ -44,6 +44,19 @@ struct Elems {
 #pragma unroll
     for (int i = 0; i < CH; ++i) v[i] = reinterpret_cast<const V *>(p)[i];
   }
+  // read and written once: past the caches
+  __device__ __forceinline__ void load_stream(const void *p) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = __ldcs(reinterpret_cast<const V *>(p) + i);
+  }
+  __device__ __forceinline__ void store_stream(void *p) const {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) __stcs(reinterpret_cast<V *>(p) + i, v[i]);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = V{};
+  }
   __device__ __forceinline__ void store(void *p) const {
 #pragma unroll
     for (int i = 0; i < CH; ++i) reinterpret_cast<V *>(p)[i] = v[i];
@@ -68,6 +81,14 @@ __device__ __forceinline__ void store_row(const float (&x)[N], void *p) {
 #pragma unroll
   for (int i = 0; i < N; ++i) e.e[i] = from_f32<T>(x[i]);
   e.store(p);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_row_stream(const float (&x)[N], void *p) {
+  Elems<T, N> e;
+#pragma unroll
+  for (int i = 0; i < N; ++i) e.e[i] = from_f32<T>(x[i]);
+  e.store_stream(p);
 }
 
 // Sequence of row r (whole warp): the last s with row0[s] <= r, or -1 when r

@@ -23,7 +23,10 @@ namespace rope {
 // ---------------------------------------------------------------------------
 // tables: angle of position p and pair i in turns = p * turn[i], turn[i] a 64-bit
 // binary fraction of one turn.  p * turn[i] modulo 2^64 is exact, so far
-// positions lose nothing: the error is p times that of turn[i] (2^-64).
+// positions lose nothing: the error is p times that of turn[i] (2^-64).  The
+// nearest quarter turn is taken off the leading 32 bits, and sin and cos of the rest,
+// at most 1/8 turn = pi/4, are their Taylor series (to x^9 and x^10: remainders below
+// 2^-29); conversion, series and scaling stay within 2^-22.
 // ---------------------------------------------------------------------------
 constexpr int MAX_PAIRS = 128;
 struct TableArgs {
@@ -35,6 +38,13 @@ struct TableArgs {
   float a;
 };
 
+// (2 pi 2^-32)^n / n!, exact in binary but for the rounding of the constant
+__host__ __device__ constexpr double turn_power(int n) {
+  double x = 1.0;
+  for (int i = 1; i <= n; ++i) x = x * 6.283185307179586476925286766559 / 4294967296.0 / i;
+  return x;
+}
+
 __global__ void k_rope_tables(const __grid_constant__ TableArgs p) {
   __shared__ uint64_t turn[MAX_PAIRS];
   for (int i = threadIdx.x; i < p.half; i += blockDim.x) turn[i] = p.turn[i];
@@ -42,30 +52,57 @@ __global__ void k_rope_tables(const __grid_constant__ TableArgs p) {
   const int per = blockDim.x / p.half;             // positions a block does at once
   const int i = threadIdx.x % p.half, r0 = threadIdx.x / p.half;
   if (r0 >= per) return;
-  for (long r = static_cast<long>(blockIdx.x) * per + r0; r < p.rows;
-       r += static_cast<long>(gridDim.x) * per) {
-    const uint64_t t = turn[i] * (static_cast<uint64_t>(p.pos0) + static_cast<uint64_t>(r));
-    // the signed fraction in [-1/2, 1/2) turns: 24 leading bits and the rest
-    const int hi = static_cast<int>(t >> 32);
-    const float f = __int2float_rn(hi);
-    const int64_t rest =
-        static_cast<int64_t>(t - (static_cast<uint64_t>(static_cast<int64_t>(f)) << 32));
-    float s, c;
-    sincospif(__fmul_rn(f, 4.656612873077393e-10f /* 2^-31: half turns */), &s, &c);
-    // cos(x + d) = cos x - d sin x, |d| < 2^-23
-    const float d = __fmul_rn(__ll2float_rn(rest), 3.406121580086565e-19f /* 2 pi 2^-64 */);
-    const float cc = __fmaf_rn(-d, s, c), ss = __fmaf_rn(d, c, s);
-    reinterpret_cast<float *>(p.cos + r * p.cos_rb)[i] = __fmul_rn(cc, p.a);
-    reinterpret_cast<float *>(p.sin + r * p.sin_rb)[i] = __fmul_rn(ss, p.a);
+  const long step = static_cast<long>(gridDim.x) * per;
+  long r = static_cast<long>(blockIdx.x) * per + r0;
+  uint64_t t = turn[i] * (static_cast<uint64_t>(p.pos0) + static_cast<uint64_t>(r));
+  const uint64_t dt = turn[i] * static_cast<uint64_t>(step);
+  char *cp = p.cos + r * p.cos_rb + i * 4, *sp = p.sin + r * p.sin_rb + i * 4;
+#pragma unroll 4
+  for (; r < p.rows; r += step) {
+    const uint32_t hi = static_cast<uint32_t>(t >> 32);
+    const uint32_t q = (hi + 0x20000000u) >> 30;   // nearest quarter turn
+    const float x = __int2float_rn(static_cast<int>(hi - (q << 30)));   // 2^-32 turns
+    // in units of u = (x 2^-29)^2 <= 1 the coefficients stay in float32's range
+    const float y = __fmul_rn(x, 1.862645149230957e-09f), u = __fmul_rn(y, y);
+    constexpr double k = 536870912.0, k2 = k * k;  // 2^29
+    constexpr float s1 = static_cast<float>(turn_power(1) * k),
+                    s3 = static_cast<float>(-turn_power(3) * k * k2),
+                    s5 = static_cast<float>(turn_power(5) * k * k2 * k2),
+                    s7 = static_cast<float>(-turn_power(7) * k * k2 * k2 * k2),
+                    s9 = static_cast<float>(turn_power(9) * k * k2 * k2 * k2 * k2),
+                    c2 = static_cast<float>(-turn_power(2) * k2),
+                    c4 = static_cast<float>(turn_power(4) * k2 * k2),
+                    c6 = static_cast<float>(-turn_power(6) * k2 * k2 * k2),
+                    c8 = static_cast<float>(turn_power(8) * k2 * k2 * k2 * k2),
+                    c10 = static_cast<float>(-turn_power(10) * k2 * k2 * k2 * k2 * k2);
+    float s = __fmaf_rn(u, s9, s7), c = __fmaf_rn(u, c10, c8);
+    s = __fmaf_rn(u, s, s5);
+    c = __fmaf_rn(u, c, c6);
+    s = __fmaf_rn(u, s, s3);
+    c = __fmaf_rn(u, c, c4);
+    s = __fmul_rn(__fmul_rn(u, s), y);
+    c = __fmaf_rn(u, c, c2);
+    s = __fmaf_rn(y, s1, s);
+    c = __fmaf_rn(u, c, 1.0f);
+    // quarter q: (c, s), (-s, c), (-c, -s), (s, -c)
+    const float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;
+    const float ca = __uint_as_float(__float_as_uint(p.a) ^ (((q + 1) & 2) << 30));
+    const float sa = __uint_as_float(__float_as_uint(p.a) ^ ((q & 2) << 30));
+    *reinterpret_cast<float *>(cp) = __fmul_rn(cc, ca);
+    *reinterpret_cast<float *>(sp) = __fmul_rn(ss, sa);
+    t += dt;
+    cp += step * p.cos_rb;
+    sp += step * p.sin_rb;
   }
 }
 
 // ---------------------------------------------------------------------------
-// One head in a warp: lane l holds columns l*N .. l*N+N-1 (head_dim = 32 N).
-// The float32 steps and their order are those of the norm-rope-quant epilogue
+// One head in GL lanes: lane g of them holds columns g*N .. g*N+N-1 (head_dim =
+// GL N), a warp 32 / GL heads; N is what 16 bytes hold, or 8.  The float32 steps and
+// their order are those of the norm-rope-quant epilogue
 // (tools/ref_qwen3.py:161-191), so the codes are the same bits.
 // ---------------------------------------------------------------------------
-template <int N>
+template <int N, int GL>
 __device__ __forceinline__ void head_norm(float (&x)[N], const float (&w)[N], float inv_hd) {
   // squares by adjacent pairs within 32-column blocks of 32/N lanes ...
   float s[N];
@@ -77,10 +114,11 @@ __device__ __forceinline__ void head_norm(float (&x)[N], const float (&w)[N], fl
     for (int i = 0; i < N; i += 2 * k) s[i] = __fadd_rn(s[i], s[i + k]);
 #pragma unroll
   for (int o = 1; o < 32 / N; o <<= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], o));
-  // ... and the N blocks in order
+  // ... and the blocks in order
   float ss = 0.0f;
 #pragma unroll
-  for (int b = 0; b < N; ++b) ss = __fadd_rn(ss, __shfl_sync(0xffffffffu, s[0], b * (32 / N)));
+  for (int b = 0; b < GL * N / 32; ++b)
+    ss = __fadd_rn(ss, __shfl_sync(0xffffffffu, s[0], b * (32 / N), GL));
   const float r = rsqrt_ref(__fadd_rn(__fmul_rn(ss, inv_hd), kEps));
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
@@ -88,11 +126,11 @@ __device__ __forceinline__ void head_norm(float (&x)[N], const float (&w)[N], fl
 
 // c, s: cos and sin of this lane's columns (half layout: of column mod half;
 // interleaved: c[i], s[i] for pair i of the lane in i < N/2)
-template <int N>
+template <int N, int GL>
 __device__ __forceinline__ void head_rotate(float (&x)[N], const float (&c)[N], const float (&s)[N],
-                                            int half, bool inter, int lane) {
+                                            int half, bool inter, int g) {
   if (inter) {
-    if (lane * N < 2 * half) {
+    if (g * N < 2 * half) {
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         const float a = x[i], b = x[i + 1];
@@ -103,11 +141,11 @@ __device__ __forceinline__ void head_rotate(float (&x)[N], const float (&c)[N], 
     return;
   }
   const int hl = half / N;                        // lanes of half a rotation
-  const bool lo = lane < hl, in = lane < 2 * hl;
-  const int other = in ? (lo ? lane + hl : lane - hl) : lane;
+  const bool lo = g < hl, in = g < 2 * hl;
+  const int other = in ? (lo ? g + hl : g - hl) : g;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float y = __shfl_sync(0xffffffffu, x[i], other);
+    const float y = __shfl_sync(0xffffffffu, x[i], other, GL);
     const float l = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y, s[i]));
     const float h = __fadd_rn(__fmul_rn(y, s[i]), __fmul_rn(x[i], c[i]));
     x[i] = in ? (lo ? l : h) : x[i];
@@ -123,23 +161,23 @@ struct Turn {   // one view of the tables
 
 // this lane's cos and sin at row `pos` (columns beyond the rotated part: unused)
 template <int N>
-__device__ __forceinline__ void load_turn(const Turn &t, long pos, int lane, float (&c)[N],
+__device__ __forceinline__ void load_turn(const Turn &t, long pos, int g, float (&c)[N],
                                           float (&s)[N]) {
   const float *cp = reinterpret_cast<const float *>(t.cos + pos * t.cos_rb);
   const float *sp = reinterpret_cast<const float *>(t.sin + pos * t.sin_rb);
-  if (lane * N >= 2 * t.half) {
+  if (g * N >= 2 * t.half) {
 #pragma unroll
     for (int i = 0; i < N; ++i) c[i] = s[i] = 0.0f;
     return;
   }
   if (t.inter) {
     Elems<float, N / 2> a, b;
-    a.load(cp + lane * (N / 2));
-    b.load(sp + lane * (N / 2));
+    a.load(cp + g * (N / 2));
+    b.load(sp + g * (N / 2));
 #pragma unroll
     for (int i = 0; i < N; ++i) c[i] = a.e[i % (N / 2)], s[i] = b.e[i % (N / 2)];
   } else {
-    const int at = lane * N < t.half ? lane * N : lane * N - t.half;
+    const int at = g * N < t.half ? g * N : g * N - t.half;
     Elems<float, N> a, b;
     a.load(cp + at);
     b.load(sp + at);
@@ -148,34 +186,33 @@ __device__ __forceinline__ void load_turn(const Turn &t, long pos, int lane, flo
   }
 }
 
-// codes of one head's columns and its scale = RN(absmax * RN(1/127))
-template <int N>
-__device__ __forceinline__ float head_int8(const float (&x)[N], void *codes) {
+// codes of one head's columns (stored where ok) and its scale = RN(absmax * RN(1/127))
+template <int N, int GL>
+__device__ __forceinline__ float head_int8(const float (&x)[N], void *codes, bool ok) {
   float m = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
-  const float scale = __fmul_rn(warp_tree_max(m), kInv127);
-  if constexpr (N >= 4) {
-    Elems<int8_t, N> e;
-    uint32_t w[N / 4];
-    quant_pack_absmax<N>(x, scale, w);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint32_t *>(e.e)[i] = w[i];
-    e.store(codes);
+  if constexpr (GL == 32) {
+    m = warp_tree_max(m);
   } else {
-    int q[N];
-    quant_n_absmax<N>(x, scale, q);
-    Elems<int8_t, N> e;
 #pragma unroll
-    for (int i = 0; i < N; ++i) e.e[i] = static_cast<int8_t>(q[i]);
-    e.store(codes);
+    for (int o = 1; o < GL; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
+  const float scale = __fmul_rn(m, kInv127);
+  uint32_t w[N / 4];
+  quant_pack_absmax<N>(x, scale, w);
+  Elems<int8_t, N> e;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint32_t *>(e.e)[i] = w[i];
+  if (ok) e.store(codes);
   return scale;
 }
 
 // ---------------------------------------------------------------------------
-// rotation of rows.  A warp takes U heads of a row: U loads in flight, one read of
-// the row's cos and sin for them.
+// rotation of rows.  A warp takes U times its 32 / GL heads of a row: U 16-byte loads a
+// lane in flight, one read of the row's cos and sin for them.  Loads and stores
+// stream past the caches (8192 rows of 16 heads: 28.2 us against 29.0; 5003
+// bf16 rows of 40 heads 25.8 against 28.5).
 // ---------------------------------------------------------------------------
 constexpr int U = 4;
 struct RowArgs {
@@ -189,48 +226,51 @@ struct RowArgs {
   float inv_hd;
 };
 
-template <typename T, int N>
+template <typename T, int N, int GL>
 __global__ void k_rope_rows(RowArgs p) {
-  constexpr int HD = 32 * N;
-  const int lane = threadIdx.x & 31;
-  const int chunks = (p.heads + U - 1) / U;
+  constexpr int HD = GL * N, HW = 32 / GL;         // heads a warp holds at once
+  const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
+  const int chunks = (p.heads + U * HW - 1) / (U * HW);
   const long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long r = unit / chunks;
   if (r >= p.rows) return;
-  const int h0 = static_cast<int>(unit % chunks) * U, nh = min(U, p.heads - h0);
+  const int h0 = static_cast<int>(unit - r * chunks) * (U * HW);
   Elems<T, N> e[U];
-  const char *xp = p.x + r * p.x_rb + (static_cast<long>(h0) * HD + lane * N) * sizeof(T);
+  const char *xp = p.x + r * p.x_rb + (static_cast<long>(h0 + hl) * HD + g * N) * sizeof(T);
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (u < nh) e[u].load(xp + u * HD * sizeof(T));
+    if (h0 + u * HW + hl < p.heads) e[u].load_stream(xp + static_cast<long>(u) * HW * HD * sizeof(T));
+    else e[u].zero();
   float w[N], c[N], s[N];
   if (p.nw) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = p.nw[lane * N + i];
+    for (int i = 0; i < N; ++i) w[i] = p.nw[g * N + i];
   }
   const int pos = p.pos[r];
   if (pos < 0 || pos >= p.t.rows) {
     if (lane == 0) atomicOr(&g_rope_error, kBadPosition);
     return;
   }
-  load_turn<N>(p.t, pos, lane, c, s);
+  load_turn<N>(p.t, pos, g, c, s);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (u >= nh) break;
-    const int h = h0 + u;
+    if (h0 + u * HW >= p.heads) break;
+    const int h = h0 + u * HW + hl;
+    const bool ok = h < p.heads;
     float x[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = to_f32(e[u].e[i]);
-    if (p.nw) head_norm<N>(x, w, p.inv_hd);
-    head_rotate<N>(x, c, s, p.t.half, p.t.inter, lane);
-    const long col = static_cast<long>(h) * HD + lane * N;
+    if (p.nw) head_norm<N, GL>(x, w, p.inv_hd);
+    head_rotate<N, GL>(x, c, s, p.t.half, p.t.inter, g);
+    const long col = static_cast<long>(h) * HD + g * N;
     char *o = p.out + r * p.out_rb;
-    if (p.out_dt == Q3_DT_F32) store_row<float, N>(x, o + col * 4);
-    else if (p.out_dt == Q3_DT_F16) store_row<__half, N>(x, o + col * 2);
-    else if (p.out_dt == Q3_DT_BF16) store_row<__nv_bfloat16, N>(x, o + col * 2);
-    else {
-      const float sc = head_int8<N>(x, o + col);
-      if (lane == 0) reinterpret_cast<float *>(p.scale + r * p.scale_rb)[h] = sc;
+    if (p.out_dt == Q3_DT_I8) {
+      const float sc = head_int8<N, GL>(x, o + col, ok);
+      if (g == 0 && ok) reinterpret_cast<float *>(p.scale + r * p.scale_rb)[h] = sc;
+    } else if (ok) {
+      if (p.out_dt == Q3_DT_F32) store_row_stream<float, N>(x, o + col * 4);
+      else if (p.out_dt == Q3_DT_F16) store_row_stream<__half, N>(x, o + col * 2);
+      else store_row_stream<__nv_bfloat16, N>(x, o + col * 2);
     }
   }
 }
@@ -253,34 +293,35 @@ struct AppendArgs {
   int n_seqs, rows, kv_heads;
 };
 
-template <typename T, int N>
+template <typename T, int N, int GL>
 __global__ void k_kv_append(AppendArgs p) {
-  constexpr int HD = 32 * N;
-  const int lane = threadIdx.x & 31;
-  const int chunks = (p.kv_heads + U - 1) / U;
+  constexpr int HD = GL * N, HW = 32 / GL;
+  const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
+  const int chunks = (p.kv_heads + U * HW - 1) / (U * HW);
   long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long r = unit / (2 * chunks);
   if (r >= p.rows) return;
-  unit %= 2 * chunks;
+  unit -= r * (2 * chunks);
   const bool is_v = unit >= chunks;
-  const int h0 = static_cast<int>(is_v ? unit - chunks : unit) * U, nh = min(U, p.kv_heads - h0);
+  const int h0 = static_cast<int>(is_v ? unit - chunks : unit) * (U * HW);
   Elems<T, N> e[U];
   const char *xp = (is_v ? p.v + r * p.v_rb : p.k + r * p.k_rb) +
-                   (static_cast<long>(h0) * HD + lane * N) * sizeof(T);
+                   (static_cast<long>(h0 + hl) * HD + g * N) * sizeof(T);
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (u < nh) e[u].load(xp + u * HD * sizeof(T));
+    if (h0 + u * HW + hl < p.kv_heads) e[u].load_stream(xp + static_cast<long>(u) * HW * HD * sizeof(T));
+    else e[u].zero();
   const bool norm = !is_v && p.nw, turn = !is_v && p.t.half;
   float w[N], c[N], s[N];
   if (norm) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = p.nw[lane * N + i];
+    for (int i = 0; i < N; ++i) w[i] = p.nw[g * N + i];
   }
   int first, count;
   const int q = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
   if (q < 0) return;                               // a row that belongs to nobody
   const long pos = static_cast<long>(p.kv_len[q]) - count + (r - first);
-  const long lp = pos / p.page_tokens;
+  const long lp = pos < 0 ? 0 : static_cast<long>(static_cast<uint64_t>(pos) / p.page_tokens);
   unsigned bad = 0;
   uint32_t page = 0;
   if (pos < 0) bad = kBadRagged;
@@ -294,8 +335,8 @@ __global__ void k_kv_append(AppendArgs p) {
     if (lane == 0) atomicOr(&g_rope_error, bad);
     return;
   }
-  if (turn) load_turn<N>(p.t, pos, lane, c, s);
-  const uint32_t slot = static_cast<uint32_t>(pos % p.page_tokens);
+  if (turn) load_turn<N>(p.t, pos, g, c, s);
+  const uint32_t slot = static_cast<uint32_t>(pos - lp * p.page_tokens);
   char *codes = (is_v ? p.pv : p.pk) + static_cast<size_t>(page) * p.page_bytes +
                 static_cast<size_t>(slot) * p.row_bytes;
   float *scale = reinterpret_cast<float *>((is_v ? p.pvs : p.pks) +
@@ -303,14 +344,16 @@ __global__ void k_kv_append(AppendArgs p) {
                                            static_cast<size_t>(slot) * p.scale_row_bytes);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (u >= nh) break;
+    if (h0 + u * HW >= p.kv_heads) break;
+    const int h = h0 + u * HW + hl;
+    const bool ok = h < p.kv_heads;
     float x[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = to_f32(e[u].e[i]);
-    if (norm) head_norm<N>(x, w, p.inv_hd);
-    if (turn) head_rotate<N>(x, c, s, p.t.half, p.t.inter, lane);
-    const float sc = head_int8<N>(x, codes + static_cast<long>(h0 + u) * HD + lane * N);
-    if (lane == 0) scale[h0 + u] = sc;
+    if (norm) head_norm<N, GL>(x, w, p.inv_hd);
+    if (turn) head_rotate<N, GL>(x, c, s, p.t.half, p.t.inter, g);
+    const float sc = head_int8<N, GL>(x, codes + static_cast<long>(h) * HD + g * N, ok);
+    if (g == 0 && ok) scale[h] = sc;
   }
 }
 
@@ -391,8 +434,11 @@ extern "C" int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_
     high = high > rot - 1.0 ? rot - 1.0 : high;
   }
   const double span = high - low > 1e-3 ? high - low : 1e-3;
-  for (uint32_t i = 0; i < half; ++i) {
-    long double f = expl(-2.0L * i / rot * logl((long double)spec->theta));
+  // powers by products: 128 roundings of 2^-64 stay below 2^-56
+  const long double ratio = expl(-2.0L / rot * logl((long double)spec->theta));
+  long double power = 1.0L;
+  for (uint32_t i = 0; i < half; ++i, power *= ratio) {
+    long double f = power;
     if (spec->scaling == Q3_ROPE_LINEAR) f /= spec->factor;
     if (yarn) {
       double ramp = (i - low) / span;
@@ -420,11 +466,13 @@ extern "C" int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_
 
 template <typename T>
 static int launch_rows(const RowArgs &p, uint32_t hd, cudaStream_t s) {
-  const long warps = static_cast<long>(p.rows) * ((p.heads + U - 1) / U);
+  constexpr int N = 16 / static_cast<int>(sizeof(T));   // head_dim 256: 8 columns a lane
+  const int per = U * (hd >= 32 * N ? 1 : 32 * N / static_cast<int>(hd));   // heads of a warp
+  const long warps = static_cast<long>(p.rows) * ((p.heads + per - 1) / per);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-  if (hd == 64) k_rope_rows<T, 2><<<blocks, 128, 0, s>>>(p);
-  else if (hd == 128) k_rope_rows<T, 4><<<blocks, 128, 0, s>>>(p);
-  else k_rope_rows<T, 8><<<blocks, 128, 0, s>>>(p);
+  if (hd == 64) k_rope_rows<T, N, 64 / N><<<blocks, 128, 0, s>>>(p);
+  else if (hd == 128) k_rope_rows<T, N, 128 / N><<<blocks, 128, 0, s>>>(p);
+  else k_rope_rows<T, 8, 32><<<blocks, 128, 0, s>>>(p);
   return launch_status();
 }
 
@@ -471,11 +519,13 @@ extern "C" int q3_rope_rows(const q3_view *x, const q3_view *nw, const int32_t *
 
 template <typename T>
 static int launch_append(const AppendArgs &p, uint32_t hd, cudaStream_t s) {
-  const long warps = static_cast<long>(p.rows) * 2 * ((p.kv_heads + U - 1) / U);
+  constexpr int N = 16 / static_cast<int>(sizeof(T));   // head_dim 256: 8 columns a lane
+  const int per = U * (hd >= 32 * N ? 1 : 32 * N / static_cast<int>(hd));   // heads of a warp
+  const long warps = static_cast<long>(p.rows) * 2 * ((p.kv_heads + per - 1) / per);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-  if (hd == 64) k_kv_append<T, 2><<<blocks, 128, 0, s>>>(p);
-  else if (hd == 128) k_kv_append<T, 4><<<blocks, 128, 0, s>>>(p);
-  else k_kv_append<T, 8><<<blocks, 128, 0, s>>>(p);
+  if (hd == 64) k_kv_append<T, N, 64 / N><<<blocks, 128, 0, s>>>(p);
+  else if (hd == 128) k_kv_append<T, N, 128 / N><<<blocks, 128, 0, s>>>(p);
+  else k_kv_append<T, 8, 32><<<blocks, 128, 0, s>>>(p);
   return launch_status();
 }
 
