@@ -532,6 +532,9 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
     }
   }
   pdl_trigger();
+  // as a dependent of the many-row kernel it began when all CTAs of that were running; what comes
+  // after waits for both
+  pdl_wait();
 }
 
 // The parts of one packed row of a (sequence, KV head) pair joined by a CTA: its warps take them in
@@ -734,11 +737,10 @@ static int opt_in(int bytes) {
 }
 
 template <int HD, int NT>
-static int launch_few(const chunk::Args &p, int ctas, cudaStream_t s) {
+static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t s) {
   constexpr int smem = chunk::WARPS * chunk::FewStage<HD>::STAGES * (int)sizeof(chunk::FewStage<HD>);
   Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
-  chunk::k_attn_few<HD, NT><<<ctas, chunk::WARPS * 32, smem, s>>>(p);
-  Q3_TRY(launch_status());
+  Q3_TRY(launch_ex(beside, chunk::k_attn_few<HD, NT>, dim3(ctas), dim3(chunk::WARPS * 32), smem, s, p));
   const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
   const unsigned z = static_cast<unsigned>(packed < p.part_rows ? packed : p.part_rows);
   return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, z),
@@ -835,22 +837,23 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   timer_begin(TIMER_ATTENTION, s);
   int st = Q3_OK;
   float *ws = static_cast<float *>(workspace);
-  if (c.few_ctas) {
-    chunk::Args f = p;
-    f.part_rows = 8 * c.nt;
-    f.part_o = ws;
-    f.part_ml = ws + c.few_slots * head_dim;
-    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(f, c.few_ctas, s)
-                                      : launch_few<128, 2>(f, c.few_ctas, s))
-                         : (c.nt == 1 ? launch_few<64, 1>(f, c.few_ctas, s)
-                                      : launch_few<64, 2>(f, c.few_ctas, s));
+  if (c.tiles) {
+    chunk::Args t = p;
+    t.splits = c.splits;
+    t.tiles = static_cast<int>(c.tiles);
+    t.part_o = ws + c.few_slots * (head_dim + 2);
+    t.part_ml = t.part_o + static_cast<size_t>(c.splits) * rows * heads * head_dim;
+    st = head_dim == 128 ? launch_many<128>(t, s) : launch_many<64>(t, s);
   }
-  if (st == Q3_OK && c.tiles) {
-    p.splits = c.splits;
-    p.tiles = static_cast<int>(c.tiles);
-    p.part_o = ws + c.few_slots * (head_dim + 2);
-    p.part_ml = p.part_o + static_cast<size_t>(c.splits) * rows * heads * head_dim;
-    st = head_dim == 128 ? launch_many<128>(p, s) : launch_many<64>(p, s);
+  if (st == Q3_OK && c.few_ctas) {
+    p.part_rows = 8 * c.nt;
+    p.part_o = ws;
+    p.part_ml = ws + c.few_slots * head_dim;
+    const bool beside = c.tiles && c.splits == 1;   // the kernel before is the many-row one
+    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, c.few_ctas, beside, s)
+                                      : launch_few<128, 2>(p, c.few_ctas, beside, s))
+                         : (c.nt == 1 ? launch_few<64, 1>(p, c.few_ctas, beside, s)
+                                      : launch_few<64, 2>(p, c.few_ctas, beside, s));
   }
   timer_end(TIMER_ATTENTION, s);
   return st;

@@ -54,7 +54,7 @@ struct TcSmem {
   alignas(16) float ks[INFO][TC_KEYS], lv[INFO][TC_KEYS], rv[INFO][TC_KEYS];
   long long place[INFO][TC_KEYS];                  // byte offset of a key's row in the pool, or -1
   float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS];
-  unsigned long long full[RING], empty[RING], info_full[INFO], info_empty[INFO];
+  unsigned long long full[RING], empty[RING], place_full[INFO], info_full[INFO], info_empty[INFO];
   unsigned long long s_full[2][2], p_full[2][2], o_full;   // [row tile][half & 1]
   uint32_t tmem;
   int abort;
@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   // KV heads first: they share the tile's row arrays, and heavy tiles of a sequence start together
   const int kvh = blockIdx.x % p.kv_heads, tile_id = blockIdx.x / p.kv_heads;
 
+  pdl_trigger();   // the few-row kernel may fill the SMs that this grid leaves
   if (warp == 0) {
     unsigned err = 0;
     long before;
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         mbar_init(&sm.empty[i], 1);
       }
       for (int i = 0; i < INFO; ++i) {
+        mbar_init(&sm.place_full[i], 1);
         mbar_init(&sm.info_full[i], 1);
         mbar_init(&sm.info_empty[i], LOADERS + ROW_WARPS);
       }
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     auto request = [&](int item) {
       if (item < items) {
         const int j = item >> 1, in = j % INFO;
-        wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
+        wait_bar(&sm.place_full[in], (j / INFO) & 1, &sm.abort);
         const char *from = ((item & 1) ? p.v : p.k) + kcol;
         const uint32_t dst = su32(raw + (item % RAW) * (TC_KEYS * HD / 16));
 #pragma unroll
@@ -693,8 +695,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == INFO_WARP) {
     // ------------------------------------------------------------------ places and scales
-    // A lane has keys i*32 + lane of a tile.  Pages are looked up two tiles ahead, scales
-    // requested one tile ahead.
+    // A lane has keys i*32 + lane of a tile.  Pages are looked up two tiles ahead; a tile's places
+    // are published, and its scales requested, one tile ahead.
     const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
     auto page_of = [&](int j, int (&pg)[4]) {
 #pragma unroll
@@ -703,51 +705,56 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         pg[i] = j < nj && key < q.kv ? table[page_index(p, key)] : -1;
       }
     };
-    struct Keys {
-      long long at[4];
+    struct Scales {
+      bool have[4];
       float ks[4], vs[4];
     };
-    auto request = [&](int j, const int (&pg)[4], Keys &k) {
+    auto publish = [&](int j, const int (&pg)[4], Scales &k) {
+      if (j >= nj) return;
+      const int in = j % INFO;
+      if (j >= INFO) wait_bar(&sm.info_empty[in], ((j / INFO) - 1) & 1, &sm.abort);
+      size_t so[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = (z0 + j) * TC_KEYS + i * 32 + lane;
-        k.at[i] = -1;
+        const uint32_t key = (z0 + j) * TC_KEYS + i * 32 + lane, slot = page_slot(p, key);
+        k.have[i] = pg[i] >= 0 && static_cast<uint32_t>(pg[i]) < p.num_pages;
+        if (pg[i] >= 0 && !k.have[i]) atomicOr(&g_chunk_tc_error, kBadPage);
+        sm.place[in][i * 32 + lane] = k.have[i] ? static_cast<long long>(pg[i]) * p.page_bytes +
+                                                      static_cast<long long>(slot) * p.row_bytes
+                                                : -1;
+        so[i] = k.have[i] ? static_cast<size_t>(pg[i]) * p.scale_page_bytes +
+                                static_cast<size_t>(slot) * p.scale_row_bytes + kvh * 4
+                          : 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.place_full[in]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         k.ks[i] = k.vs[i] = 0.0f;
-        if (pg[i] >= 0) {
-          if (static_cast<uint32_t>(pg[i]) < p.num_pages) {
-            const uint32_t slot = page_slot(p, key);
-            k.at[i] = static_cast<long long>(pg[i]) * p.page_bytes +
-                      static_cast<long long>(slot) * p.row_bytes;
-            const size_t so = static_cast<size_t>(pg[i]) * p.scale_page_bytes +
-                              static_cast<size_t>(slot) * p.scale_row_bytes + kvh * 4;
-            k.ks[i] = __ldg(reinterpret_cast<const float *>(p.ks + so));
-            k.vs[i] = __ldg(reinterpret_cast<const float *>(p.vs + so));
-          } else {
-            atomicOr(&g_chunk_tc_error, kBadPage);
-          }
+        if (k.have[i]) {
+          k.ks[i] = __ldg(reinterpret_cast<const float *>(p.ks + so[i]));
+          k.vs[i] = __ldg(reinterpret_cast<const float *>(p.vs + so[i]));
         }
       }
     };
-    int pg[4];
-    Keys now;
+    int pg[4], pg1[4];
+    Scales now;
     page_of(0, pg);
-    request(0, pg, now);
-    page_of(1, pg);
+    page_of(1, pg1);
+    publish(0, pg, now);
     for (int j = 0; j < nj; ++j) {
       const int in = j % INFO;
-      Keys next;
-      request(j + 1, pg, next);
-      page_of(j + 2, pg);
-      if (j >= INFO) wait_bar(&sm.info_empty[in], ((j / INFO) - 1) & 1, &sm.abort);
+      Scales next;
+      publish(j + 1, pg1, next);
+      page_of(j + 2, pg1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = i * 32 + lane, k = key & 15;
         const int to = (key & ~15) + ((k & 7) >> 1) * 4 + (k >> 3) * 2 + (k & 1);
         const float v = fmaxf(now.vs[i], kVsMin);    // (NaN: fmaxf drops it ...
-        sm.place[in][key] = now.at[i];
         sm.ks[in][to] = __fmul_rn(now.ks[i], p.scale_log2);
         // ... and the rows that see it get NaN); a key that is not there: weight 0
-        sm.lv[in][to] = now.at[i] < 0 ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
+        sm.lv[in][to] = !now.have[i] ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
         sm.rv[in][to] = rcp(v);
       }
       __syncwarp();

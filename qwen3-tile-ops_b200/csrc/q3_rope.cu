@@ -459,7 +459,7 @@ extern "C" int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_
   p.half = (int)half;
   p.pos0 = pos0;
   const int threads = 256, per = threads / (int)half;
-  const long blocks = ((long)p.rows + per - 1) / per, most = 16L * sm_count();
+  const long blocks = ((long)p.rows + per - 1) / per, most = 4L * sm_count();
   k_rope_tables<<<(unsigned)(blocks < most ? blocks : most), threads, 0, (cudaStream_t)stream>>>(p);
   return launch_status();
 }
