@@ -728,6 +728,7 @@ static int opt_in(int bytes) {
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) {
+      cudaGetLastError();
       set_cuda_error(e);
       return Q3_ERR_CUDA;
     }

@@ -851,6 +851,7 @@ static int launch(const Args &p, cudaStream_t s) {
     const cudaError_t e =
         cudaFuncSetAttribute(k_attn_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) {
+      cudaGetLastError();
       q3h::set_cuda_error(e);
       return Q3_ERR_CUDA;
     }

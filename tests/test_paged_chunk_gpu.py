@@ -628,3 +628,68 @@ def test_attention_stream_argument(ops):
     torch.cuda.current_stream().wait_stream(s)
     want, tol = ref_attention(P, q64, 4, True, 0, 0.125)
     check_rows(o, None, want, tol, 4, 64, P.rows)
+
+
+def test_mixed_batch_captured_and_beside_itself(ops):
+    """A batch of decode rows and prompt chunks (both attention kernels, split keys, the joins) in a
+    graph, replayed after its lengths, rows and pages changed, while the same call runs on a second
+    stream with a workspace of its own."""
+    heads, kvh, hd = 8, 2, 128
+    lens = [(1, 3000), (70, 1500), (0, 5), (300, 900), (4, 64), (129, 129)]
+    P = Pool(ops, lens, kvh, hd, seed=12)
+    n = len(lens)
+    size = max(16, ops.attention_chunk_workspace_bytes(P.rows, n, 300, P.mp * 32, heads, kvh, hd))
+    q, _, _ = make_q(P, heads, "f16", 3)
+    ws = [torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    out = [torch.full((P.rows, heads * hd), 7.0, device="cuda", dtype=torch.float16)
+           for _ in range(2)]
+
+    def call(i):
+        ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, n, 300,
+                                  out[i], None, heads, kvh, hd, True, 0, hd ** -0.5, workspace=ws[i])
+    call(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(0)
+    side = torch.cuda.Stream()
+    for step in range(3):
+        q.mul_(1.1)
+        lens = [(a, b - step * (b > a + 2)) for a, b in lens]
+        if step:   # rows move from one sequence to another, within max_rows
+            lens[0], lens[1] = (lens[0][0] + 20, lens[0][1]), (lens[1][0] - 20, lens[1][1])
+        P.lens = lens
+        P.row0.copy_(torch.tensor(np.cumsum([0] + [a for a, _ in lens]), dtype=torch.int32))
+        P.kv_len.copy_(torch.tensor([b for _, b in lens], dtype=torch.int32))
+        P.tables.copy_(P.tables.flip(0))
+        for o in out:
+            o.fill_(7.0)
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            call(1)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(out[0], out[1])
+        want, tol = ref_attention(P, q.double().view(-1, heads, hd), heads, True, 0, hd ** -0.5)
+        check_rows(out[0], None, want, tol, heads, hd, P.rows)
+
+
+@pytest.mark.parametrize("seqs", [40, 1100])
+def test_many_sequences(ops, seqs):
+    """More sequences than a warp's lanes, and than its second look-up round."""
+    rng = np.random.default_rng(seqs)
+    lens = [(int(a), int(a) + int(b)) for a, b in zip(rng.integers(0, 4, seqs),
+                                                      rng.integers(0, 60, seqs))]
+    lens[seqs // 2] = (37, 64)
+    P = Pool(ops, lens, 1, 64, page=16, seed=seqs)
+    x = torch.randn(P.rows, 64, device="cuda", generator=gen(2)).half()
+    cos, sin = tables_f32(P.mp * 16, 64)
+    ops.paged_kv_append_batch(x, x, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, seqs, 1, 64,
+                              cos=cos, sin=sin)
+    v, r = [], 0
+    for s, (a, b) in enumerate(lens):                  # the last rows' V codes, as appended
+        (_, _), (v8, vs) = P.cached(s)
+        v.append((v8 * vs[..., None])[b - a:b, 0])
+    v = torch.cat(v)
+    assert ((v - x.double()).abs() <= x.double().abs().amax(-1, keepdim=True) / 127 * 0.501).all()
+    run_attention(ops, P, 2, "f16", "bf16")
