@@ -65,6 +65,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 constexpr int WARPS = 4;
 constexpr int KB = 32;                             // keys of a block
 constexpr int MIN_UNITS = 4;                       // least run of a warp
+constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that is never cut
 
 template <int HD>
 struct FewStage {
@@ -162,25 +163,44 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
   const uint32_t w = blockIdx.x * WARPS + wid, slice = w / p.kv_heads;
   const int kvh = w - slice * p.kv_heads;
 
+  pdl_trigger();   // the join may start: it looks up its parts while this kernel works
   unsigned err = 0;
-  uint32_t none;
-  const uint32_t total = count_units(p, 0, lane, &err, none);
-  if (w == 0 && err) atomicOr(&g_chunk_error, err);
-  const Slices cut(total, gridDim.x * WARPS / p.kv_heads);
-  if (total && slice < cut.n) {
-    uint32_t u = cut.first(slice);
-    const uint32_t u1 = cut.first(slice + 1);
-    long before;
-    int s = find_unit(p.n_seqs, u, lane, before, [&](int x) { return units_of(p, x, &err); });
-    while (u < u1 && s >= 0 && s < p.n_seqs) {
+  uint32_t u = 0, u1 = 1;
+  long before = 0;
+  int s = -1;
+  if (p.whole) {   // a sequence a slice: nothing to look up, no parts
+    if (slice < static_cast<uint32_t>(p.n_seqs)) s = slice;
+    if (s >= 0 && kvh == 0) {
+      load_seq(p, s, &err);
+      if (err && lane == 0) atomicOr(&g_chunk_error, err);
+    }
+  } else {
+    // sequences 0 .. 31 in registers; more are looked up in turn
+    const uint32_t mine = lane < p.n_seqs ? units_of(p, lane, &err) : 0;
+    uint32_t total = __reduce_add_sync(0xffffffffu, mine);
+    for (int x = 32 + lane; x - lane < p.n_seqs; x += 32)
+      total += __reduce_add_sync(0xffffffffu, x < p.n_seqs ? units_of(p, x, &err) : 0);
+    if (w == 0 && err) atomicOr(&g_chunk_error, err);
+    const Slices cut(total, gridDim.x * WARPS / p.kv_heads);
+    if (total && slice < cut.n) {
+      u = cut.first(slice);
+      u1 = cut.first(slice + 1);
+      s = find_unit(p.n_seqs, u, lane, before,
+                    [&](int x) { return x == lane ? mine : units_of(p, x, &err); });
+    }
+  }
+  if (s >= 0) {
+    while (u < u1 && s < p.n_seqs) {
       // the sequence of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
       const Seq q = load_seq(p, s, &err);
       int pb0;
       const int pn = seq_units(p, q, pb0);
       if (pn == 0) {
+        if (p.whole) break;
         ++s;
         continue;
       }
+      if (p.whole) u1 = pn;
       const int off = static_cast<int>(u - static_cast<uint32_t>(before));
       const int b = pb0 + off;
       const int run = static_cast<int>(u1 - u) < pn - off ? static_cast<int>(u1 - u) : pn - off;
@@ -531,7 +551,6 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
       ++s;
     }
   }
-  pdl_trigger();
   // as a dependent of the many-row kernel it began when all CTAs of that were running; what comes
   // after waits for both
   pdl_wait();
@@ -661,6 +680,7 @@ __global__ void k_join_tiles(const Args p) {
 // the others to the tensor-core kernel of many rows.
 struct Plan {
   int nt, few_rows, few_ctas;                      // few_ctas 0: no such sequence can be there
+  bool whole;                                      // their keys are not cut
   long tiles;                                      // tiles 0: likewise
   int splits;
   size_t few_slots, bytes;                         // parts of k_attn_few; the whole workspace
@@ -674,13 +694,17 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
   c.few_rows = 16;
   c.nt = packed > 8 && group <= c.few_rows ? 2 : 1;
   if (group <= c.few_rows) {
+    // Up to 256 keys a warp takes a whole sequence: its 8 blocks cost what 4 of them and the join do
+    c.whole = max_kv <= WHOLE_KEYS;
     const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB);
     const long slices = (units + MIN_UNITS - 1) / MIN_UNITS;
     const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2), least = (kv_heads + WARPS - 1) / WARPS;
     long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
     ctas = ctas < most ? ctas : most;
-    c.few_ctas = static_cast<int>(ctas > least ? ctas : least);   // a slice at least
-    c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
+    ctas = ctas > least ? ctas : least;            // a slice at least
+    if (c.whole) ctas = (static_cast<long>(n_seqs) * kv_heads + WARPS - 1) / WARPS;
+    c.few_ctas = static_cast<int>(ctas);
+    if (!c.whole) c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
   }
   c.splits = 1;
   if (packed > c.few_rows) {
@@ -744,6 +768,7 @@ static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t 
   Q3_TRY(launch_ex(beside, chunk::k_attn_few<HD, NT>, dim3(ctas), dim3(chunk::WARPS * 32), smem, s, p));
   const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
   const unsigned z = static_cast<unsigned>(packed < p.part_rows ? packed : p.part_rows);
+  if (p.whole) return Q3_OK;
   return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, z),
                    dim3(chunk::JOIN_WARPS * 32), 0, s, p,
                    static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads);
@@ -792,7 +817,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   const uint32_t max_kv = max_pages * kv->page_tokens;
   const chunk::Plan c =
       chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
-  if (c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
+  if (static_cast<uint64_t>(n_seqs) * kv_heads > 0x7fffffffu || c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
     return Q3_ERR_SHAPE;
   if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;
@@ -848,6 +873,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   }
   if (st == Q3_OK && c.few_ctas) {
     p.part_rows = 8 * c.nt;
+    p.whole = c.whole;
     p.part_o = ws;
     p.part_ml = ws + c.few_slots * head_dim;
     const bool beside = c.tiles && c.splits == 1;   // the kernel before is the many-row one

@@ -24,6 +24,7 @@ struct Args {
   int tiles;                     // query tiles a sequence may have
   int few_rows;                  // packed rows of a sequence that k_attn_few takes
   int part_rows;                 // rows of one of its parts
+  int whole;                     // it takes a sequence's keys as a whole
   int page_shift;                // log2 of page_tokens, or -1
   int whole_blocks;              // a 32-key block lies in one page
   float *part_o, *part_ml;       // parts: sums [..][hd], and their (maximum, sum of weights)
