@@ -168,9 +168,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
   uint32_t u = 0, u1 = 1;
   long before = 0;
   int s = -1;
-  if (p.whole) {   // a sequence a slice: nothing to look up, no parts
-    if (slice < static_cast<uint32_t>(p.n_seqs)) s = slice;
-    if (s >= 0 && kvh == 0) {
+  int m0 = 0;                                      // first packed row of this warp's
+  if (p.whole) {   // 8 NT packed rows of a sequence a slice: nothing to look up, no parts
+    const uint32_t at = slice / p.tiles;
+    m0 = static_cast<int>(slice - at * p.tiles) * (8 * NT);
+    if (at < static_cast<uint32_t>(p.n_seqs)) s = at;
+    if (s >= 0 && kvh == 0 && m0 == 0) {
       load_seq(p, s, &err);
       if (err && lane == 0) atomicOr(&g_chunk_error, err);
     }
@@ -193,21 +196,26 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
     while (u < u1 && s < p.n_seqs) {
       // the sequence of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
       const Seq q = load_seq(p, s, &err);
-      int pb0;
-      const int pn = seq_units(p, q, pb0);
-      if (pn == 0) {
+      int pb0, pn = seq_units(p, q, pb0);
+      const int packed = min(8 * NT, q.n * p.group - m0);
+      if (pn == 0 || packed <= 0) {
         if (p.whole) break;
         ++s;
         continue;
       }
-      if (p.whole) u1 = pn;
+      const int pmin = q.pos0 + m0 / p.group;      // position of the first of the rows
+      if (p.whole) {
+        int lo, hi;
+        key_range(p, q, pmin, q.pos0 + (m0 + packed - 1) / p.group, lo, hi);
+        pb0 = lo / KB;
+        pn = (hi + KB - 1) / KB - pb0;
+        u1 = pn;
+      }
       const int off = static_cast<int>(u - static_cast<uint32_t>(before));
       const int b = pb0 + off;
       const int run = static_cast<int>(u1 - u) < pn - off ? static_cast<int>(u1 - u) : pn - off;
       const int be = b + run;
       const bool whole = off == 0 && run == pn;
-      const int packed = q.n * p.group;
-
       const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
       const long kcol = static_cast<long>(kvh) * HD;
       // table index and slot of key x*32 + lane; its page is requested one step before it is used
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
         float scale = 0.0f;
 #pragma unroll
         for (int x = 0; x < KW; ++x) qf[n][x][0] = qf[n][x][1] = 0;
-        const int mm = min(m, packed - 1);
+        const int mm = m0 + min(m, packed - 1);
         const long r = q.first + mm / p.group;
         const int h = kvh * p.group + mm % p.group;
         const char *qp = p.q + r * p.q_rb;
@@ -341,7 +349,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           a[n][j] = __shfl_sync(0xffffffffu, scale, (t4 * 2 + j) * 4);
-          pq[n][j] = q.pos0 + min(n * 8 + t4 * 2 + j, packed - 1) / p.group;
+          pq[n][j] = q.pos0 + (m0 + min(n * 8 + t4 * 2 + j, packed - 1)) / p.group;
           mref[n][j] = kNegInf;
           lsum[n][j] = 0.0f;
         }
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
           rv[i] = rcp(fmaxf(v, kVsMin));             // (NaN: fmaxf drops it ...
           lv[i] = v != v ? v : lg2(fmaxf(v, kVsMin));// ... and the rows that see it get NaN)
         }
-        const bool masked = mask != 0xffffffffu || x * KB + KB - 1 > q.pos0 || p.window > 0;
+        const bool masked = mask != 0xffffffffu || x * KB + KB - 1 > pmin || p.window > 0;
         // relative to the reference of the row's weights, which moves when one outgrows it by 2^8
         float top[NT][2];
         bool grow = false;
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
             const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);   // no key seen: zeros
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) y[i] = __fmul_rn(y[i], inv);
-            const int mm = min(m, packed - 1);
+            const int mm = m0 + min(m, packed - 1);
             store_part8<HD / 8>(p, q.first + mm / p.group, kvh * p.group + mm % p.group, g, ok, y);
           } else if (ok) {
             const long at = slot * p.part_rows + m;
@@ -679,7 +687,8 @@ __global__ void k_join_tiles(const Args p) {
 // How a call is cut.  Sequences with at most few_rows packed rows go to k_attn_few (nt tiles of 8),
 // the others to the tensor-core kernel of many rows.
 struct Plan {
-  int nt, few_rows, few_ctas;                      // few_ctas 0: no such sequence can be there
+  int nt, few_rows;
+  long few_ctas, few_tiles;                        // few_ctas 0: no such sequence can be there
   bool whole;                                      // their keys are not cut
   long tiles;                                      // tiles 0: likewise
   int splits;
@@ -694,7 +703,8 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
   c.few_rows = 16;
   c.nt = packed > 8 && group <= c.few_rows ? 2 : 1;
   if (group <= c.few_rows) {
-    // Up to 256 keys a warp takes a whole sequence: its 8 blocks cost what 4 of them and the join do
+    // Up to 256 keys a warp takes a whole sequence: its 8 blocks cost what 4 of them and the join do,
+    // and less than the 12 us that a CTA of many rows takes to start and end
     c.whole = max_kv <= WHOLE_KEYS;
     const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB);
     const long slices = (units + MIN_UNITS - 1) / MIN_UNITS;
@@ -702,8 +712,12 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
     long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
     ctas = ctas < most ? ctas : most;
     ctas = ctas > least ? ctas : least;            // a slice at least
-    if (c.whole) ctas = (static_cast<long>(n_seqs) * kv_heads + WARPS - 1) / WARPS;
-    c.few_ctas = static_cast<int>(ctas);
+    if (c.whole) {   // then all rows go there, in tiles
+      c.few_rows = 0x7fffffff;
+      c.few_tiles = (packed + 8 * c.nt - 1) / (8 * c.nt);
+      ctas = (static_cast<long>(n_seqs) * c.few_tiles * kv_heads + WARPS - 1) / WARPS;
+    }
+    c.few_ctas = ctas;
     if (!c.whole) c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
   }
   c.splits = 1;
@@ -817,7 +831,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   const uint32_t max_kv = max_pages * kv->page_tokens;
   const chunk::Plan c =
       chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
-  if (static_cast<uint64_t>(n_seqs) * kv_heads > 0x7fffffffu || c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
+  if (c.few_ctas > 0x7fffffff / chunk::WARPS || c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
     return Q3_ERR_SHAPE;
   if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;
@@ -874,13 +888,15 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   if (st == Q3_OK && c.few_ctas) {
     p.part_rows = 8 * c.nt;
     p.whole = c.whole;
+    p.tiles = static_cast<int>(c.few_tiles);
     p.part_o = ws;
     p.part_ml = ws + c.few_slots * head_dim;
     const bool beside = c.tiles && c.splits == 1;   // the kernel before is the many-row one
-    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, c.few_ctas, beside, s)
-                                      : launch_few<128, 2>(p, c.few_ctas, beside, s))
-                         : (c.nt == 1 ? launch_few<64, 1>(p, c.few_ctas, beside, s)
-                                      : launch_few<64, 2>(p, c.few_ctas, beside, s));
+    const int ctas = static_cast<int>(c.few_ctas);
+    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, ctas, beside, s)
+                                      : launch_few<128, 2>(p, ctas, beside, s))
+                         : (c.nt == 1 ? launch_few<64, 1>(p, ctas, beside, s)
+                                      : launch_few<64, 2>(p, ctas, beside, s));
   }
   timer_end(TIMER_ATTENTION, s);
   return st;
