@@ -126,6 +126,33 @@ def test_rope_rows(ops, rows, heads, hd, rot, inter, xt, ot, norm):
     assert (out[rows:] == 7.0).all()
 
 
+@pytest.mark.parametrize("hd,rot,inter", [(64, 64, False), (64, 32, True), (128, 128, False),
+                                          (256, 128, False), (256, 256, True)])
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rope_rows_codes(ops, hd, rot, inter, xt, norm):
+    """int8 output: the bits of the float32 steps, through MatrixViews, heads left over in a warp."""
+    rows, heads, V = 11, 13, ops.MatrixView
+    g = gen(hd + rot)
+    x = torch.randn(rows, heads * hd, device="cuda", generator=g).to(TYPES[xt])
+    pos = torch.randint(0, 70, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    cos, sin = tables_f32(70, rot)
+    nw = torch.rand(1, hd, device="cuda", generator=g) + 0.5 if norm else None
+    out = torch.full((rows, (heads + 2) * hd), 5, device="cuda", dtype=torch.int8)
+    scale = torch.full((rows, heads + 1), 5.0, device="cuda")
+    ops.rope_rows(V.of(x), pos, V.of(cos), sin, V.of(out).cols_of(hd, heads * hd), heads, hd,
+                  nw=nw, scale=V.of(scale), interleaved=inter)
+    p = pos.long()
+    host = lambda y: y.float().cpu().numpy()          # noqa: E731
+    y = norm_rope_f32(host(x).reshape(rows, heads, hd), host(nw)[0] if norm else None, host(cos[p]),
+                      host(sin[p]), inter)
+    q, sc = int8_f32(y)
+    got = out.cpu().numpy()
+    assert np.array_equal(got[:, hd:-hd], q.reshape(rows, -1))
+    assert (got[:, :hd] == 5).all() and (got[:, -hd:] == 5).all()
+    assert np.array_equal(scale.cpu().numpy()[:, :heads], sc) and (scale[:, heads] == 5.0).all()
+
+
 def test_rope_rows_in_place_and_bad_positions(ops, q3, request):
     request.node.keywords["status"] = True
     g = gen(3)
@@ -353,6 +380,9 @@ SHAPES = [
     (4, 2, 128, 32, [(64, 1000), (257, 257), (300, 777)]),
     (6, 2, 64, 32, [(200, 431), (45, 45), (2, 900)]),
     (3, 3, 128, 64, [(129, 640)]),
+    (2, 1, 64, 1, [(3, 40), (70, 300)]),
+    (2, 2, 128, 4096, [(1, 3000), (90, 400)]),
+    (30, 2, 64, 32, [(2, 500), (9, 9)]),
 ]
 
 
@@ -693,3 +723,36 @@ def test_many_sequences(ops, seqs):
     v = torch.cat(v)
     assert ((v - x.double()).abs() <= x.double().abs().amax(-1, keepdim=True) / 127 * 0.501).all()
     run_attention(ops, P, 2, "f16", "bf16")
+
+
+def test_ragged_arrays_that_do_not_fit(ops, q3, request):
+    """row0 that falls, or passes the rows: a status, the sequences that fit computed."""
+    request.node.keywords["status"] = True
+    P = Pool(ops, [(5, 40), (2, 300), (4, 50), (30, 60)], 2, 64, seed=2)
+    q, _, q64 = make_q(P, 2, "f16", 1)
+    want, tol = ref_attention(P, q64, 2, True, 0, 0.125)
+    o = torch.full((P.rows, 128), 7.0, device="cuda", dtype=torch.float16)
+    P.row0.copy_(torch.tensor([0, 5, 4, 11, 11 + 31], dtype=torch.int32))   # -1 rows; beyond q
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 4, 31, o,
+                              None, 2, 2, 64, True, 0, 0.125)
+    k = torch.randn(P.rows, 128, device="cuda")
+    assert q3._lib.lib().q3_device_status() == 1 << 5
+    check_rows(o[:4], None, want[:4], tol[:4], 2, 64, 4)   # sequence 0's rows but the shared one
+    assert (o[11:] == 7).all()
+    ops.paged_kv_append_batch(k, k, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 4, 2, 64)
+    torch.cuda.synchronize()
+    q3._lib.lib().q3_device_status()
+
+
+def test_raw_stream_argument(ops):
+    """A stream given by its handle, with a workspace from the caller's stream."""
+    P = Pool(ops, [(1, 9000)], 1, 128, seed=5)
+    s = torch.cuda.Stream()
+    q, _, q64 = make_q(P, 2, "f16", 2)
+    o = torch.empty(1, 256, device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 1, 1, o,
+                              None, 2, 1, 128, True, 0, 0.125, stream=s.cuda_stream)
+    s.synchronize()
+    want, tol = ref_attention(P, q64, 2, True, 0, 0.125)
+    check_rows(o, None, want, tol, 2, 128, 1)
