@@ -73,6 +73,10 @@ struct Call {
       refuse("operands on different devices: " + t.device().str() + " and cuda:" + std::to_string(dev));
     return t;
   }
+  // an empty tensor has no address: any aligned one, of which nothing is read
+  static void *address(const at::Tensor &t) {
+    return t.numel() ? t.data_ptr() : reinterpret_cast<void *>(256);
+  }
   uint32_t u32(int i) const {
     const unsigned long x = PyLong_AsUnsignedLong(args[i]);
     if (x == static_cast<unsigned long>(-1) && PyErr_Occurred()) throw PyError{};
@@ -94,6 +98,11 @@ struct Call {
     if (args[i] == Py_None) return nullptr;
     std::memset(&v, 0, sizeof v);
     if (!THPVariable_Check(args[i])) {
+      PyObject *owner = PyObject_GetAttrString(args[i], "owner");
+      if (!owner) throw PyError{};
+      const int at = THPVariable_Check(owner) ? THPVariable_Unpack(owner).get_device() : dev;
+      Py_DECREF(owner);
+      if (at != dev) refuse("operands on different devices");
       auto get = [&](const char *name) -> long long {
         PyObject *o = PyObject_GetAttrString(args[i], name);
         if (!o) throw PyError{};
@@ -127,7 +136,7 @@ struct Call {
     if (rb > INT32_MAX || rb < INT32_MIN || cb > INT32_MAX || cb < INT32_MIN || rows > UINT32_MAX ||
         cols > UINT32_MAX)
       refuse("a size or stride of a view is too large");
-    v.data = t.data_ptr();
+    v.data = address(t);
     v.row_bytes = static_cast<int32_t>(rb);
     v.col_bytes = static_cast<int32_t>(cb);
     v.rows = static_cast<uint32_t>(rows);
@@ -144,7 +153,7 @@ struct Call {
     if (!ok || !t.is_contiguous() || t.numel() < n)
       refuse(std::string(what) + ": a contiguous array of at least " + std::to_string(n) + type +
              " is needed");
-    return t.data_ptr();
+    return address(t);
   }
   q3_paged_kv pool(int i) const {
     Py_buffer b;

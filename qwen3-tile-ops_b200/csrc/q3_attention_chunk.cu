@@ -579,7 +579,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   int pb0;
   const int pn = seq_units(p, q, pb0);
   const int m = blockIdx.z;                        // packed row
-  if (pn == 0 || m >= q.n * p.group) return;       // refused, or the other kernel's
+  // (also a CTA with nothing to join waits: when this grid ends, the results are there)
+  if (pn == 0 || m >= q.n * p.group) {             // refused, or the other kernel's
+    pdl_wait();
+    return;
+  }
   if (wid == 0) {   // the slices that have units of the sequence
     uint32_t before;
     const Slices cut(count_units(p, s, lane, &err, before), most);
@@ -590,10 +594,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   }
   __syncthreads();
   const uint32_t w0 = range[0], w1 = range[1];
+  pdl_wait();
   if (w0 == w1) return;                            // stored whole
   const long r = q.first + m / p.group;
   const int h = kvh * p.group + m % p.group;
-  pdl_wait();
   float mm = kNegInf, l = 0.0f, x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;

@@ -61,8 +61,9 @@ struct TcSmem {
   int seq, tile;                                   // this CTA's, from the lookup
 };
 
-// Bounded wait for the phase with parity par (about a second, or until another thread gave up)
-__device__ __forceinline__ void wait_bar(unsigned long long *b, uint32_t par, int *abort) {
+// Bounded wait for the phase with parity par (about a second, or until another thread gave up); false:
+// it has not come, and what it stands for must not be used as an address
+__device__ __forceinline__ bool wait_bar(unsigned long long *b, uint32_t par, int *abort) {
   const uint32_t at = su32(b);
   uint64_t t0 = 0;
   for (uint32_t it = 1;; ++it) {
@@ -73,9 +74,9 @@ __device__ __forceinline__ void wait_bar(unsigned long long *b, uint32_t par, in
         : "=r"(ok)
         : "r"(at), "r"(par)
         : "memory");
-    if (ok) return;
+    if (ok) return true;
     if ((it & 63) == 0) {
-      if (*reinterpret_cast<volatile int *>(abort)) return;
+      if (*reinterpret_cast<volatile int *>(abort)) return false;
       const uint64_t t = gtime();
       if (t0 == 0) t0 = t;
       else if (t - t0 > 1000000000ull) break;
@@ -83,6 +84,7 @@ __device__ __forceinline__ void wait_bar(unsigned long long *b, uint32_t par, in
   }
   atomicOr(&g_chunk_tc_error, kErrWait);
   *reinterpret_cast<volatile int *>(abort) = 1;
+  return false;
 }
 
 // kind::f16 with float32 sums: f16 x f16, M = 128, N = n; b_mn: B is MN-major
@@ -652,12 +654,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     auto request = [&](int item) {
       if (item < items) {
         const int j = item >> 1, in = j % INFO;
-        wait_bar(&sm.place_full[in], (j / INFO) & 1, &sm.abort);
+        const bool known = wait_bar(&sm.place_full[in], (j / INFO) & 1, &sm.abort);
         const char *from = ((item & 1) ? p.v : p.k) + kcol;
         const uint32_t dst = su32(raw + (item % RAW) * (TC_KEYS * HD / 16));
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
-          const long long at = sm.place[in][row0 + i * CR];
+          const long long at = known ? sm.place[in][row0 + i * CR] : -1;
           cp16(dst + i * LOADERS * 512, at >= 0 ? from + at : p.k, at >= 0);
         }
         __syncwarp();

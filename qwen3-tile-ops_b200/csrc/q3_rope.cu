@@ -536,8 +536,9 @@ int check_pool(const q3_paged_kv *kv, uint32_t kv_heads, uint32_t head_dim, uint
   if (!kv || !kv->k || !kv->v || !kv->ks || !kv->vs) return Q3_ERR_NULL;
   if (kv_heads == 0 || kv_heads > 4096 || num_pages == 0 || num_pages > 65536 || max_pages == 0)
     return Q3_ERR_SHAPE;
+  // (positions rounded up to a tile of keys stay below 2^31)
   if (kv->page_tokens == 0 || kv->page_tokens > 32768 ||
-      (uint64_t)max_pages * kv->page_tokens > 0x7fffffffu)
+      (uint64_t)max_pages * kv->page_tokens > 0x7fffff00u)
     return Q3_ERR_SHAPE;
   if (kv->row_bytes < kv_heads * head_dim || kv->scale_row_bytes < kv_heads * 4 ||
       (uint64_t)kv->page_tokens * kv->row_bytes > kv->page_bytes ||

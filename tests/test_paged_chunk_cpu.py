@@ -189,6 +189,15 @@ def test_attention_refuses(L):
     assert attn_call(L, **big, ws=0x1008, ws_bytes=n) == ALIGN
 
 
+def test_longest_tables(L):
+    """Positions rounded up to a tile of keys stay below 2^31."""
+    long = pool(L, page_tokens=32767, page_bytes=32767 * 256, scale_page_bytes=32767 * 8)
+    assert append_call(L, kv=long, max_pages=65537) == OK
+    assert append_call(L, kv=long, max_pages=65538) == SHAPE   # 2^31 - 2 tokens
+    assert attn_call(L, kv=long, max_pages=65537) == OK
+    assert attn_call(L, kv=long, max_pages=65538) == SHAPE
+
+
 def test_attention_workspace_bytes(L):
     f = L.lib().q3_attention_chunk_workspace_bytes
     assert f(0, 1, 1, 4096, 4, 2, 128) == 0 and f(4, 0, 1, 4096, 4, 2, 128) == 0

@@ -756,3 +756,40 @@ def test_raw_stream_argument(ops):
     s.synchronize()
     want, tol = ref_attention(P, q64, 2, True, 0, 0.125)
     check_rows(o, None, want, tol, 2, 128, 1)
+
+
+def test_results_complete_when_the_call_ends(ops):
+    """Short sequences in long tables: none is cut, so the join has nothing to do, and what follows
+    on the stream still sees every result."""
+    lens = [(1 + s % 3, 3 + 7 * s % 90) for s in range(300)]
+    heads, hd = 4, 64
+    P = Pool(ops, lens, 2, hd, seed=11, spare=20)
+    q, _, q64 = make_q(P, heads, "f16", 3)
+    seen = []
+    for _ in range(8):
+        o = torch.full((P.rows, heads * hd), 7.0, device="cuda", dtype=torch.float16)
+        ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len,
+                                  len(lens), P.max_rows, o, None, heads, 2, hd, True, 0, 0.125)
+        seen.append(o.clone())
+    want, tol = ref_attention(P, q64, heads, True, 0, 0.125)
+    check_rows(seen[0], None, want, tol, heads, hd, P.rows)
+    assert all(torch.equal(x, seen[0]) for x in seen)
+
+
+def test_nothing_to_do(ops):
+    """No rows, and no sequences: a call that does nothing."""
+    P = Pool(ops, [(0, 5), (0, 0)], 2, 64)
+    x = torch.empty(0, 128, device="cuda", dtype=torch.float16)
+    cos, sin = tables_f32(8, 64)
+    ops.rope_tables(cos[:0], sin[:0], 1e6)
+    ops.rope_rows(x, P.row0[:0], cos, sin, x, 2, 64)
+    before = P.k.clone()
+    for n in (2, 0):
+        ops.paged_kv_append_batch(x, x, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len[:n], n, 2,
+                                  64, cos=cos, sin=sin)
+        ops.attention_chunk_batch(x, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len[:n], n,
+                                  1, x, None, 2, 2, 64, True, 0, 0.125)
+    o = torch.full((3, 128), 7.0, device="cuda", dtype=torch.float16)
+    ops.attention_chunk_batch(o.clone(), None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2,
+                              1, o, None, 2, 2, 64, True, 0, 0.125)   # rows that belong to nobody
+    assert (o == 7).all() and torch.equal(P.k, before)
