@@ -46,25 +46,37 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 // ---------------------------------------------------------------------------
-// Few rows: sequences with at most 8 NT packed rows (packed row m is head m %
-// group of new row m / group of the sequence).  A unit of work is one 32-key block
-// of a sequence; the units of the whole batch, in order, are cut into equal slices,
+// Few rows: sequences with at most few_rows packed rows (packed row m is head m %
+// group of new row m / group of the sequence), in row tiles of 8 NT.  A unit of work is
+// one 32-key block for one row tile; the units of the whole batch, in order, are cut into equal slices,
 // and a warp takes one KV head of a slice, so ragged lengths and any number of
 // sequences fill one resident wave evenly, and the heads of a token, which lie side
 // by side in memory, are read at about the same time.  A warp works alone: it keeps
-// the running maximum and sums of its run of a sequence and stores the result when
-// it has the whole sequence, else a part (at most two a warp: its first and its last
-// sequence) that k_attn_join joins.
+// the running maximum and sums of its run of a row tile and stores the result when
+// it has all of its blocks, else a part (at most two a warp: of its first and its last
+// row tile) that k_attn_join joins.
 //
 // Keys are the M side of the products (S^T = K8 q^T, o^T = V8^T p^T), so a decode
 // step with a group of 2 wastes 6 of 8 columns instead of 14 of 16 rows.  A warp
 // keeps STAGES blocks in shared memory or on their way there (cp.async); a fragment
 // is built from 16-byte reads of codes, since the contraction over d and the rows of
-// o^T may be permuted freely.  Reading the cache once is the bound.
+// o^T may be permuted freely.
+//
+// Reading the cache once is the bound: 64 sequences of 2048 tokens (277 MB) 54 us, 5.1 TB/s, and
+// 5.9 TB/s between the start and the end; the loads alone take as long.  Units that
+// take one KV head each, dealt evenly, took 64 us, and 71 against 56 for 2 x 65011 tokens.
+// Two stages of 32 keys: three leave fewer warps an SM (58 us); L2 prefetch of later pages 61 us.
 // ---------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int KB = 32;                             // keys of a block
-constexpr int MIN_UNITS = 4;                       // least run of a warp
+// Least units of a slice.  Alone, short slices spread a small batch (one sequence of 2000 tokens 8.5 us;
+// slices of 4 10.2, of 1 8.5 with more parts).  Beside the many-row kernel this one has the SMs that
+// are left, and many short slices queue there (16 ragged sequences 64 us; of 2 72, of 32 79).
+constexpr int ALONE_UNITS = 2, BESIDE_UNITS = 8;
+// Most packed rows of a sequence of this kernel, in tiles that read the keys again.  Alone: 8 sequences
+// of 32 packed rows over 4000 tokens 44 us, in the many-row kernel 54; 64 over 2000 161 and 187; with 48
+// rows 242 and 187.  Beside: 32 makes the ragged batch above 2 us slower.
+constexpr int ALONE_ROWS = 32, BESIDE_ROWS = 16;
 constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that is never cut
 
 template <int HD>
@@ -74,8 +86,12 @@ struct FewStage {
   float ks[KB], vs[KB];
 };
 
-// Units of sequence s (0: not this kernel's) and its first block
-__device__ __forceinline__ int seq_units(const Args &p, const Seq &s, int &b0) {
+// Row tiles of sequence s, of 2^row_shift packed rows
+__device__ __forceinline__ int row_tiles(const Args &p, const Seq &s) {
+  return (s.n * p.group + (1 << p.row_shift) - 1) >> p.row_shift;
+}
+// Blocks of sequence s (0: not this kernel's) and the first of them; a tile's units are its blocks
+__device__ __forceinline__ int seq_blocks(const Args &p, const Seq &s, int &b0) {
   b0 = 0;
   if (!s.ok || s.n * p.group > p.few_rows) return 0;
   int lo, hi;
@@ -85,9 +101,11 @@ __device__ __forceinline__ int seq_units(const Args &p, const Seq &s, int &b0) {
 }
 __device__ __forceinline__ int units_of(const Args &p, int s, unsigned *err) {
   int b0;
-  return seq_units(p, load_seq(p, s, err), b0);
+  const Seq q = load_seq(p, s, err);
+  const int n = seq_blocks(p, q, b0);
+  return n ? n * row_tiles(p, q) : 0;
 }
-// All units, and those of the sequences before s0 (whole warp; the host bounds them below 2^31)
+// All units, and those of the sequences before s0 (whole warp; the host bounds them by 2^31)
 __device__ __forceinline__ uint32_t count_units(const Args &p, int s0, int lane, unsigned *err,
                                                 uint32_t &before) {
   uint32_t x = 0, y = 0;
@@ -102,8 +120,8 @@ __device__ __forceinline__ uint32_t count_units(const Args &p, int s0, int lane,
 // The slices of `total` units: the first `more` have each + 1 of them
 struct Slices {
   uint32_t n, each, more;
-  __device__ __forceinline__ Slices(uint32_t total, uint32_t most) {
-    n = (total + MIN_UNITS - 1) / MIN_UNITS;
+  __device__ __forceinline__ Slices(uint32_t total, uint32_t most, uint32_t least) {
+    n = (total + least - 1) / least;
     n = n < most ? n : most;
     n = n ? n : 1;
     each = total / n;
@@ -184,7 +202,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
     for (int x = 32 + lane; x - lane < p.n_seqs; x += 32)
       total += __reduce_add_sync(0xffffffffu, x < p.n_seqs ? units_of(p, x, &err) : 0);
     if (w == 0 && err) atomicOr(&g_chunk_error, err);
-    const Slices cut(total, gridDim.x * WARPS / p.kv_heads);
+    const Slices cut(total, gridDim.x * WARPS / p.kv_heads, p.min_units);
     if (total && slice < cut.n) {
       u = cut.first(slice);
       u1 = cut.first(slice + 1);
@@ -196,11 +214,18 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
     while (u < u1 && s < p.n_seqs) {
       // the sequence of unit u, its blocks [pb0, pb0 + pn), and this warp's run [b, be) of them
       const Seq q = load_seq(p, s, &err);
-      int pb0, pn = seq_units(p, q, pb0);
+      int pb0, pn = seq_blocks(p, q, pb0);
+      int off = static_cast<int>(u - static_cast<uint32_t>(before));
+      m0 = p.whole ? m0 : 0;
+      if (!p.whole && off >= pn && pn) {           // a row tile behind the first
+        m0 = off / pn;
+        off -= m0 * pn;
+        m0 *= 8 * NT;
+      }
       const int packed = min(8 * NT, q.n * p.group - m0);
       if (pn == 0 || packed <= 0) {
         if (p.whole) break;
-        ++s;
+        ++s;                                       // (a sequence without units)
         continue;
       }
       const int pmin = q.pos0 + m0 / p.group;      // position of the first of the rows
@@ -211,7 +236,6 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
         pn = (hi + KB - 1) / KB - pb0;
         u1 = pn;
       }
-      const int off = static_cast<int>(u - static_cast<uint32_t>(before));
       const int b = pb0 + off;
       const int run = static_cast<int>(u1 - u) < pn - off ? static_cast<int>(u1 - u) : pn - off;
       const int be = b + run;
@@ -543,7 +567,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
             const int mm = m0 + min(m, packed - 1);
             store_part8<HD / 8>(p, q.first + mm / p.group, kvh * p.group + mm % p.group, g, ok, y);
           } else if (ok) {
-            const long at = slot * p.part_rows + m;
+            const long at = slot * (8 * NT) + m;
             Elems<float, HD / 8> e;
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) e.e[i] = y[i];
@@ -555,8 +579,10 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
           }
         }
       u += run;
-      before += pn;
-      ++s;
+      if (m0 + 8 * NT >= q.n * p.group || p.whole) {   // on to the next sequence
+        before += static_cast<long>(pn) * row_tiles(p, q);
+        ++s;
+      }
     }
   }
   // as a dependent of the many-row kernel it began when all CTAs of that were running; what comes
@@ -565,7 +591,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
 }
 
 // The parts of one packed row of a (sequence, KV head) pair joined by a CTA: its warps take them in
-// turn, JOIN_AT loads at once.
+// turn, JOIN_AT loads at once.  Bound by latency: 111 parts a sequence at 2 x 65011 tokens; it looks
+// its parts up while the kernel before it still works, and adds about 2 us.
 constexpr int JOIN_WARPS = 8, JOIN_AT = 4;
 template <int HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uint32_t most) {
@@ -577,7 +604,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   unsigned err = 0;
   const Seq q = load_seq(p, s, &err);
   int pb0;
-  const int pn = seq_units(p, q, pb0);
+  const int pn = seq_blocks(p, q, pb0);
   const int m = blockIdx.z;                        // packed row
   // (also a CTA with nothing to join waits: when this grid ends, the results are there)
   if (pn == 0 || m >= q.n * p.group) {             // refused, or the other kernel's
@@ -586,8 +613,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   }
   if (wid == 0) {   // the slices that have units of the sequence
     uint32_t before;
-    const Slices cut(count_units(p, s, lane, &err, before), most);
+    const Slices cut(count_units(p, s, lane, &err, before), most, p.min_units);
     if (lane == 0) {
+      before += (m >> p.row_shift) * pn;
       range[0] = cut.of(before);
       range[1] = cut.of(before + pn - 1);
     }
@@ -612,8 +640,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
 #pragma unroll
       for (int i = 0; i < N; ++i) e[k].e[i] = 0.0f;
       if (wk <= w1) {   // the warp's part: of its last sequence if this one begins with it
-        const long at = (2 * (static_cast<long>(wk) * p.kv_heads + kvh) + (wk == w0 ? 1 : 0)) *
-                            p.part_rows + m;
+        const long at = ((2 * (static_cast<long>(wk) * p.kv_heads + kvh) + (wk == w0 ? 1 : 0))
+                         << p.row_shift) + (m & ((1 << p.row_shift) - 1));
         pm[k] = p.part_ml[at * 2];
         pl[k] = p.part_ml[at * 2 + 1];
         e[k].load(p.part_o + at * HD + lane * N);
@@ -654,6 +682,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   store_out<N>(p, r, h, lane, x);
 }
 
+// The parts of k_attn_tc's key ranges: a warp a row and head.  Bound by latency; a few MB at most, since
+// keys are split only while the tiles cannot fill the card.
 template <int HD>
 __global__ void k_join_tiles(const Args p) {
   constexpr int N = HD / 32;
@@ -691,7 +721,7 @@ __global__ void k_join_tiles(const Args p) {
 // How a call is cut.  Sequences with at most few_rows packed rows go to k_attn_few (nt tiles of 8),
 // the others to the tensor-core kernel of many rows.
 struct Plan {
-  int nt, few_rows;
+  int nt, few_rows, min_units;
   long few_ctas, few_tiles;                        // few_ctas 0: no such sequence can be there
   bool whole;                                      // their keys are not cut
   long tiles;                                      // tiles 0: likewise
@@ -704,14 +734,19 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
   const long group = heads / kv_heads;
   const long packed = static_cast<long>(max_rows < rows ? max_rows : rows) * group;
   const int sms = q3h::sm_count();
-  c.few_rows = 16;
-  c.nt = packed > 8 && group <= c.few_rows ? 2 : 1;
-  if (group <= c.few_rows) {
-    // Up to 256 keys a warp takes a whole sequence: its 8 blocks cost what 4 of them and the join do,
-    // and less than the 12 us that a CTA of many rows takes to start and end
-    c.whole = max_kv <= WHOLE_KEYS;
-    const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB);
-    const long slices = (units + MIN_UNITS - 1) / MIN_UNITS;
+  const bool mixed = packed > ALONE_ROWS;
+  c.few_rows = mixed ? BESIDE_ROWS : ALONE_ROWS;
+  c.min_units = mixed ? BESIDE_UNITS : ALONE_UNITS;
+  c.nt = packed > 8 ? 2 : 1;
+  if (group <= 16) {
+    // Up to 256 keys a warp takes a whole sequence if that gives each SM a warp (64 sequences of 220
+    // keys 12.5 us, cut 17.4; 8 of them 11.4 and 10.1), or to spare the many-row kernel (4 x 60 rows 15 us
+    // against 17)
+    c.whole = max_kv <= WHOLE_KEYS && (packed > 16 || static_cast<long>(n_seqs) * kv_heads > sms);
+    const long most_rows = packed < c.few_rows ? packed : c.few_rows;
+    const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB) *
+                       ((most_rows + 8 * c.nt - 1) / (8 * c.nt));
+    const long slices = (units + c.min_units - 1) / c.min_units;
     const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2), least = (kv_heads + WARPS - 1) / WARPS;
     long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
     ctas = ctas < most ? ctas : most;
@@ -731,7 +766,8 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
     c.tiles = all < each ? all : each;
     const long ctas = c.tiles * kv_heads;
     long z = ctas >= sms ? 1 : sms / ctas;         // one CTA on each SM
-    const long most = (max_kv + 4 * TC_KEYS - 1) / (4 * TC_KEYS);
+    // (parts of at least two key tiles: 200 rows over 1000 tokens 24.8 us; of four 27.2)
+    const long most = (max_kv + 2 * TC_KEYS - 1) / (2 * TC_KEYS);
     z = z < most ? z : most;
     c.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   }
@@ -785,7 +821,7 @@ static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t 
   Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
   Q3_TRY(launch_ex(beside, chunk::k_attn_few<HD, NT>, dim3(ctas), dim3(chunk::WARPS * 32), smem, s, p));
   const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
-  const unsigned z = static_cast<unsigned>(packed < p.part_rows ? packed : p.part_rows);
+  const unsigned z = static_cast<unsigned>(packed < p.few_rows ? packed : p.few_rows);
   if (p.whole) return Q3_OK;
   return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, z),
                    dim3(chunk::JOIN_WARPS * 32), 0, s, p,
@@ -890,8 +926,9 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     st = head_dim == 128 ? launch_many<128>(t, s) : launch_many<64>(t, s);
   }
   if (st == Q3_OK && c.few_ctas) {
-    p.part_rows = 8 * c.nt;
+    p.row_shift = c.nt == 1 ? 3 : 4;
     p.whole = c.whole;
+    p.min_units = c.min_units;
     p.tiles = static_cast<int>(c.few_tiles);
     p.part_o = ws;
     p.part_ml = ws + c.few_slots * head_dim;

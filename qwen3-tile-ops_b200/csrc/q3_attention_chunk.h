@@ -21,9 +21,10 @@ struct Args {
   int causal, window;
   float scale_log2;              // qk_scale * log2(e)
   int splits;                    // parts of the key range (1: results go to o)
-  int tiles;                     // query tiles a sequence may have
+  int tiles;                     // many rows: tiles of the batch; few rows, whole: tiles of a sequence
   int few_rows;                  // packed rows of a sequence that k_attn_few takes
-  int part_rows;                 // rows of one of its parts
+  int min_units;                 // least units of a slice
+  int row_shift;                 // log2 of the packed rows of its row tiles, and of a part
   int whole;                     // it takes a sequence's keys as a whole
   int page_shift;                // log2 of page_tokens, or -1
   int whole_blocks;              // a 32-key block lies in one page

