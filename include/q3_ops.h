@@ -363,7 +363,8 @@ int q3_paged_kv_append_batch(const q3_view *k, const q3_view *v, const q3_view *
  * scale per head, as q3_quant_rows_heads), f16 or bf16.  heads is a multiple
  * of kv_heads, at most 16 times it.  max_rows: no sequence has more new rows;
  * one that has sets status bit 5 and is skipped.  The workspace of
- * q3_attention_chunk_workspace_bytes (max_kv = max_pages * page_tokens) is written
+ * q3_attention_chunk_workspace_bytes (the call's own sizes: the bytes need not
+ * grow with each; max_kv = max_pages * page_tokens, at most 2^31 - 256) is written
  * by the call; calls that may overlap on the GPU need one each. */
 size_t q3_attention_chunk_workspace_bytes(uint32_t rows, uint32_t n_seqs, uint32_t max_rows,
                                           uint32_t max_kv, uint32_t heads, uint32_t kv_heads,
