@@ -47,17 +47,19 @@ __host__ __device__ constexpr double turn_power(int n) {
 }
 
 __global__ void k_rope_tables(const __grid_constant__ TableArgs p) {
+  pdl_trigger();
   __shared__ uint64_t turn[MAX_PAIRS];
   for (int i = threadIdx.x; i < p.half; i += blockDim.x) turn[i] = p.turn[i];
   __syncthreads();
   const int per = blockDim.x / p.half;             // positions a block does at once
   const int i = threadIdx.x % p.half, r0 = threadIdx.x / p.half;
-  if (r0 >= per) return;
+  if (r0 >= per) return;   // (others of the block wait below)
   const long step = static_cast<long>(gridDim.x) * per;
   long r = static_cast<long>(blockIdx.x) * per + r0;
   uint64_t t = turn[i] * (static_cast<uint64_t>(p.pos0) + static_cast<uint64_t>(r));
   const uint64_t dt = turn[i] * static_cast<uint64_t>(step);
   char *cp = p.cos + r * p.cos_rb + i * 4, *sp = p.sin + r * p.sin_rb + i * 4;
+  pdl_wait();
 #pragma unroll 4
   for (; r < p.rows; r += step) {
     const uint32_t hi = static_cast<uint32_t>(t >> 32);
@@ -230,12 +232,14 @@ struct RowArgs {
 template <typename T, int N, int GL>
 __global__ void k_rope_rows(RowArgs p) {
   constexpr int HD = GL * N, HW = 32 / GL;         // heads a warp holds at once
+  pdl_trigger();
   const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
   const int chunks = (p.heads + U * HW - 1) / (U * HW);
   const long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long r = unit / chunks;
   if (r >= p.rows) return;
   const int h0 = static_cast<int>(unit - r * chunks) * (U * HW);
+  pdl_wait();
   Elems<T, N> e[U];
   const char *xp = p.x + r * p.x_rb + (static_cast<long>(h0 + hl) * HD + g * N) * sizeof(T);
 #pragma unroll
@@ -298,6 +302,7 @@ struct AppendArgs {
 template <typename T, int N, int GL>
 __global__ void k_kv_append(AppendArgs p) {
   constexpr int HD = GL * N, HW = 32 / GL;
+  pdl_trigger();
   const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
   const int chunks = (p.kv_heads + U * HW - 1) / (U * HW);
   long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -306,6 +311,7 @@ __global__ void k_kv_append(AppendArgs p) {
   unit -= r * (2 * chunks);
   const bool is_v = unit >= chunks;
   const int h0 = static_cast<int>(is_v ? unit - chunks : unit) * (U * HW);
+  pdl_wait();
   Elems<T, N> e[U];
   const char *xp = (is_v ? p.v + r * p.v_rb : p.k + r * p.k_rb) +
                    (static_cast<long>(h0 + hl) * HD + g * N) * sizeof(T);
@@ -462,8 +468,8 @@ extern "C" int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_
   p.pos0 = pos0;
   const int threads = 256, per = threads / (int)half;
   const long blocks = ((long)p.rows + per - 1) / per, most = 4L * sm_count();
-  k_rope_tables<<<(unsigned)(blocks < most ? blocks : most), threads, 0, (cudaStream_t)stream>>>(p);
-  return launch_status();
+  return launch_ex(true, k_rope_tables, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0,
+                   (cudaStream_t)stream, p);
 }
 
 template <typename T>
@@ -472,10 +478,10 @@ static int launch_rows(const RowArgs &p, uint32_t hd, cudaStream_t s) {
   const int per = U * (hd >= 32 * N ? 1 : 32 * N / static_cast<int>(hd));   // heads of a warp
   const long warps = static_cast<long>(p.rows) * ((p.heads + per - 1) / per);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-  if (hd == 64) k_rope_rows<T, N, 64 / N><<<blocks, 128, 0, s>>>(p);
-  else if (hd == 128) k_rope_rows<T, N, 128 / N><<<blocks, 128, 0, s>>>(p);
-  else k_rope_rows<T, 8, 32><<<blocks, 128, 0, s>>>(p);
-  return launch_status();
+  const dim3 grid(blocks), block(128);
+  return hd == 64    ? launch_ex(true, k_rope_rows<T, N, 64 / N>, grid, block, 0, s, p)
+         : hd == 128 ? launch_ex(true, k_rope_rows<T, N, 128 / N>, grid, block, 0, s, p)
+                     : launch_ex(true, k_rope_rows<T, 8, 32>, grid, block, 0, s, p);
 }
 
 extern "C" int q3_rope_rows(const q3_view *x, const q3_view *nw, const int32_t *pos,
@@ -525,10 +531,10 @@ static int launch_append(const AppendArgs &p, uint32_t hd, cudaStream_t s) {
   const int per = U * (hd >= 32 * N ? 1 : 32 * N / static_cast<int>(hd));   // heads of a warp
   const long warps = static_cast<long>(p.rows) * 2 * ((p.kv_heads + per - 1) / per);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-  if (hd == 64) k_kv_append<T, N, 64 / N><<<blocks, 128, 0, s>>>(p);
-  else if (hd == 128) k_kv_append<T, N, 128 / N><<<blocks, 128, 0, s>>>(p);
-  else k_kv_append<T, 8, 32><<<blocks, 128, 0, s>>>(p);
-  return launch_status();
+  const dim3 grid(blocks), block(128);
+  return hd == 64    ? launch_ex(true, k_kv_append<T, N, 64 / N>, grid, block, 0, s, p)
+         : hd == 128 ? launch_ex(true, k_kv_append<T, N, 128 / N>, grid, block, 0, s, p)
+                     : launch_ex(true, k_kv_append<T, 8, 32>, grid, block, 0, s, p);
 }
 
 namespace q3 {
