@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "q3_common.cuh"
 
 namespace q3 {
@@ -62,33 +64,54 @@ struct Elems {
     for (int i = 0; i < CH; ++i) reinterpret_cast<V *>(p)[i] = v[i];
   }
 };
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
+// float32 of the elements; 16-bit ones two at a time, as a word holds them
+template <typename T, int N>
+__device__ __forceinline__ void to_f32(const Elems<T, N> &e, float (&x)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = e.e[i];
+  } else {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(e.v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
+        x[2 * i] = y.x, x[2 * i + 1] = y.y;
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Elems<T, N> from_f32(const float (&x)[N]) {
+  Elems<T, N> e;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) e.e[i] = x[i];
+  } else {
+    uint32_t *w = reinterpret_cast<uint32_t *>(e.v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 y = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&y);
+      } else {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&y);
+      }
+    }
+  }
+  return e;
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_row(const float (&x)[N], void *p) {
-  Elems<T, N> e;
-#pragma unroll
-  for (int i = 0; i < N; ++i) e.e[i] = from_f32<T>(x[i]);
-  e.store(p);
+  from_f32<T>(x).store(p);
 }
-
 template <typename T, int N>
 __device__ __forceinline__ void store_row_stream(const float (&x)[N], void *p) {
-  Elems<T, N> e;
-#pragma unroll
-  for (int i = 0; i < N; ++i) e.e[i] = from_f32<T>(x[i]);
-  e.store_stream(p);
+  from_f32<T>(x).store_stream(p);
 }
 
 // Sequence of row r (whole warp): the last s with row0[s] <= r, or -1 when r

@@ -105,8 +105,9 @@ __global__ void k_rope_tables(const __grid_constant__ TableArgs p) {
 // their order are those of the norm-rope-quant epilogue
 // (tools/ref_qwen3.py:161-191), so the codes are the same bits.
 // ---------------------------------------------------------------------------
+constexpr int U = 4;                               // heads a lane holds at once
 template <int N, int GL>
-__device__ __forceinline__ void head_norm(float (&x)[N], const float (&w)[N], float inv_hd) {
+__device__ __forceinline__ float head_mean(const float (&x)[N], float inv_hd) {
   // squares by adjacent pairs within 32-column blocks of 32/N lanes ...
   float s[N];
 #pragma unroll
@@ -122,13 +123,31 @@ __device__ __forceinline__ void head_norm(float (&x)[N], const float (&w)[N], fl
 #pragma unroll
   for (int b = 0; b < GL * N / 32; ++b)
     ss = __fadd_rn(ss, __shfl_sync(0xffffffffu, s[0], b * (32 / N), GL));
-  const float r = rsqrt_ref(__fadd_rn(__fmul_rn(ss, inv_hd), kEps));
+  return __fadd_rn(__fmul_rn(ss, inv_hd), kEps);
+}
+
+template <int N, int GL>
+__device__ __forceinline__ void head_scale(float (&x)[N], const float (&w)[N], float r) {
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
 }
+// the roots of U heads at once: that of head u in the lanes with g % U == u
+template <typename T, int N, int GL>
+__device__ __forceinline__ float head_rsqrt(const Elems<T, N> (&e)[U], float inv_hd, int g) {
+  float m = 1.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float x[N];
+    to_f32(e[u], x);
+    const float y = head_mean<N, GL>(x, inv_hd);
+    m = (g % U) == u ? y : m;
+  }
+  return rsqrt_ref(m);
+}
 
-// c, s: cos and sin of this lane's columns (half layout: of column mod half;
-// interleaved: c[i], s[i] for pair i of the lane in i < N/2)
+// c, s: cos and sin of this lane's columns (half layout: of column mod half, s negated in the lower
+// half, so that x c + y s is both x c - y s and y s + x c, with the same rounding; interleaved: c[i],
+// s[i] for pair i of the lane in i < N/2)
 template <int N, int GL>
 __device__ __forceinline__ void head_rotate(float (&x)[N], const float (&c)[N], const float (&s)[N],
                                             int half, bool inter, int g) {
@@ -144,14 +163,13 @@ __device__ __forceinline__ void head_rotate(float (&x)[N], const float (&c)[N], 
     return;
   }
   const int hl = half / N;                        // lanes of half a rotation
-  const bool lo = g < hl, in = g < 2 * hl;
-  const int other = in ? (lo ? g + hl : g - hl) : g;
+  const bool in = half * 2 == GL * N || g < 2 * hl;   // (the first for the compiler: often all columns)
+  const int other = in ? (g < hl ? g + hl : g - hl) : g;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float y = __shfl_sync(0xffffffffu, x[i], other, GL);
-    const float l = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y, s[i]));
-    const float h = __fadd_rn(__fmul_rn(y, s[i]), __fmul_rn(x[i], c[i]));
-    x[i] = in ? (lo ? l : h) : x[i];
+    const float z = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y, s[i]));
+    x[i] = in ? z : x[i];
   }
 }
 
@@ -185,7 +203,7 @@ __device__ __forceinline__ void load_turn(const Turn &t, long pos, int g, float 
     a.load(cp + at);
     b.load(sp + at);
 #pragma unroll
-    for (int i = 0; i < N; ++i) c[i] = a.e[i], s[i] = b.e[i];
+    for (int i = 0; i < N; ++i) c[i] = a.e[i], s[i] = g * N < t.half ? -b.e[i] : b.e[i];
   }
 }
 
@@ -215,9 +233,12 @@ __device__ __forceinline__ float head_int8(const float (&x)[N], void *codes, boo
 // rotation of rows.  A warp takes U times its 32 / GL heads of a row: U 16-byte loads a
 // lane in flight, one read of the row's cos and sin for them.  Loads and stores
 // stream past the caches (8192 rows of 16 heads: 28.2 us against 29.0; 5003
-// bf16 rows of 40 heads 25.8 against 28.5).
+// bf16 rows of 40 heads 25.8 against 28.5).  Bound by HBM and, with the norm, nearly by issue
+// slots: pairs of 16-bit elements converted at once, one multiply-add form for both halves
+// and one root for U heads brought 24.3 and 20.7 us (5.7 and 5.0 TB/s), 8192 bf16 rows of 32 heads
+// with norm 42.7 -> 33.3.  Registers are held to what 8 CTAs an SM leave (9 for f32; 7 and 5 for
+// heads in a whole warp): without the limit 23 us, at 10 CTAs 39 for the bf16 rows with norm.
 // ---------------------------------------------------------------------------
-constexpr int U = 4;
 struct RowArgs {
   const char *x;
   char *out, *scale;
@@ -230,7 +251,7 @@ struct RowArgs {
 };
 
 template <typename T, int N, int GL>
-__global__ void k_rope_rows(RowArgs p) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? (GL == 32 ? 7 : 8) : N == 8 ? 5 : 9) k_rope_rows(RowArgs p) {
   constexpr int HD = GL * N, HW = 32 / GL;         // heads a warp holds at once
   pdl_trigger();
   const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
@@ -257,15 +278,16 @@ __global__ void k_rope_rows(RowArgs p) {
     return;
   }
   load_turn<N>(p.t, pos, g, c, s);
+  float rs = 0.0f;
+  if (p.nw) rs = head_rsqrt<T, N, GL>(e, p.inv_hd, g);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (h0 + u * HW >= p.heads) break;
     const int h = h0 + u * HW + hl;
     const bool ok = h < p.heads;
     float x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f32(e[u].e[i]);
-    if (p.nw) head_norm<N, GL>(x, w, p.inv_hd);
+    to_f32(e[u], x);
+    if (p.nw) head_scale<N, GL>(x, w, __shfl_sync(0xffffffffu, rs, u, GL));
     head_rotate<N, GL>(x, c, s, p.t.half, p.t.inter, g);
     const long col = static_cast<long>(h) * HD + g * N;
     char *o = p.out + r * p.out_rb;
@@ -344,6 +366,8 @@ __global__ void k_kv_append(AppendArgs p) {
     return;
   }
   if (turn) load_turn<N>(p.t, pos, g, c, s);
+  float rs = 0.0f;
+  if (norm) rs = head_rsqrt<T, N, GL>(e, p.inv_hd, g);
   const uint32_t slot = static_cast<uint32_t>(pos - lp * p.page_tokens);
   char *codes = (is_v ? p.pv : p.pk) + static_cast<size_t>(page) * p.page_bytes +
                 static_cast<size_t>(slot) * p.row_bytes;
@@ -356,9 +380,8 @@ __global__ void k_kv_append(AppendArgs p) {
     const int h = h0 + u * HW + hl;
     const bool ok = h < p.kv_heads;
     float x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f32(e[u].e[i]);
-    if (norm) head_norm<N, GL>(x, w, p.inv_hd);
+    to_f32(e[u], x);
+    if (norm) head_scale<N, GL>(x, w, __shfl_sync(0xffffffffu, rs, u, GL));
     if (turn) head_rotate<N, GL>(x, c, s, p.t.half, p.t.inter, g);
     const float sc = head_int8<N, GL>(x, codes + static_cast<long>(h) * HD + g * N, ok);
     if (g == 0 && ok) scale[h] = sc;

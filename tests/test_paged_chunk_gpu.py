@@ -819,3 +819,25 @@ def test_attention_row_tiles_across_slices(ops, seqs):
     lens = [(int(a), int(a + b)) for a, b in zip(rng.integers(1, 17, seqs), rng.integers(0, 900, seqs))]
     lens[0] = (16, 2500)
     run_attention(ops, Pool(ops, lens, 2, 64, page=32, seed=seqs), 4, "f16", "f16")
+
+
+def test_steps_without_a_pause(ops):
+    """Tables written anew and rows turned by them in place, back to back on one stream: each call
+    sees what the one before it wrote, and none overwrites what one before it still reads."""
+    rows, heads, hd, n = 4000, 8, 128, 8192
+    cos = torch.empty(n, hd // 2, device="cuda")
+    sin = torch.empty_like(cos)
+    pos = torch.randint(0, n, (rows,), device="cuda", dtype=torch.int32, generator=gen(1))
+    x0 = torch.randn(rows, heads * hd, device="cuda", generator=gen(2))
+
+    def steps(x, pause):
+        for i in range(12):
+            ops.rope_tables(cos, sin, 1e4, pos0=1000 * i)
+            pause()
+            ops.rope_rows(x, pos, cos, sin, x, heads)
+            pause()
+        return x
+
+    want = steps(x0.clone(), torch.cuda.synchronize)
+    for _ in range(3):
+        assert torch.equal(steps(x0.clone(), lambda: None), want)
