@@ -841,3 +841,41 @@ def test_steps_without_a_pause(ops):
     want = steps(x0.clone(), torch.cuda.synchronize)
     for _ in range(3):
         assert torch.equal(steps(x0.clone(), lambda: None), want)
+
+
+def test_captured_on_forked_streams(ops):
+    """Tables, rows and appends captured behind copies, on a stream that forks from the capture and
+    joins it again."""
+    P = Pool(ops, [(3, 70), (2, 40)], 2, 64, seed=4)
+    cos, sin = tables_f32(100, 64)
+    x = torch.randn(P.rows, 128, device="cuda", generator=gen(5))
+    pos = torch.tensor([67, 68, 69, 38, 39], device="cuda", dtype=torch.int32)
+    y, z = torch.zeros_like(x), torch.zeros_like(x)
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        y.copy_(x)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            ops.rope_rows(y, pos, cos, sin, y, 2, 64)
+            ops.paged_kv_append_batch(y, x, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 2,
+                                      64)
+        ops.rope_rows(x, pos, cos, sin, z, 2, 64)
+        main.wait_stream(side)
+        ops.rope_rows(y, pos, cos, sin, y, 2, 64)
+        z.add_(y)
+
+    side = torch.cuda.Stream()
+    step(side)
+    torch.cuda.synchronize()
+    want, k, ks = z.clone(), P.k.clone(), P.ks.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(side)
+    for _ in range(3):
+        z.zero_(), y.zero_(), P.k.zero_(), P.ks.zero_()
+        g.replay()
+    torch.cuda.synchronize()
+    row = (P.tables[0, 69 // 32].long() & 0xFFFF, 69 % 32)
+    assert torch.equal(z, want) and torch.equal(P.k[row], k[row]) and torch.equal(P.ks[row], ks[row])
+    assert (P.k[row] != 0).any()
