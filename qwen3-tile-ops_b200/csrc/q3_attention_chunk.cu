@@ -590,51 +590,52 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const 
   pdl_wait();
 }
 
-// The parts of one packed row of a (sequence, KV head) pair joined by a CTA: its warps take them in
-// turn, JOIN_AT loads at once.  Bound by latency: 111 parts a sequence at 2 x 65011 tokens; it looks
-// its parts up while the kernel before it still works, and adds about 2 us.
+// Parts joined: a CTA takes R packed rows of a (sequence, KV head) pair, 8 / R warps a row, which take its
+// parts in turn, JOIN_AT loads at once.  Bound by latency: look-ups, which hide behind the kernel
+// before it only where its CTAs leave room on the SMs, then the parts (111 a sequence at 2 x 65011
+// tokens).  R is the least of 1, 2, 4, 8 that leaves 6 CTAs an SM or fewer: whole calls with R = 1, 2,
+// 4, 8 take 8.4, 9.2, 10.0, 12.4 us (16 rows in all), 57.0, 53.8, 53.7, 54.6 (64 x 2048 tokens, 1024 rows),
+// 92, 79, 72, 69 (8192 rows).
 constexpr int JOIN_WARPS = 8, JOIN_AT = 4;
-template <int HD>
+template <int HD, int R>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uint32_t most) {
-  constexpr int N = HD / 32;
+  constexpr int N = HD / 32, WR = JOIN_WARPS / R;  // warps of a row
   __shared__ float so[JOIN_WARPS][HD], sm[JOIN_WARPS], sl[JOIN_WARPS];
-  __shared__ uint32_t range[2];
+  __shared__ uint32_t units[2];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int s = blockIdx.x, kvh = blockIdx.y;
   unsigned err = 0;
   const Seq q = load_seq(p, s, &err);
   int pb0;
   const int pn = seq_blocks(p, q, pb0);
-  const int m = blockIdx.z;                        // packed row
+  const int m = blockIdx.z * R + wid / WR, wr = wid % WR;   // packed row
   // (also a CTA with nothing to join waits: when this grid ends, the results are there)
-  if (pn == 0 || m >= q.n * p.group) {             // refused, or the other kernel's
+  if (pn == 0 || static_cast<int>(blockIdx.z) * R >= q.n * p.group) {   // refused, or the other kernel's
     pdl_wait();
     return;
   }
-  if (wid == 0) {   // the slices that have units of the sequence
+  if (wid == 0) {
     uint32_t before;
-    const Slices cut(count_units(p, s, lane, &err, before), most, p.min_units);
-    if (lane == 0) {
-      before += (m >> p.row_shift) * pn;
-      range[0] = cut.of(before);
-      range[1] = cut.of(before + pn - 1);
-    }
+    const uint32_t total = count_units(p, s, lane, &err, before);
+    if (lane == 0) units[0] = total, units[1] = before;
   }
   __syncthreads();
-  const uint32_t w0 = range[0], w1 = range[1];
+  // the slices that have units of the row's tile
+  const Slices cut(units[0], most, p.min_units);
+  const uint32_t u0 = units[1] + (m >> p.row_shift) * pn, w0 = cut.of(u0), w1 = cut.of(u0 + pn - 1);
   pdl_wait();
-  if (w0 == w1) return;                            // stored whole
+  const bool join = m < q.n * p.group && w0 != w1;   // (one slice: stored whole)
   const long r = q.first + m / p.group;
   const int h = kvh * p.group + m % p.group;
   float mm = kNegInf, l = 0.0f, x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
-  for (uint32_t w = w0 + wid; w <= w1; w += JOIN_WARPS * JOIN_AT) {
+  for (uint32_t w = w0 + wr; join && w <= w1; w += WR * JOIN_AT) {
     float pm[JOIN_AT], pl[JOIN_AT];
     Elems<float, N> e[JOIN_AT];
 #pragma unroll
     for (int k = 0; k < JOIN_AT; ++k) {
-      const uint32_t wk = w + k * JOIN_WARPS;
+      const uint32_t wk = w + k * WR;
       pm[k] = kNegInf;
       pl[k] = 0.0f;
 #pragma unroll
@@ -661,20 +662,20 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   for (int i = 0; i < N; ++i) so[wid][lane * N + i] = x[i];
   if (lane == 0) sm[wid] = mm, sl[wid] = l;
   __syncthreads();
-  if (wid) return;
+  if (wr || !join) return;
   float top = kNegInf;
 #pragma unroll
-  for (int i = 0; i < JOIN_WARPS; ++i) top = fmaxf(top, sm[i]);
+  for (int i = 0; i < WR; ++i) top = fmaxf(top, sm[wid + i]);
   const float base = top == kNegInf ? 0.0f : top;
   l = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < JOIN_WARPS; ++k) {
-    const float f = ex2(__fsub_rn(sm[k], base));
-    l = __fmaf_rn(f, sl[k], l);
+  for (int k = 0; k < WR; ++k) {
+    const float f = ex2(__fsub_rn(sm[wid + k], base));
+    l = __fmaf_rn(f, sl[wid + k], l);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f, so[k][lane * N + i], x[i]);
+    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f, so[wid + k][lane * N + i], x[i]);
   }
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
@@ -823,9 +824,15 @@ static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t 
   const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
   const unsigned z = static_cast<unsigned>(packed < p.few_rows ? packed : p.few_rows);
   if (p.whole) return Q3_OK;
-  return launch_ex(true, chunk::k_attn_join<HD>, dim3(p.n_seqs, p.kv_heads, z),
-                   dim3(chunk::JOIN_WARPS * 32), 0, s, p,
-                   static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads);
+  const uint32_t most = static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads;
+  const long pairs = static_cast<long>(p.n_seqs) * p.kv_heads, room = 6L * sm_count();
+  const unsigned r = pairs * z <= room ? 1 : pairs * ((z + 1) / 2) <= room ? 2 : pairs * ((z + 3) / 4) <= room ? 4 : 8;
+  const auto join = r == 1   ? chunk::k_attn_join<HD, 1>
+                    : r == 2 ? chunk::k_attn_join<HD, 2>
+                    : r == 4 ? chunk::k_attn_join<HD, 4>
+                             : chunk::k_attn_join<HD, 8>;
+  return launch_ex(true, join, dim3(p.n_seqs, p.kv_heads, (z + r - 1) / r),
+                   dim3(chunk::JOIN_WARPS * 32), 0, s, p, most);
 }
 
 template <int HD>
