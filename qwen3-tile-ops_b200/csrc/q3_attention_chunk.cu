@@ -73,10 +73,10 @@ constexpr int KB = 32;                             // keys of a block
 // slices of 4 10.2, of 1 8.5 with more parts).  Beside the many-row kernel this one has the SMs that
 // are left, and many short slices queue there (16 ragged sequences 64 us; of 2 72, of 32 79).
 constexpr int ALONE_UNITS = 2, BESIDE_UNITS = 8;
-// Most packed rows of a sequence of this kernel, in tiles that read the keys again.  Alone: 8 sequences
-// of 32 packed rows over 4000 tokens 44 us, in the many-row kernel 54; 64 over 2000 161 and 187; with 48
-// rows 242 and 187.  Beside: 32 makes the ragged batch above 2 us slower.
-constexpr int ALONE_ROWS = 32, BESIDE_ROWS = 16;
+// Most packed rows of a sequence of this kernel, in tiles that read the keys again.  Alone: 2 sequences of
+// 48 packed rows over 1000 tokens 15.1 us, in the many-row kernel 20.4; 64 over 2000 177 and 181; 8 of 64
+// rows over 4000 63 and 54.  Beside the many-row kernel: 16 ragged sequences 62.8 us, with 32 rows 64.0.
+constexpr int ALONE_ROWS = 48, BESIDE_ROWS = 16;
 constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that is never cut
 
 template <int HD>
@@ -105,7 +105,7 @@ __device__ __forceinline__ int units_of(const Args &p, int s, unsigned *err) {
   const int n = seq_blocks(p, q, b0);
   return n ? n * row_tiles(p, q) : 0;
 }
-// All units, and those of the sequences before s0 (whole warp; the host bounds them by 2^31)
+// All units, and those of the sequences before s0 (whole warp; the host bounds them by 3 2^30)
 __device__ __forceinline__ uint32_t count_units(const Args &p, int s0, int lane, unsigned *err,
                                                 uint32_t &before) {
   uint32_t x = 0, y = 0;

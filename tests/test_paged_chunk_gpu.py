@@ -803,6 +803,9 @@ def test_nothing_to_do(ops):
     (3, 1, 64, 32, 33, [(9, 1500)]),
     (2, 2, 64, 32, 0, [(17, 3000), (32, 300), (33, 33)]),          # rows one behind the most
     (4, 2, 128, 32, 0, [(1, 200), (4, 4), (2, 130)]),              # short, and few of them
+    (2, 2, 64, 32, 0, [(48, 2000), (33, 300), (1, 1), (47, 47)]),
+    (8, 2, 128, 16, 100, [(12, 1500), (9, 30), (5, 400)]),
+    (2, 2, 64, 32, 0, [(49, 3000), (48, 300), (16, 90), (17, 33)]),
 ])
 def test_attention_row_tiles(ops, heads, kvh, hd, page, window, lens):
     P = Pool(ops, lens, kvh, hd, page, seed=heads + len(lens))
