@@ -699,19 +699,36 @@ __global__ void k_join_tiles(const Args p) {
   unsigned err = 0;
   const Seq q = load_seq(p, s, &err);
   if (!q.ok || q.n * p.group <= p.few_rows) return;
-  float mm = kNegInf, l = 0.0f, x[N];
-  for (int z = 0; z < p.splits; ++z)
-    mm = fmaxf(mm, p.part_ml[((static_cast<long>(z) * p.rows + r) * p.heads + h) * 2]);
-  const float base = mm == kNegInf ? 0.0f : mm;
+  // lane z has the maximum and sum of part z, and of z + 32 (splits <= 64)
+  const long at = r * p.heads + h, step = static_cast<long>(p.rows) * p.heads;
+  float pm[2], pl[2], f[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int z = lane + i * 32;
+    pm[i] = z < p.splits ? p.part_ml[(z * step + at) * 2] : kNegInf;
+    pl[i] = z < p.splits ? p.part_ml[(z * step + at) * 2 + 1] : 0.0f;
+  }
+  const float mm = warp_tree_max(fmaxf(pm[0], pm[1])), base = mm == kNegInf ? 0.0f : mm;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) f[i] = ex2(__fsub_rn(pm[i], base));
+  const float l = warp_tree_sum(__fmaf_rn(f[1], pl[1], __fmul_rn(f[0], pl[0])));
+  float x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.0f;
-  for (int z = 0; z < p.splits; ++z) {
-    const long at = (static_cast<long>(z) * p.rows + r) * p.heads + h;
-    const float f = ex2(__fsub_rn(p.part_ml[at * 2], base));
-    if (f == 0.0f) continue;                       // (a part without keys has no sums)
-    l = __fmaf_rn(f, p.part_ml[at * 2 + 1], l);
+  for (int z0 = 0; z0 < p.splits; z0 += JOIN_AT) {
+    Elems<float, N> e[JOIN_AT];
+    float fz[JOIN_AT];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f, p.part_o[at * HD + lane * N + i], x[i]);
+    for (int k = 0; k < JOIN_AT; ++k) {
+      const int z = z0 + k;
+      fz[k] = __shfl_sync(0xffffffffu, z < 32 ? f[0] : f[1], z & 31);
+      if (fz[k] != 0.0f) e[k].load(p.part_o + (z * step + at) * HD + lane * N);
+      else e[k].zero();                              // (a part without keys has no sums)
+    }
+#pragma unroll
+    for (int k = 0; k < JOIN_AT; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(fz[k], e[k].e[i], x[i]);
   }
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
