@@ -68,6 +68,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // Two stages of 32 keys: three leave fewer warps an SM (58 us); L2 prefetch of later pages 61 us.
 // ---------------------------------------------------------------------------
 constexpr int WARPS = 4;
+// CTAs an SM: what registers give without spills (head_dim 64: three CTAs with two stages each 17.1 us for 24
+// sequences of 5 new rows and 70 for 64 of 20; two CTAs with four stages 17.8 and 78)
+__host__ __device__ constexpr int few_ctas_sm(int hd, int nt) { return hd == 64 || nt == 1 ? 3 : 2; }
 constexpr int KB = 32;                             // keys of a block
 // Least units of a slice.  Alone, short slices spread a small batch (one sequence of 2000 tokens 8.5 us;
 // slices of 4 10.2, of 1 8.5 with more parts).  Beside the many-row kernel this one has the SMs that
@@ -81,7 +84,7 @@ constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence th
 
 template <int HD>
 struct FewStage {
-  static constexpr int STAGES = HD == 128 ? 2 : 4;
+  static constexpr int STAGES = 2;
   uint4 k[KB * HD / 16], v[KB * HD / 16];
   float ks[KB], vs[KB];
 };
@@ -169,7 +172,7 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool ok) {
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) k_attn_few(const Args p) {
+__global__ void __launch_bounds__(WARPS * 32, few_ctas_sm(HD, NT)) k_attn_few(const Args p) {
   constexpr int KW = HD / 16, VW = HD / 32;   // k16 steps; words of a thread's V bytes
   constexpr int CH = HD / 16;                 // 16-byte chunks of a row
   using Stage = FewStage<HD>;
@@ -765,7 +768,7 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
     const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB) *
                        ((most_rows + 8 * c.nt - 1) / (8 * c.nt));
     const long slices = (units + c.min_units - 1) / c.min_units;
-    const long most = static_cast<long>(sms) * (c.nt == 1 ? 3 : 2), least = (kv_heads + WARPS - 1) / WARPS;
+    const long most = static_cast<long>(sms) * few_ctas_sm(head_dim, c.nt), least = (kv_heads + WARPS - 1) / WARPS;
     long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
     ctas = ctas < most ? ctas : most;
     ctas = ctas > least ? ctas : least;            // a slice at least
