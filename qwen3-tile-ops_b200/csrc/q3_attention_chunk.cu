@@ -846,7 +846,10 @@ static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t 
   if (p.whole) return Q3_OK;
   const uint32_t most = static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads;
   const long pairs = static_cast<long>(p.n_seqs) * p.kv_heads, room = 6L * sm_count();
-  const unsigned r = pairs * z <= room ? 1 : pairs * ((z + 1) / 2) <= room ? 2 : pairs * ((z + 3) / 4) <= room ? 4 : 8;
+  const unsigned r = pairs * z <= room               ? 1
+                     : pairs * ((z + 1) / 2) <= room ? 2
+                     : pairs * ((z + 3) / 4) <= room ? 4
+                                                     : 8;
   const auto join = r == 1   ? chunk::k_attn_join<HD, 1>
                     : r == 2 ? chunk::k_attn_join<HD, 2>
                     : r == 4 ? chunk::k_attn_join<HD, 4>
@@ -898,7 +901,8 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   const uint32_t max_kv = max_pages * kv->page_tokens;
   const chunk::Plan c =
       chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim);
-  if (c.few_ctas > 0x7fffffff / chunk::WARPS || c.tiles * kv_heads > 0x7fffffff || static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
+  if (c.few_ctas > 0x7fffffff / chunk::WARPS || c.tiles * kv_heads > 0x7fffffff ||
+      static_cast<uint64_t>(n_seqs) * max_kv > 0x7fffffffull * 16)
     return Q3_ERR_SHAPE;
   if (c.bytes) {
     if (!workspace) return Q3_ERR_NULL;

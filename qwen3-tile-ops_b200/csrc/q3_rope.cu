@@ -27,7 +27,8 @@ namespace rope {
 // nearest quarter turn is taken off the leading 32 bits, and sin and cos of the rest,
 // at most 1/8 turn = pi/4, are their Taylor series (to x^9 and x^10: remainders below
 // 2^-29); conversion, series and scaling stay within 2^-22.  131072 positions of 64 pairs are bound by
-// their stores (67 MB in 13.2 us, 5.1 TB/s; with two CTAs an SM 15.7), 4096 by launch (2.4 us; 3.1 if not launched as a dependent).
+// their stores (67 MB in 13.2 us, 5.1 TB/s; with two CTAs an SM 15.7), 4096 by launch
+// (2.4 us; 3.1 if not launched as a dependent).
 // ---------------------------------------------------------------------------
 constexpr int MAX_PAIRS = 128;
 struct TableArgs {
@@ -251,7 +252,8 @@ struct RowArgs {
 };
 
 template <typename T, int N, int GL>
-__global__ void __launch_bounds__(128, sizeof(T) == 2 ? (GL == 32 ? 7 : 8) : N == 8 ? 5 : 9) k_rope_rows(RowArgs p) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? (GL == 32 ? 7 : 8) : N == 8 ? 5 : 9)
+    k_rope_rows(RowArgs p) {
   constexpr int HD = GL * N, HW = 32 / GL;         // heads a warp holds at once
   pdl_trigger();
   const int lane = threadIdx.x & 31, g = lane % GL, hl = lane / GL;
