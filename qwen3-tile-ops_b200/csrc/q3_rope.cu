@@ -358,7 +358,7 @@ __global__ void k_kv_append(AppendArgs p) {
   uint32_t page = 0;
   if (pos < 0) bad = kBadRagged;
   else if (lp >= p.max_pages) bad = kBadTable;
-  else if (turn && pos >= p.t.rows) bad = kBadPosition;
+  else if (p.t.half && pos >= p.t.rows) bad = kBadPosition;   // (V is not rotated, but goes with its K)
   else {
     page = p.tables[static_cast<long>(q) * p.max_pages + lp];
     if (page >= p.num_pages) bad = kBadPage;

@@ -882,3 +882,33 @@ def test_captured_on_forked_streams(ops):
     row = (P.tables[0, 69 // 32].long() & 0xFFFF, 69 % 32)
     assert torch.equal(z, want) and torch.equal(P.k[row], k[row]) and torch.equal(P.ks[row], ks[row])
     assert (P.k[row] != 0).any()
+
+
+@pytest.mark.parametrize("t,hd,inter", [("f32", 128, False), ("bf16", 64, True)])
+def test_append_beyond_the_tables(ops, q3, request, t, hd, inter):
+    """Tables shorter than the page table: a token at a position that they lack is not written at
+    all, neither K nor V; the others are as with longer tables."""
+    request.node.keywords["status"] = True
+    lens = [(3, 51), (1, 50), (1, 64), (2, 97)]        # positions 48 49 50 | 49 | 63 | 95 96
+    P, kvh = Pool(ops, lens, 3, hd, seed=17), 3
+    k, v = (torch.randn(P.rows, kvh * hd, device="cuda", generator=gen(s)).to(TYPES[t])
+            for s in (1, 2))
+    cos, sin = tables_f32(97, hd)
+    arrays = P.k, P.v, P.ks, P.vs
+    before = [y.clone() for y in arrays]
+    call = lambda n: ops.paged_kv_append_batch(                                    # noqa: E731
+        k, v, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, len(lens), kvh, hd, cos=cos[:n],
+        sin=sin[:n], interleaved=inter)
+    call(97)
+    assert q3._lib.lib().q3_device_status() == 0
+    full = [y.clone() for y in arrays]
+    for y, z in zip(arrays, before):
+        y.copy_(z)
+    call(50)
+    assert q3._lib.lib().q3_device_status() == 1 << 4
+    tab = P.tables.long() & 0xFFFF
+    for s, j in ((0, 50), (2, 63), (3, 95), (3, 96)):
+        for y, z in zip(full, before):
+            y[tab[s, j // 32], j % 32] = z[tab[s, j // 32], j % 32]
+    for got, want in zip(arrays, full):
+        assert torch.equal(got, want)
