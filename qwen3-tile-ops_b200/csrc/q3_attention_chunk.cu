@@ -6,11 +6,12 @@
 //     p_ij = 2^(t_ij - M_i) <= 1,
 //     o_i  = sum_j p_ij V8_j  /  sum_j p_ij / vs_j.
 // The V scale rides in the exponent, so p spans [0, 1] whatever the scales are
-// and the f16 rounding of p (2^-11 relative, the only rounding to fewer than 32
-// bits) falls on weights relative to the row's largest contribution.  The codes
-// are exact in f16, the products are summed in float32, and one pass keeps the
-// running maximum: the accumulators are rescaled only when it grows by more
-// than 2^8 over the reference in use (p then stays below 2^8, far inside f16).
+// and the f16 rounding of p falls on weights relative to the row's largest
+// contribution: 2^-11 of a weight, and 2^-32 of the largest one for weights below
+// 2^-21 of it.  The codes are exact in f16, the products are summed in float32,
+// and one pass keeps the running maximum: M is in fact a reference 2^7 below
+// the maximum at the time it was set, and the accumulators are rescaled only when
+// a weight outgrows it by 2^15 (p stays inside f16).
 //
 // bf16 queries are multiplied by a power of two per row, which brings the row's
 // maximum to [2^10, 2^11): their 8 bits then fit f16 exactly down to 2^-24 of
@@ -437,11 +438,11 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas_sm(HD, NT)) k_attn_few(co
         for (int i = 0; i < 4; ++i) {
           ks[i] = st.ks[i * 8 + g];
           const float v = st.vs[i * 8 + g];
-          rv[i] = rcp(fmaxf(v, kVsMin));             // (NaN: fmaxf drops it ...
+          rv[i] = __fmul_rn(rcp(fmaxf(v, kVsMin)), kSumScale);   // (NaN: fmaxf drops it ...
           lv[i] = v != v ? v : lg2(fmaxf(v, kVsMin));// ... and the rows that see it get NaN)
         }
         const bool masked = mask != 0xffffffffu || x * KB + KB - 1 > pmin || p.window > 0;
-        // relative to the reference of the row's weights, which moves when one outgrows it by 2^8
+        // relative to the reference of the row's weights, which moves when one outgrows it by 2^kRefMove
         float top[NT][2];
         bool grow = false;
 #pragma unroll
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas_sm(HD, NT)) k_attn_few(co
               mx = fmaxf(mx, y);
             }
             top[n][j] = mx;
-            grow = grow || mx > 8.0f || mref[n][j] == kNegInf;
+            grow = grow || mx > kRefMove || mref[n][j] == kNegInf;
           }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -475,9 +476,10 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas_sm(HD, NT)) k_attn_few(co
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
               const bool none = mref[n][j] == kNegInf;
-              const float up = mx > (none ? kNegInf : 8.0f) ? mx : 0.0f;
+              const bool move = mx > (none ? kNegInf : kRefMove);
+              const float up = move ? __fsub_rn(mx, kRefBelow) : 0.0f;
               const float f = none ? 1.0f : ex2(-up);    // (without a reference the sums are zero)
-              if (mx > (none ? kNegInf : 8.0f)) mref[n][j] = none ? up : __fadd_rn(mref[n][j], up);
+              if (move) mref[n][j] = none ? up : __fadd_rn(mref[n][j], up);
               lsum[n][j] = __fmul_rn(lsum[n][j], f);
 #pragma unroll
               for (int d = 0; d < HD / 16; ++d) {
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas_sm(HD, NT)) k_attn_few(co
             y[2 * i + 1] = o[i][n][2 + j];
           }
           if (whole) {
-            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);   // no key seen: zeros
+            const float inv = inverse_sum(l);
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) y[i] = __fmul_rn(y[i], inv);
             const int mm = m0 + min(m, packed - 1);
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(f, so[wid + k][lane * N + i], x[i]);
   }
-  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  const float inv = inverse_sum(l);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = __fmul_rn(x[i], inv);
   store_out<N>(p, r, h, lane, x);
@@ -733,7 +735,7 @@ __global__ void k_join_tiles(const Args p) {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(fz[k], e[k].e[i], x[i]);
   }
-  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  const float inv = inverse_sum(l);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = __fmul_rn(x[i], inv);
   store_out<N>(p, r, h, lane, x);

@@ -76,6 +76,13 @@ __device__ __forceinline__ void split_range(int b0, int b1, int splits, int z, i
 }
 
 constexpr float kVsMin = 7.888609052210118e-31f;   // 2^-100
+// Weights are formed relative to a reference kRefBelow under the maximum so far (in powers of two) and
+// it moves when one outgrows it by 2^kRefMove: they stay within f16's range, and those down to
+// 2^-32 of the largest are not lost in the sums over the fraction while those under it, in
+// float32, have them.  The sums of p / vs carry 2^-kRefBelow (in rv): no term passes 2^108.
+constexpr float kRefBelow = 7.0f, kRefMove = 15.0f, kSumScale = 0.0078125f;
+// the sums over the fraction by those under it (no key seen: zeros)
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : __fdiv_rn(kSumScale, l); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

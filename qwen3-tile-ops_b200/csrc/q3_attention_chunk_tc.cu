@@ -9,7 +9,7 @@
 //   warps 0-15   rows: eight warps a tile, two a TMEM lane quadrant, 16 rows each
 //   warps 16-23  codes of K and V from global memory, widened to f16 (exact), into a
 //                ring of three operand tiles in the 128-byte-swizzled layout
-//   warp 24      page lookups, and the keys' scales as ks qk_scale log2 e, log2 vs, 1 / vs
+//   warp 24      page lookups, and the keys' scales as ks qk_scale log2 e, log2 vs, 2^-7 / vs
 //   warp 25      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
 // The loads are plain ones because each code passes through registers on its
@@ -209,7 +209,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Half a key tile (64 keys) for 16 rows of a warp, a thread holding rows e = 0, 1 (lane / 4 and + 8) and
 // columns 8i + 2 (lane % 4), + 1: scores at `st` to weights in their place.  ks holds ks qk_scale
 // log2 e; UNIT: a = 1 in all rows.  The reference of a row's weights moves only when a weight
-// outgrows it by 2^8, which a vote tells, so no row maximum is formed otherwise; then the sums at
+// outgrows it by 2^kRefMove, which a vote tells, so no row maximum is formed otherwise; then the sums at
 // `ot` are rescaled, once the products before this half's are in (`next`, the barrier of the next
 // half's scores, which follow them, with parity par; par < 0: there are none).
 template <int HD, bool MASK, bool UNIT>
@@ -254,16 +254,16 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
       mx1 = max3(mx1, y[2], y[3]);
     }
   }
-  const bool grow = fmaxf(mx0, mx1) > 8.0f || mref[0] == kNegInf || mref[1] == kNegInf;
+  const bool grow = fmaxf(mx0, mx1) > kRefMove || mref[0] == kNegInf || mref[1] == kNegInf;
   if (__any_sync(0xffffffffu, grow)) {
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
     // maxima relative to the old references (0 where there was none yet)
-    const bool g0 = mx0 > (mref[0] == kNegInf ? kNegInf : 8.0f);
-    const bool g1 = mx1 > (mref[1] == kNegInf ? kNegInf : 8.0f);
-    const float u0 = g0 ? -mx0 : 0.0f, u1 = g1 ? -mx1 : 0.0f;
+    const bool g0 = mx0 > (mref[0] == kNegInf ? kNegInf : kRefMove);
+    const bool g1 = mx1 > (mref[1] == kNegInf ? kNegInf : kRefMove);
+    const float u0 = g0 ? __fsub_rn(kRefBelow, mx0) : 0.0f, u1 = g1 ? __fsub_rn(kRefBelow, mx1) : 0.0f;
     // (without a reference all sums are still zero)
     const float r0 = mref[0] == kNegInf ? 1.0f : ex2(u0), r1 = mref[1] == kNegInf ? 1.0f : ex2(u1);
     b0 = __fadd_rn(b0, u0);
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         p.part_ml[at * 2 + 1] = mine > 0 ? lsum : 0.0f;
       }
     } else if (mine > 0) {
-      const float inv = lsum == 0.0f ? 0.0f : __fdiv_rn(1.0f, lsum);   // no key seen: zeros
+      const float inv = inverse_sum(lsum);
       const bool i8 = p.o_dt == Q3_DT_I8;
       const int es = i8 ? 1 : 2;
       char *out = p.o + r * p.o_rb + (static_cast<long>(h) * HD + ps * OC * 32) * es;
@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         sm.ks[in][to] = __fmul_rn(now.ks[i], p.scale_log2);
         // ... and the rows that see it get NaN); a key that is not there: weight 0
         sm.lv[in][to] = !now.have[i] ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
-        sm.rv[in][to] = rcp(v);
+        sm.rv[in][to] = __fmul_rn(rcp(v), kSumScale);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_full[in]);

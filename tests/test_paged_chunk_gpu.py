@@ -912,3 +912,51 @@ def test_append_beyond_the_tables(ops, q3, request, t, hd, inter):
             y[tab[s, j // 32], j % 32] = z[tab[s, j // 32], j % 32]
     for got, want in zip(arrays, full):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("heads,kvh,lens", [
+    (8, 8, [(1, 60000)] * 444),                        # a slice of the keys is a sequence or more
+    (64, 8, [(512, 60000)])])                          # 128 tiles: keys in one part
+def test_attention_one_heavy_key(ops, heads, kvh, lens):
+    """60000 keys of 2^-25.4 of the first one's weight each: together 0.14 % of the sum.  All values
+    are 1, so the result is 1 if the sums over and under the fraction see the same weights.
+    Weights are rounded to f16: the heavy one is a power of two but for 2^-18 (its logit's float32
+    steps: 25.4 + 7 bits of 2^-24 twice), the light ones, 2^-32.4 times f16's largest power of
+    two and so at least 2^-18.4, are off by at most 2^-25 each, 2^-6.6 of themselves; the result
+    by half a step of f16 at 1."""
+    hd, light = 64, 60000 * 2.0 ** -25.4
+    P = Pool(ops, [(1, 60000)], kvh, hd)
+    P.k.zero_(), P.v.fill_(100), P.ks.fill_(1.0), P.vs.fill_(0.01)
+    tab = P.tables.long() & 0xFFFF
+    P.k[tab[0, 0], 0] = 100                            # (a query is one in column 0 only)
+    n = len(lens)
+    tables = P.tables.expand(n, -1).contiguous()       # one cache, read by all
+    rows = sum(a for a, _ in lens)
+    row0 = torch.tensor(np.cumsum([0] + [a for a, _ in lens]), dtype=torch.int32, device="cuda")
+    kv_len = torch.tensor([b for _, b in lens], dtype=torch.int32, device="cuda")
+    q = torch.zeros(rows, heads, hd, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1.0
+    o = torch.empty(rows, heads * hd, device="cuda", dtype=torch.float16)
+    ops.attention_chunk_batch(q.view(rows, -1), None, P.kv, P.n_pages, tables, P.mp, row0, kv_len, n,
+                              lens[0][0], o, None, heads, kvh, hd, False, 0, 0.254 * math.log(2.0))
+    tol = 2.0 ** -12 + 2.0 ** -17 + light * 2.0 ** -6.6 + 2 * 2.0 ** -11 * light
+    assert tol < light / 2
+    assert ((o.double() - 1.0).abs() <= tol).all(), float((o.double() - 1.0).abs().max())
+
+
+@pytest.mark.parametrize("otype", ["bf16", "i8"])
+@pytest.mark.parametrize("power", [-93, 110])
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_far_value_scales(ops, new, power, otype):
+    """V scales near the ends of float32: the sums of weights over scales stay in range.  (Those of
+    2^-93 times 0.005 and more pass 2^-100, as which the operator counts smaller ones.)"""
+    P = Pool(ops, [(new, 3000), (new, 300)], 2, 128, seed=23)
+    P.vs.mul_(2.0 ** power)
+    q, _, q64 = make_q(P, 4, "bf16", 1, spread=4.0)
+    o = torch.empty(P.rows, 512, device="cuda", dtype=torch.int8 if otype == "i8" else TYPES[otype])
+    os = torch.empty(P.rows, 4, device="cuda") if otype == "i8" else None
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, new, o,
+                              os, 4, 2, 128, True, 0, 128 ** -0.5)
+    P.vs.clamp_(min=2.0 ** -100)
+    want, tol = ref_attention(P, q64, 4, True, 0, 128 ** -0.5)
+    check_rows(o, os, want, tol, 4, 128, P.rows)
