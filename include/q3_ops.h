@@ -305,8 +305,11 @@ int q3_prefill_batch(void *blob, const q3_layout *layout, const q3_kv_pool *pool
  * views (none is allowed); they are its last tokens, at positions
  * kv_len[s] - n_s + i, n_s = row0[s+1] - row0[s]: kv_len counts them.  Rows at
  * and behind row0[n_seqs] belong to nobody and are left as they were.  What
- * these arrays and the page tables hold is checked on the device: a row that
- * does not fit is skipped and sets a bit of q3_device_status.
+ * these arrays and the page tables hold is checked on the device: what does not
+ * fit is skipped and sets a bit of q3_device_status.  A sequence whose rows do not
+ * all exist is skipped by append and attention alike; beyond that the append goes
+ * row by row (one with a position that is negative, or outside the page table or
+ * the rotary tables, is not written, its neighbours are), the attention by sequence.
  * Row views: head h of row r at columns h*head_dim; head_dim 64, 128 or 256
  * (attention: 64 or 128); bases and row strides in multiples of 16 bytes. */
 enum { Q3_ROPE_NONE = 0, Q3_ROPE_LINEAR = 1, Q3_ROPE_YARN = 2 };

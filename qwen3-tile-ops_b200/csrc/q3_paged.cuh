@@ -114,6 +114,11 @@ __device__ __forceinline__ void store_row_stream(const float (&x)[N], void *p) {
   from_f32<T>(x).store_stream(p);
 }
 
+// Rows first .. end-1 of a sequence do not all exist (none: nothing is missing)
+__device__ __forceinline__ bool rows_missing(int first, int end, int rows) {
+  return first != end && (first < 0 || end < first || end > rows);
+}
+
 // Sequence of row r (whole warp): the last s with row0[s] <= r, or -1 when r
 // belongs to nobody.  Each round a warp looks at 32 places of the ascending
 // array, so 1024 sequences take two rounds.  Whatever row0 holds, reads stay in

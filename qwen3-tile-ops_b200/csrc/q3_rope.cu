@@ -331,7 +331,16 @@ __global__ void k_kv_append(AppendArgs p) {
   const int chunks = (p.kv_heads + U * HW - 1) / (U * HW);
   long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long r = unit / (2 * chunks);
-  if (r >= p.rows) return;
+  if (r >= p.rows) {
+    // one warp more than the rows need: do the sequences' rows exist?
+    if (unit != static_cast<long>(p.rows) * (2 * chunks)) return;
+    pdl_wait();
+    bool bad = false;
+    for (int s = lane; s < p.n_seqs; s += 32)
+      bad = bad || rows_missing(p.row0[s], p.row0[s + 1], p.rows);
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&g_rope_error, kBadRagged);
+    return;
+  }
   unit -= r * (2 * chunks);
   const bool is_v = unit >= chunks;
   const int h0 = static_cast<int>(is_v ? unit - chunks : unit) * (U * HW);
@@ -351,7 +360,8 @@ __global__ void k_kv_append(AppendArgs p) {
   }
   int first, count;
   const int q = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
-  if (q < 0) return;                               // a row that belongs to nobody
+  // a row that belongs to nobody, or to a sequence that the extra warp reports
+  if (q < 0 || rows_missing(first, first + count, p.rows)) return;
   const long pos = static_cast<long>(p.kv_len[q]) - count + (r - first);
   const long lp = pos < 0 ? 0 : static_cast<long>(static_cast<uint64_t>(pos) / p.page_tokens);
   unsigned bad = 0;
@@ -554,7 +564,7 @@ template <typename T>
 static int launch_append(const AppendArgs &p, uint32_t hd, cudaStream_t s) {
   constexpr int N = 16 / static_cast<int>(sizeof(T));   // head_dim 256: 8 columns a lane
   const int per = U * (hd >= 32 * N ? 1 : 32 * N / static_cast<int>(hd));   // heads of a warp
-  const long warps = static_cast<long>(p.rows) * 2 * ((p.kv_heads + per - 1) / per);
+  const long warps = static_cast<long>(p.rows) * 2 * ((p.kv_heads + per - 1) / per) + 1;
   const unsigned blocks = (unsigned)((warps + 3) / 4);
   const dim3 grid(blocks), block(128);
   return hd == 64    ? launch_ex(true, k_kv_append<T, N, 64 / N>, grid, block, 0, s, p)

@@ -960,3 +960,34 @@ def test_attention_far_value_scales(ops, new, power, otype):
     P.vs.clamp_(min=2.0 ** -100)
     want, tol = ref_attention(P, q64, 4, True, 0, 128 ** -0.5)
     check_rows(o, os, want, tol, 4, 128, P.rows)
+
+
+@pytest.mark.parametrize("row0,written", [
+    ([0, 5, 4, 11, 42], [0, 2]),       # -1 rows; the last sequence passes the rows
+    ([0, 5, 20, 41, 50], [0, 1, 2]),   # all of the last one's rows are behind the end
+    ([-3, 5, 5, 9, 9], [2]),           # rows before the first
+    ([0, 41, 30, 30, 30], [0])])       # falls, and a row's last sequence has no rows
+def test_append_ragged_arrays_that_do_not_fit(ops, q3, request, row0, written):
+    """Sequences whose rows are not all there are skipped, with a status; others written."""
+    request.node.keywords["status"] = True
+    kvh, hd, rows = 2, 64, 41
+    P = Pool(ops, [(5, 90), (2, 90), (4, 90), (30, 90)], kvh, hd, seed=2)
+    P.row0.copy_(torch.tensor(row0, dtype=torch.int32))
+    k = torch.randn(rows, kvh * hd, device="cuda", generator=gen(1))
+    before = [y.clone() for y in (P.k, P.v, P.ks, P.vs)]
+    ops.paged_kv_append_batch(k, k, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 4, kvh, hd)
+    assert q3._lib.lib().q3_device_status() == 1 << 5
+    tab = P.tables.long() & 0xFFFF
+    may, must = set(), set()
+    for s in written:
+        a, b = row0[s], row0[s + 1]
+        for r in range(a, b):
+            j = 90 - (b - a) + r - a
+            at = (int(tab[s, j // 32]), j % 32)
+            may.add(at)
+            # (a row that two sequences claim is written for one of them)
+            if sum(row0[x] <= r < row0[x + 1] for x in range(4)) == 1 and row0 == sorted(row0):
+                must.add(at)
+    for got, old in zip((P.k, P.v, P.ks, P.vs), before):
+        changed = {(int(a), int(b)) for a, b in (got != old).any(-1).nonzero()}
+        assert must <= changed <= may
