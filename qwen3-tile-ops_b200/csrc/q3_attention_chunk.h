@@ -46,7 +46,7 @@ __device__ __forceinline__ Seq load_seq(const Args &p, int s, unsigned *err) {
   q.pos0 = q.kv - q.n;
   q.ok = q.n > 0;
   if (q.n == 0) return q;
-  if (q.n < 0 || q.first < 0 || end > p.rows || q.n > p.max_rows || q.kv < q.n) {
+  if (rows_missing(q.first, end, p.rows) || q.n > p.max_rows || q.kv < q.n) {
     *err |= kBadRagged;
     q.ok = false;
   } else if (static_cast<uint32_t>(q.kv) > p.max_pages * p.page_tokens) {

@@ -991,3 +991,20 @@ def test_append_ragged_arrays_that_do_not_fit(ops, q3, request, row0, written):
     for got, old in zip((P.k, P.v, P.ks, P.vs), before):
         changed = {(int(a), int(b)) for a, b in (got != old).any(-1).nonzero()}
         assert must <= changed <= may
+
+
+@pytest.mark.parametrize("new", [4, 300])
+def test_row_numbers_that_wrap(ops, q3, request, new):
+    """row0 whose difference fits only modulo 2^32: refused, not taken for one row."""
+    request.node.keywords["status"] = True
+    P = Pool(ops, [(new, 700), (3, 90)], 2, 64, seed=6)
+    big = 2 ** 31
+    P.row0.copy_(torch.tensor([big - 1, -big, -big + new], dtype=torch.int32))
+    x = torch.randn(P.rows, 128, device="cuda", generator=gen(1)).half()
+    o = torch.full((P.rows, 128), 7.0, device="cuda", dtype=torch.float16)
+    before = P.k.clone()
+    ops.attention_chunk_batch(x, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, new, o,
+                              None, 2, 2, 64, True, 0, 0.125)
+    assert q3._lib.lib().q3_device_status() == 1 << 5 and (o == 7).all()
+    ops.paged_kv_append_batch(x, x, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 2, 64)
+    assert q3._lib.lib().q3_device_status() == 1 << 5 and torch.equal(P.k, before)
