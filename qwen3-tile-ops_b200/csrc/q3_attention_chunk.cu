@@ -688,24 +688,26 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) k_attn_join(const Args p, uin
   store_out<N>(p, r, h, lane, x);
 }
 
-// The parts of k_attn_tc's key ranges: a warp a row and head.  Bound by latency; a few MB at most, since
-// keys are split only while the tiles cannot fill the card.
+// The parts of k_attn_tc's key ranges, 256 rows each in the order of its CTAs: a warp a packed row of a
+// tile.  Bound by latency; 20 MB written and read at most, since keys are split only while the tiles
+// cannot fill the card (148 parts of 256 rows).
+constexpr int TILE_WARPS = 4;
 template <int HD>
-__global__ void k_join_tiles(const Args p) {
+__global__ void __launch_bounds__(TILE_WARPS * 32) k_join_tiles(const Args p) {
   constexpr int N = HD / 32;
   const int lane = threadIdx.x & 31;
-  const long unit = static_cast<long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const long r = unit / p.heads;
-  const int h = static_cast<int>(unit % p.heads);
-  if (r >= p.rows) return;
-  int first, count;
-  const int s = find_seq(p.row0, p.n_seqs, static_cast<int>(r), lane, first, count);
-  if (s < 0) return;
+  const int kvh = blockIdx.x % p.kv_heads, row = blockIdx.y * TILE_WARPS + (threadIdx.x >> 5);
   unsigned err = 0;
+  int tile;
+  const int s = find_tile(p, blockIdx.x / p.kv_heads, lane, &err, tile);
+  if (s < 0) return;
   const Seq q = load_seq(p, s, &err);
-  if (!q.ok || q.n * p.group <= p.few_rows) return;
+  const int m = tile * TC_ROWS + row;
+  if (m >= q.n * p.group) return;
+  const long r = q.first + m / p.group;
+  const int h = kvh * p.group + m % p.group;
   // lane z has the maximum and sum of part z, and of z + 32 (splits <= 64)
-  const long at = r * p.heads + h, step = static_cast<long>(p.rows) * p.heads;
+  const long at = static_cast<long>(blockIdx.x) * p.splits * TC_ROWS + row, step = TC_ROWS;
   float pm[2], pl[2], f[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -794,7 +796,7 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
     z = z < most ? z : most;
     c.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   }
-  const size_t parts = c.splits > 1 ? static_cast<size_t>(c.splits) * rows * heads : 0;
+  const size_t parts = c.splits > 1 ? static_cast<size_t>(c.splits) * c.tiles * kv_heads * TC_ROWS : 0;
   c.bytes = (c.few_slots + parts) * (head_dim + 2) * 4;
   return c;
 }
@@ -864,8 +866,10 @@ template <int HD>
 static int launch_many(const chunk::Args &p, cudaStream_t s) {
   Q3_TRY(chunk::launch_tc(p, HD, s));
   if (p.splits == 1) return Q3_OK;
-  const long warps = static_cast<long>(p.rows) * p.heads;
-  chunk::k_join_tiles<HD><<<(unsigned)((warps + 3) / 4), 128, 0, s>>>(p);
+  const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
+  const unsigned rows = packed < chunk::TC_ROWS ? (unsigned)packed : chunk::TC_ROWS;   // of a tile
+  chunk::k_join_tiles<HD><<<dim3(p.tiles * p.kv_heads, (rows + chunk::TILE_WARPS - 1) / chunk::TILE_WARPS),
+                            chunk::TILE_WARPS * 32, 0, s>>>(p);
   return launch_status();
 }
 
@@ -955,7 +959,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     t.splits = c.splits;
     t.tiles = static_cast<int>(c.tiles);
     t.part_o = ws + c.few_slots * (head_dim + 2);
-    t.part_ml = t.part_o + static_cast<size_t>(c.splits) * rows * heads * head_dim;
+    t.part_ml = t.part_o + static_cast<size_t>(c.splits) * c.tiles * kv_heads * chunk::TC_ROWS * head_dim;
     st = head_dim == 128 ? launch_many<128>(t, s) : launch_many<64>(t, s);
   }
   if (st == Q3_OK && c.few_ctas) {

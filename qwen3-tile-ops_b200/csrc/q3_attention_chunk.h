@@ -173,6 +173,19 @@ __device__ __forceinline__ int find_unit(int n_seqs, long unit, int lane, long &
 // Many rows (q3_attention_chunk_tc.cu): sequences with more than few_rows packed rows.  `tiles` is the
 // number of 256-row tiles that the batch can have.
 constexpr int TC_ROWS = 256, TC_KEYS = 128;
+__device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
+  const Seq q = load_seq(p, s, err);
+  const int packed = q.n * p.group;
+  return q.ok && packed > p.few_rows ? (packed + TC_ROWS - 1) / TC_ROWS : 0;
+}
+// Sequence of tile `id` of the batch, -1: there is no such tile, and its place in the sequence: the last
+// one, which has most keys, first (whole warp)
+__device__ __forceinline__ int find_tile(const Args &p, int id, int lane, unsigned *err, int &tile) {
+  long before;
+  const int s = find_unit(p.n_seqs, id, lane, before, [&](int x) { return tiles_of(p, x, err); });
+  tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, err) - 1 - (id - before));
+  return s;
+}
 int launch_tc(const Args &p, int head_dim, cudaStream_t s);
 
 }  // namespace chunk

@@ -328,12 +328,6 @@ __device__ __forceinline__ void asm_less_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
 }
 
-__device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
-  const Seq q = load_seq(p, s, err);
-  const int packed = q.n * p.group;
-  return q.ok && packed > p.few_rows ? (packed + TC_ROWS - 1) / TC_ROWS : 0;
-}
-
 template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   constexpr int HALVES = HD / 64;
@@ -349,13 +343,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
   pdl_trigger();   // the few-row kernel may fill the SMs that this grid leaves
   if (warp == 0) {
     unsigned err = 0;
-    long before;
-    const int s = find_unit(p.n_seqs, tile_id, lane, before,
-                            [&](int x) { return tiles_of(p, x, &err); });
+    int tile;
+    const int s = find_tile(p, tile_id, lane, &err, tile);
     if (lane == 0) {
       sm.seq = s;
-      // the last tile, which has most keys, first
-      sm.tile = s < 0 ? 0 : static_cast<int>(tiles_of(p, s, &err) - 1 - (tile_id - before));
+      sm.tile = tile;
       sm.abort = 0;
       for (int i = 0; i < RING; ++i) {
         mbar_init(&sm.full[i], LOADERS);
@@ -572,7 +564,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       *reinterpret_cast<uint4 *>(stage + lane * bytes + ((c ^ (lane & (bytes / 16 - 1))) * 16)) = x;
     };
     if (p.splits > 1) {
-      const long at = (static_cast<long>(blockIdx.z) * p.rows + r) * p.heads + h;
+      const long at = (static_cast<long>(blockIdx.x) * p.splits + blockIdx.z) * TC_ROWS + m;
       if (mine > 0) {
 #pragma unroll 1
         for (int c = ps * OC; c < ps * OC + OC; ++c) {

@@ -211,3 +211,22 @@ def test_wrappers_refuse(q3):
         q3.ops.rope_rows(x, x, x, x, x, 2)
     with pytest.raises(ValueError):
         q3.ops.rope_tables(x, x, 1e6)
+
+
+def test_attention_workspace_of_padded_rows(L):
+    """Parts of split keys are those of the rows that sequences can have: rows that belong to nobody
+    take none, and a card's worth of 256-row parts is the most."""
+    f = L.lib().q3_attention_chunk_workspace_bytes
+    for hd in (64, 128):
+        for n_seqs, max_rows, max_kv in ((1, 256, 8192), (3, 200, 30000), (1, 100, 100000)):
+            own = f(n_seqs * max_rows, n_seqs, max_rows, max_kv, 8, 8, hd)
+            assert own > 0
+            for rows in (4096, 8192, 100000):
+                assert f(rows, n_seqs, max_rows, max_kv, 8, 8, hd) == own
+    for rows in (64, 200, 8192, 1 << 20):
+        for n_seqs in (1, 2, 7, 30, 200):
+            for max_rows in (49, 256, 1000, 1 << 20):
+                for kvh in (1, 2, 8):
+                    parts = 148 * 256 * 130 * 4        # of the tensor-core kernel: a CTA an SM
+                    few = 2 * 148 * 3 * 4 * 16 * 130 * 4
+                    assert f(rows, n_seqs, max_rows, 50000, 4 * kvh, kvh, 128) <= parts + few

@@ -1008,3 +1008,27 @@ def test_row_numbers_that_wrap(ops, q3, request, new):
     assert q3._lib.lib().q3_device_status() == 1 << 5 and (o == 7).all()
     ops.paged_kv_append_batch(x, x, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 2, 64)
     assert q3._lib.lib().q3_device_status() == 1 << 5 and torch.equal(P.k, before)
+
+
+@pytest.mark.parametrize("otype", ["f16", "i8"])
+@pytest.mark.parametrize("heads,kvh,hd,lens,most,pad", [
+    (4, 4, 128, [(200, 5000)], 200, 4000), (6, 2, 64, [(90, 9000), (300, 3000), (1, 40)], 310, 999),
+    (2, 1, 64, [(50, 700), (70, 3000), (256, 2000), (0, 9), (257, 300), (3, 8000)], 257, 77)])
+def test_attention_padded_rows(ops, heads, kvh, hd, lens, most, pad, otype):
+    """Split keys in a batch with rows behind its last sequence: a workspace of the rows that
+    sequences can have, no word behind it written, and the padding left as it was."""
+    P = Pool(ops, lens, kvh, hd, seed=31)
+    rows, n = P.rows + pad, len(lens)
+    q, _, q64 = make_q(P, heads, "f16", 4, rows=rows)
+    size = ops.attention_chunk_workspace_bytes(rows, n, most, P.mp * 32, heads, kvh, hd)
+    assert 0 < size <= 148 * (256 + 2 * 3 * 4 * 16) * (hd + 2) * 4   # a part a CTA; two a warp, of 16
+    ws = torch.full((size + 4096,), 0xFF, dtype=torch.uint8, device="cuda")
+    o = torch.full((rows, heads * hd), 7, device="cuda",
+                   dtype=torch.int8 if otype == "i8" else torch.float16)
+    os = torch.full((rows, heads), 7.0, device="cuda")
+    ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, n, most, o,
+                              os if otype == "i8" else None, heads, kvh, hd, True, 0, hd ** -0.5,
+                              workspace=ws[:size])
+    want, tol = ref_attention(P, q64[:P.rows], heads, True, 0, hd ** -0.5)
+    check_rows(o, os, want, tol, heads, hd, P.rows)
+    assert (o[P.rows:] == 7).all() and (os[P.rows:] == 7.0).all() and (ws[size:] == 0xFF).all()
