@@ -746,6 +746,7 @@ __global__ void __launch_bounds__(TILE_WARPS * 32) k_join_tiles(const Args p) {
 // How a call is cut.  Sequences with at most few_rows packed rows go to k_attn_few (nt tiles of 8),
 // the others to the tensor-core kernel of many rows.
 struct Plan {
+  long packed;                                     // most packed rows of a sequence
   int nt, few_rows, min_units;
   long few_ctas, few_tiles;                        // few_ctas 0: no such sequence can be there
   bool whole;                                      // their keys are not cut
@@ -757,7 +758,9 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
                       uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
   Plan c{};
   const long group = heads / kv_heads;
-  const long packed = static_cast<long>(max_rows < rows ? max_rows : rows) * group;
+  // (one with more new rows than its table holds tokens is refused)
+  const uint32_t most_new = max_rows < rows ? max_rows : rows;
+  const long packed = c.packed = static_cast<long>(most_new < max_kv ? most_new : max_kv) * group;
   const int sms = q3h::sm_count();
   const bool mixed = packed > ALONE_ROWS;
   c.few_rows = mixed ? BESIDE_ROWS : ALONE_ROWS;
@@ -841,11 +844,10 @@ static int opt_in(int bytes) {
 }
 
 template <int HD, int NT>
-static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t s) {
+static int launch_few(const chunk::Args &p, long packed, int ctas, bool beside, cudaStream_t s) {
   constexpr int smem = chunk::WARPS * chunk::FewStage<HD>::STAGES * (int)sizeof(chunk::FewStage<HD>);
   Q3_TRY((opt_in<&chunk::k_attn_few<HD, NT>>(smem)));
   Q3_TRY(launch_ex(beside, chunk::k_attn_few<HD, NT>, dim3(ctas), dim3(chunk::WARPS * 32), smem, s, p));
-  const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
   const unsigned z = static_cast<unsigned>(packed < p.few_rows ? packed : p.few_rows);
   if (p.whole) return Q3_OK;
   const uint32_t most = static_cast<uint32_t>(ctas) * chunk::WARPS / p.kv_heads;
@@ -863,10 +865,9 @@ static int launch_few(const chunk::Args &p, int ctas, bool beside, cudaStream_t 
 }
 
 template <int HD>
-static int launch_many(const chunk::Args &p, cudaStream_t s) {
+static int launch_many(const chunk::Args &p, long packed, cudaStream_t s) {
   Q3_TRY(chunk::launch_tc(p, HD, s));
   if (p.splits == 1) return Q3_OK;
-  const long packed = static_cast<long>(p.max_rows < p.rows ? p.max_rows : p.rows) * p.group;
   const unsigned rows = packed < chunk::TC_ROWS ? (unsigned)packed : chunk::TC_ROWS;   // of a tile
   chunk::k_join_tiles<HD><<<dim3(p.tiles * p.kv_heads, (rows + chunk::TILE_WARPS - 1) / chunk::TILE_WARPS),
                             chunk::TILE_WARPS * 32, 0, s>>>(p);
@@ -960,7 +961,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     t.tiles = static_cast<int>(c.tiles);
     t.part_o = ws + c.few_slots * (head_dim + 2);
     t.part_ml = t.part_o + static_cast<size_t>(c.splits) * c.tiles * kv_heads * chunk::TC_ROWS * head_dim;
-    st = head_dim == 128 ? launch_many<128>(t, s) : launch_many<64>(t, s);
+    st = head_dim == 128 ? launch_many<128>(t, c.packed, s) : launch_many<64>(t, c.packed, s);
   }
   if (st == Q3_OK && c.few_ctas) {
     p.row_shift = c.nt == 1 ? 3 : 4;
@@ -971,10 +972,10 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     p.part_ml = ws + c.few_slots * head_dim;
     const bool beside = c.tiles && c.splits == 1;   // the kernel before is the many-row one
     const int ctas = static_cast<int>(c.few_ctas);
-    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, ctas, beside, s)
-                                      : launch_few<128, 2>(p, ctas, beside, s))
-                         : (c.nt == 1 ? launch_few<64, 1>(p, ctas, beside, s)
-                                      : launch_few<64, 2>(p, ctas, beside, s));
+    st = head_dim == 128 ? (c.nt == 1 ? launch_few<128, 1>(p, c.packed, ctas, beside, s)
+                                      : launch_few<128, 2>(p, c.packed, ctas, beside, s))
+                         : (c.nt == 1 ? launch_few<64, 1>(p, c.packed, ctas, beside, s)
+                                      : launch_few<64, 2>(p, c.packed, ctas, beside, s));
   }
   timer_end(TIMER_ATTENTION, s);
   return st;

@@ -230,3 +230,15 @@ def test_attention_workspace_of_padded_rows(L):
                     parts = 148 * 256 * 130 * 4        # of the tensor-core kernel: a CTA an SM
                     few = 2 * 148 * 3 * 4 * 16 * 130 * 4
                     assert f(rows, n_seqs, max_rows, 50000, 4 * kvh, kvh, 128) <= parts + few
+
+
+def test_attention_workspace_of_loose_bounds(L):
+    """A sequence has no more new rows than its table holds tokens: a looser max_rows changes
+    nothing."""
+    f = L.lib().q3_attention_chunk_workspace_bytes
+    for rows, n_seqs, max_kv, kvh in ((4096, 1, 1000, 1), (4096, 2, 16, 8), (2000, 3, 24, 2),
+                                      (500, 1, 40, 4), (4096, 64, 256, 8)):
+        for hd in (64, 128):
+            tight = f(rows, n_seqs, max_kv, max_kv, 2 * kvh, kvh, hd)
+            for loose in (2 * max_kv, 1 << 20, (1 << 32) - 1):
+                assert f(rows, n_seqs, loose, max_kv, 2 * kvh, kvh, hd) == tight

@@ -1032,3 +1032,15 @@ def test_attention_padded_rows(ops, heads, kvh, hd, lens, most, pad, otype):
     want, tol = ref_attention(P, q64[:P.rows], heads, True, 0, hd ** -0.5)
     check_rows(o, os, want, tol, heads, hd, P.rows)
     assert (o[P.rows:] == 7).all() and (os[P.rows:] == 7.0).all() and (ws[size:] == 0xFF).all()
+
+
+@pytest.mark.parametrize("kvh,hd,page,lens", [
+    (2, 64, 16, [(1 + s % 5, 5 + s % 12) for s in range(64)]),       # no table holds 17 tokens
+    (2, 128, 32, [(1 + 3 * s, 60 + 3 * s) for s in range(40)]),      # whole sequences, in tiles
+    (1, 128, 32, [(7, 320), (300, 320), (40, 90)]), (2, 64, 8, [(8, 8), (3, 7)])])
+def test_attention_loose_max_rows(ops, kvh, hd, page, lens):
+    """max_rows far over what the tables hold: the same results as with the least one."""
+    P = Pool(ops, lens, kvh, hd, page, seed=14)
+    tight = run_attention(ops, P, 4, "f16", "f16")
+    for P.max_rows in (P.rows, 100000, 2 ** 32 - 1):
+        assert torch.equal(run_attention(ops, P, 4, "f16", "f16"), tight)
