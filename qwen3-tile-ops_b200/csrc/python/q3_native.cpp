@@ -232,6 +232,7 @@ PyObject *paged_kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // head_dim, causal, window, qk_scale, workspace, stream
 PyObject *attention_chunk(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&] {
+    if (n == 20 && a[18] != Py_None && !THPVariable_Check(a[18])) refuse("workspace: a tensor is needed");
     Call c(a, n, 20, 0);
     q3_view q, qs, o, os;
     const q3_view *pq = c.view(0, q), *pqs = c.view(1, qs), *po = c.view(10, o), *pos = c.view(11, os);

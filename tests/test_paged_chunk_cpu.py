@@ -242,3 +242,13 @@ def test_attention_workspace_of_loose_bounds(L):
             tight = f(rows, n_seqs, max_kv, max_kv, 2 * kvh, kvh, hd)
             for loose in (2 * max_kv, 1 << 20, (1 << 32) - 1):
                 assert f(rows, n_seqs, loose, max_kv, 2 * kvh, kvh, hd) == tight
+
+
+def test_wrapper_refuses_other_workspaces(q3):
+    """A workspace that is no tensor is named, before anything is done with it."""
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(2, 256)
+    for ws in (bytearray(64), 0x1000, [1], "ws"):
+        with pytest.raises(ValueError, match="workspace: a"):
+            q3.ops.attention_chunk_batch(x, None, pool(q3._lib), 9, x, 1, x, x, 1, 1, x, None, 4, 2, 64,
+                                         True, 0, 0.1, workspace=ws)
