@@ -4,6 +4,7 @@
 // small batches; building a view with ctypes takes 2.4 us and a call of it 3 us more
 // on the host, against about 1 us for a whole call here.
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -65,6 +66,23 @@ struct Call {
       Py_DECREF(s);
     }
     if (PyErr_Occurred()) throw PyError{};
+  }
+
+  // The stream given is being captured into a graph, the current one is not: what the allocator gives
+  // now belongs to the current one, and is another tensor's when the graph is replayed.
+  bool foreign_capture() const {
+    return given && capturing(static_cast<cudaStream_t>(stream)) &&
+           !capturing(c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  static bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(s, &status);
+    if (e == cudaErrorStreamCaptureImplicit) {   // the legacy stream beside a blocking captured one
+      cudaGetLastError();
+      return false;
+    }
+    C10_CUDA_CHECK(e);
+    return status != cudaStreamCaptureStatusNone;
   }
 
   const at::Tensor &tensor(int i) const {
@@ -253,6 +271,8 @@ PyObject *attention_chunk(PyObject *, PyObject *const *a, Py_ssize_t n) {
       bytes = t.nbytes();
     } else if ((bytes = q3_attention_chunk_workspace_bytes(q.rows, seqs, max_rows, mp * kv.page_tokens,
                                                            heads, kvh, hd))) {
+      if (c.foreign_capture())
+        refuse("workspace: needed where the stream given is being captured and the current one is not");
       ws = at::empty({static_cast<int64_t>(bytes)},
                      at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c.dev));
       at_ = ws.data_ptr();

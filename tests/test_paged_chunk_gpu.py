@@ -1044,3 +1044,36 @@ def test_attention_loose_max_rows(ops, kvh, hd, page, lens):
     tight = run_attention(ops, P, 4, "f16", "f16")
     for P.max_rows in (P.rows, 100000, 2 ** 32 - 1):
         assert torch.equal(run_attention(ops, P, 4, "f16", "f16"), tight)
+
+
+def test_attention_workspace_in_a_foreign_capture(ops):
+    """A call onto a captured stream from one that is not: its own workspace would go back to the
+    allocator while the graph still uses it, so one must be given; then the graph replays."""
+    P = Pool(ops, [(1, 9000), (100, 300)], 2, 64, seed=5)
+    q, _, q64 = make_q(P, 4, "f16", 2)
+    o = torch.zeros(P.rows, 256, device="cuda", dtype=torch.float16)
+    size = ops.attention_chunk_workspace_bytes(P.rows, 2, 100, P.mp * 32, 4, 2, 64)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def call(stream, ws=None):
+        ops.attention_chunk_batch(q, None, P.kv, P.n_pages, P.tables, P.mp, P.row0, P.kv_len, 2, 100,
+                                  o, None, 4, 2, 64, True, 0, 0.125, workspace=ws, stream=stream)
+    other, inside = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = torch.cuda.current_stream()
+        for current in (other, torch.cuda.default_stream()):   # not part of the capture
+            with torch.cuda.stream(current):
+                for stream in (captured, captured.cuda_stream):
+                    with pytest.raises(ValueError, match="workspace"):
+                        call(stream)
+                call(captured, ws)
+        inside.wait_stream(captured)                   # part of it: the graph's own memory
+        call(inside)
+        captured.wait_stream(inside)
+    want, tol = ref_attention(P, q64, 4, True, 0, 0.125)
+    for _ in range(2):
+        o.zero_()
+        graph.replay()
+        check_rows(o, None, want, tol, 4, 64, P.rows)
