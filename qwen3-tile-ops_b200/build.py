@@ -53,10 +53,20 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def _native(lib: Path) -> None:
-    """``_native.so`` next to the library, which it finds by its own place."""
+    """``_native.so`` next to the library, which it finds by its own place.  A host that uses the
+    C ABI alone may lack what it is built against: then the library is all there is."""
     import sysconfig
 
-    import torch
+    missing = None
+    try:
+        import torch
+    except ImportError as e:
+        missing = str(e)
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        missing = "Python.h is not there"
+    if missing:
+        sys.stderr.write(f"{NATIVE.name} not built, for use from Python only: {missing}\n")
+        return
     src = CSRC / "python" / "q3_native.cpp"
     newest = max(f.stat().st_mtime for f in (src, INCLUDE / "q3_ops.h", Path(torch.__file__)))
     if NATIVE.exists() and NATIVE.stat().st_mtime >= newest:
