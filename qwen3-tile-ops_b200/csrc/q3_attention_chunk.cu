@@ -81,7 +81,7 @@ constexpr int ALONE_UNITS = 2, BESIDE_UNITS = 8;
 // 48 packed rows over 1000 tokens 15.1 us, in the many-row kernel 20.4; 64 over 2000 177 and 181; 8 of 64
 // rows over 4000 63 and 54.  Beside the many-row kernel: 16 ragged sequences 62.8 us, with 32 rows 64.0.
 constexpr int ALONE_ROWS = 48, BESIDE_ROWS = 16;
-constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that is never cut
+constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that one warp takes (make_plan)
 
 template <int HD>
 struct FewStage {
@@ -744,13 +744,15 @@ __global__ void __launch_bounds__(TILE_WARPS * 32) k_join_tiles(const Args p) {
 }
 
 // How a call is cut.  Sequences with at most few_rows packed rows go to k_attn_few (nt tiles of 8),
-// the others to the tensor-core kernel of many rows.
+// the others to the tensor-core kernel of many rows.  Which of them there are is known on the device
+// only, so k_attn_few (and, unless `whole`, its join) is always launched, the other kernel where
+// max_rows allows such sequences (tiles > 0).
 struct Plan {
   long packed;                                     // most packed rows of a sequence
   int nt, few_rows, min_units;
-  long few_ctas, few_tiles;                        // few_ctas 0: no such sequence can be there
+  long few_ctas, few_tiles;
   bool whole;                                      // their keys are not cut
-  long tiles;                                      // tiles 0: likewise
+  long tiles;                                      // 0: no sequence can have more than few_rows
   int splits;
   size_t few_slots, bytes;                         // parts of k_attn_few; the whole workspace
 };
@@ -766,27 +768,25 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
   c.few_rows = mixed ? BESIDE_ROWS : ALONE_ROWS;
   c.min_units = mixed ? BESIDE_UNITS : ALONE_UNITS;
   c.nt = packed > 8 ? 2 : 1;
-  if (group <= 16) {
-    // Up to 256 keys a warp takes a whole sequence if that gives each SM a warp (64 sequences of 220
-    // keys 12.5 us, cut 17.4; 8 of them 11.4 and 10.1), or to spare the many-row kernel (4 x 60 rows 15 us
-    // against 17)
-    c.whole = max_kv <= WHOLE_KEYS && (packed > 16 || static_cast<long>(n_seqs) * kv_heads > sms);
-    const long most_rows = packed < c.few_rows ? packed : c.few_rows;
-    const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB) *
-                       ((most_rows + 8 * c.nt - 1) / (8 * c.nt));
-    const long slices = (units + c.min_units - 1) / c.min_units;
-    const long most = static_cast<long>(sms) * few_ctas_sm(head_dim, c.nt), least = (kv_heads + WARPS - 1) / WARPS;
-    long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
-    ctas = ctas < most ? ctas : most;
-    ctas = ctas > least ? ctas : least;            // a slice at least
-    if (c.whole) {   // then all rows go there, in tiles
-      c.few_rows = 0x7fffffff;
-      c.few_tiles = (packed + 8 * c.nt - 1) / (8 * c.nt);
-      ctas = (static_cast<long>(n_seqs) * c.few_tiles * kv_heads + WARPS - 1) / WARPS;
-    }
-    c.few_ctas = ctas;
-    if (!c.whole) c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
+  // Up to 256 keys a warp takes a whole sequence if that gives each SM a warp (64 sequences of 220
+  // keys 12.5 us, cut 17.4; 8 of them 11.4 and 10.1), or to spare the many-row kernel (4 x 60 rows 15 us
+  // against 17)
+  c.whole = max_kv <= WHOLE_KEYS && (packed > 16 || static_cast<long>(n_seqs) * kv_heads > sms);
+  const long most_rows = packed < c.few_rows ? packed : c.few_rows;
+  const long units = static_cast<long>(n_seqs) * ((max_kv + KB - 1) / KB) *
+                     ((most_rows + 8 * c.nt - 1) / (8 * c.nt));
+  const long slices = (units + c.min_units - 1) / c.min_units;
+  const long most = static_cast<long>(sms) * few_ctas_sm(head_dim, c.nt), least = (kv_heads + WARPS - 1) / WARPS;
+  long ctas = (slices * kv_heads + WARPS - 1) / WARPS;
+  ctas = ctas < most ? ctas : most;
+  ctas = ctas > least ? ctas : least;              // a slice at least
+  if (c.whole) {   // then all rows go there, in tiles
+    c.few_rows = 0x7fffffff;
+    c.few_tiles = (packed + 8 * c.nt - 1) / (8 * c.nt);
+    ctas = (static_cast<long>(n_seqs) * c.few_tiles * kv_heads + WARPS - 1) / WARPS;
   }
+  c.few_ctas = ctas;
+  if (!c.whole) c.few_slots = 2 * static_cast<size_t>(c.few_ctas) * WARPS * 8 * c.nt;
   c.splits = 1;
   if (packed > c.few_rows) {
     const long all = static_cast<long>(rows) * group / TC_ROWS + n_seqs;
@@ -821,7 +821,9 @@ extern "C" size_t q3_attention_chunk_workspace_bytes(uint32_t rows, uint32_t n_s
                                                      uint32_t max_rows, uint32_t max_kv,
                                                      uint32_t heads, uint32_t kv_heads,
                                                      uint32_t head_dim) {
-  if (!rows || !n_seqs || !max_rows || !max_kv || !heads || !kv_heads || heads % kv_heads) return 0;
+  if (!rows || !n_seqs || !max_rows || !max_kv || !heads || !kv_heads || heads % kv_heads ||
+      heads / kv_heads > 16 || (head_dim != 64 && head_dim != 128))
+    return 0;
   return chunk::make_plan(rows, n_seqs, max_rows, max_kv, heads, kv_heads, head_dim).bytes;
 }
 
@@ -950,7 +952,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   p.scale_log2 = (float)((double)qk_scale * 1.4426950408889634);
   p.page_shift = (p.page_tokens & (p.page_tokens - 1)) ? -1 : __builtin_ctz(p.page_tokens);
   p.whole_blocks = p.page_tokens % chunk::KB == 0;
-  p.few_rows = c.few_ctas ? c.few_rows : 0;
+  p.few_rows = c.few_rows;
   cudaStream_t s = (cudaStream_t)stream;
   timer_begin(TIMER_ATTENTION, s);
   int st = Q3_OK;
@@ -963,7 +965,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     t.part_ml = t.part_o + static_cast<size_t>(c.splits) * c.tiles * kv_heads * chunk::TC_ROWS * head_dim;
     st = head_dim == 128 ? launch_many<128>(t, c.packed, s) : launch_many<64>(t, c.packed, s);
   }
-  if (st == Q3_OK && c.few_ctas) {
+  if (st == Q3_OK) {
     p.row_shift = c.nt == 1 ? 3 : 4;
     p.whole = c.whole;
     p.min_units = c.min_units;

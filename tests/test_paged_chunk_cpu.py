@@ -252,3 +252,10 @@ def test_wrapper_refuses_other_workspaces(q3):
         with pytest.raises(ValueError, match="workspace: a"):
             q3.ops.attention_chunk_batch(x, None, pool(q3._lib), 9, x, 1, x, x, 1, 1, x, None, 4, 2, 64,
                                          True, 0, 0.1, workspace=ws)
+
+
+def test_attention_workspace_bytes_of_refused_groups(L):
+    f = L.lib().q3_attention_chunk_workspace_bytes
+    assert f(64, 2, 32, 4096, 32, 2, 128) > 0                  # 16 query heads a KV head
+    for rows in (1, 64, 4096):
+        assert f(rows, 2, 2000, 4096, 34, 2, 128) == 0 and f(rows, 2, 1, 4096, 68, 4, 64) == 0
