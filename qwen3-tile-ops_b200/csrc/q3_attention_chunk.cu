@@ -904,7 +904,8 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
     }
   }
   const uint32_t rows = q->rows;
-  if (o->rows < rows || rows > 0x7fffffffu / 16 || n_seqs > 0x7ffffffeu) return Q3_ERR_SHAPE;
+  // (packed rows, rounded up to a tile, stay below 2^31)
+  if (o->rows < rows || rows > 0x7fffff00u / 16 || n_seqs > 0x7ffffffeu) return Q3_ERR_SHAPE;
   if (rows == 0 || n_seqs == 0) return Q3_OK;
   if (max_rows == 0) return Q3_ERR_SHAPE;
   const uint32_t max_kv = max_pages * kv->page_tokens;

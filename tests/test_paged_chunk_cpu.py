@@ -259,3 +259,12 @@ def test_attention_workspace_bytes_of_refused_groups(L):
     assert f(64, 2, 32, 4096, 32, 2, 128) > 0                  # 16 query heads a KV head
     for rows in (1, 64, 4096):
         assert f(rows, 2, 2000, 4096, 34, 2, 128) == 0 and f(rows, 2, 1, 4096, 68, 4, 64) == 0
+
+
+def test_attention_refuses_rows_past_32_bits(L):
+    """Packed rows, rounded up to a tile, stay below 2^31."""
+    big = lambda n, dt: view(L, n, 16 * 64, dt)                # noqa: E731
+    call = lambda n: attn_call(L, q=big(n, F16), o=big(n, F16), heads=16, kvh=1, hd=64,  # noqa: E731
+                               max_rows=1)
+    assert call(2 ** 27 - 1) == SHAPE and call(2 ** 27 - 15) == SHAPE
+    assert call(2 ** 27 - 16) == NULL                          # 2^31 - 256: on to the workspace
