@@ -891,7 +891,8 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   if (heads == 0 || heads % kv_heads || heads / kv_heads > 16) return Q3_ERR_SHAPE;
   if (causal != 0 && causal != 1) return Q3_ERR_MODE;
   if (window && (!causal || window > 0x7fffffffu)) return Q3_ERR_SHAPE;
-  if (!(qk_scale > 0.0f && qk_scale < INFINITY)) return Q3_ERR_SHAPE;
+  const float scale_log2 = (float)((double)qk_scale * 1.4426950408889634);
+  if (!(qk_scale > 0.0f && scale_log2 < INFINITY)) return Q3_ERR_SHAPE;
   for (int i = 0; i < 2; ++i) {
     const q3_view *x = i ? o : q, *xs = i ? os : q_scale;
     if (x->dtype != Q3_DT_I8 && x->dtype != Q3_DT_F16 && x->dtype != Q3_DT_BF16)
@@ -950,7 +951,7 @@ extern "C" int q3_attention_chunk_batch(const q3_view *q, const q3_view *q_scale
   p.group = (int)(heads / kv_heads);
   p.causal = causal;
   p.window = (int)window;
-  p.scale_log2 = (float)((double)qk_scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.page_shift = (p.page_tokens & (p.page_tokens - 1)) ? -1 : __builtin_ctz(p.page_tokens);
   p.whole_blocks = p.page_tokens % chunk::KB == 0;
   p.few_rows = c.few_rows;

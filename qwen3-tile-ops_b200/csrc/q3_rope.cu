@@ -458,7 +458,7 @@ extern "C" int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_
                 spec->beta_slow > 0.0 && spec->beta_fast >= spec->beta_slow &&
                 spec->beta_fast < INFINITY))
     return Q3_ERR_SHAPE;
-  if (!(spec->attn_factor < INFINITY)) return Q3_ERR_SHAPE;
+  if (!((float)spec->attn_factor < INFINITY)) return Q3_ERR_SHAPE;
   if (cos->rows == 0) return Q3_OK;
 
   TableArgs p;

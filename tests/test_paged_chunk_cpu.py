@@ -268,3 +268,9 @@ def test_attention_refuses_rows_past_32_bits(L):
                                max_rows=1)
     assert call(2 ** 27 - 1) == SHAPE and call(2 ** 27 - 15) == SHAPE
     assert call(2 ** 27 - 16) == NULL                          # 2^31 - 256: on to the workspace
+
+
+def test_factors_past_float32(L):
+    """Finite in the type that they are given in, not in the one that is used."""
+    assert tables(L, attn_factor=1e39) == SHAPE and tables(L, attn_factor=3e38) == OK
+    assert attn_call(L, scale=3e38) == SHAPE and attn_call(L, scale=2e38) == OK
