@@ -14,8 +14,9 @@
 // a weight outgrows it by 2^15 (p stays inside f16).
 //
 // bf16 queries are multiplied by a power of two per row, which brings the row's
-// maximum to [2^10, 2^11): their 8 bits then fit f16 exactly down to 2^-24 of
-// the row's maximum, and one f16 path serves all query types.
+// maximum to [2^10, 2^11) (many rows: or by 2^10, where that serves as well): their
+// 8 bits then fit f16 exactly down to 2^-24 of the row's maximum, and one f16
+// path serves all query types.
 #include <atomic>
 
 #include "q3_attention_chunk.h"

@@ -9,7 +9,7 @@
 //   warps 0-15   rows: eight warps a tile, two a TMEM lane quadrant, 16 rows each
 //   warps 16-23  codes of K and V from global memory, widened to f16 (exact), into a
 //                ring of three operand tiles in the 128-byte-swizzled layout
-//   warp 24      page lookups, and the keys' scales as ks qk_scale log2 e, log2 vs, 2^-7 / vs
+//   warp 24      page lookups, the keys' scales: ks qk_scale log2 e (2^-10), log2 vs, 2^-7 / vs
 //   warp 25      issues the products: S = Q K8^T (both operands in shared
 //                memory), O += P V8 (P in TMEM, over its scores)
 // The loads are plain ones because each code passes through registers on its
@@ -48,6 +48,7 @@ constexpr int TC_THREADS = 896;                    // whole warpgroups: two warp
 constexpr int RING = 3;                            // operand tiles K0, V0, K1, V1, ...
 constexpr int RAW = 3;                             // their codes, loaded or on the way
 constexpr int INFO = 4;                            // key tiles whose places and scales are known
+constexpr float BF16_UP = 1024.0f;                 // on bf16 queries
 constexpr int TMEM_O = 256;                        // S (and P) of tile t at 128 t, O at 256 + 128 t
 
 template <int HD>
@@ -451,8 +452,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
                                  fabsf(__uint_as_float(w[k] & 0xffff0000u))));
 #pragma unroll
           for (int o = 1; o < G8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          // within [2^-6, 2^15) f16 holds the row as it is (to 2^-19 of its maximum)
-          if (mx != 0.0f && !(mx >= 0.015625f && mx < 32768.0f)) bf16_scale(mx, up, down);
+          // rows of usual size, [2^-3, 2^5), take 2^10, which the keys' scales undo (a = 1 then): exact
+          // in f16 down to 2^-24 of the maximum, as others are with a power of their own
+          if (mx != 0.0f && !(mx >= 0.125f && mx < 32.0f)) {
+            bf16_scale(mx, up, down);
+            down = __fmul_rn(down, BF16_UP);
+          } else {
+            up = BF16_UP;
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             w[k] = pack_f16(__fmul_rn(__uint_as_float(w[k] << 16), up),
@@ -698,6 +705,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     // A lane has keys i*32 + lane of a tile.  Pages are looked up two tiles ahead; a tile's places
     // are published, and its scales requested, one tile ahead.
     const uint16_t *table = p.tables + static_cast<long>(s) * p.max_pages;
+    const float scale = p.q_dt == Q3_DT_BF16 ? __fmul_rn(p.scale_log2, 1.0f / BF16_UP) : p.scale_log2;
     auto page_of = [&](int j, int (&pg)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -752,7 +760,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
         const int key = i * 32 + lane, k = key & 15;
         const int to = (key & ~15) + ((k & 7) >> 1) * 4 + (k >> 3) * 2 + (k & 1);
         const float v = fmaxf(now.vs[i], kVsMin);    // (NaN: fmaxf drops it ...
-        sm.ks[in][to] = __fmul_rn(now.ks[i], p.scale_log2);
+        sm.ks[in][to] = __fmul_rn(now.ks[i], scale);
         // ... and the rows that see it get NaN); a key that is not there: weight 0
         sm.lv[in][to] = !now.have[i] ? kNegInf : now.vs[i] != now.vs[i] ? now.vs[i] : lg2(v);
         sm.rv[in][to] = __fmul_rn(rcp(v), kSumScale);

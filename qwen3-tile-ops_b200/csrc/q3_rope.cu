@@ -1,7 +1,7 @@
 // Rotary positions and the append to the paged int8 cache: tables of cos and
 // sin with scaled positions, rotation of row heads (with the head norm before
 // and the int8 codes after it), and the same on the way of new K/V rows into
-// their pages.  All three are bound by HBM for many rows and by launch and
+// their pages.  Tables and rows are bound by HBM for many rows, the append by its
 // load latency for few.
 #include <math.h>
 

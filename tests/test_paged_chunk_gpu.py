@@ -1077,3 +1077,21 @@ def test_attention_workspace_in_a_foreign_capture(ops):
         o.zero_()
         graph.replay()
         check_rows(o, None, want, tol, 4, 64, P.rows)
+
+
+@pytest.mark.parametrize("power", [-20, -6, -4, -3, 0, 4, 5, 12])
+@pytest.mark.parametrize("new", [3, 140])
+def test_attention_small_elements_of_bf16_queries(ops, new, power):
+    """One large element a row that meets zeros, all others 2^-12 of it, with their lowest bit set:
+    the logits are theirs alone, so they have to be exact in the products."""
+    P = Pool(ops, [(new, 200), (new, 333)], 1, 64, seed=26)
+    P.k.view(-1, 64)[:, 0] = 0
+    q = torch.full((P.rows, 2, 64), 2.0 ** -12 * (1 + 2.0 ** -7), device="cuda")
+    q[..., 0] = 1.0
+    q = (q * 2.0 ** power).to(torch.bfloat16)
+    scale = 6000.0 * 2.0 ** -power                     # logits of about 10
+    o = torch.empty(P.rows, 128, device="cuda", dtype=torch.float16)
+    ops.attention_chunk_batch(q.view(P.rows, -1), None, P.kv, P.n_pages, P.tables, P.mp, P.row0,
+                              P.kv_len, 2, new, o, None, 2, 1, 64, True, 0, scale)
+    want, tol = ref_attention(P, q.double(), 2, True, 0, scale)
+    check_rows(o, None, want, tol, 2, 64, P.rows)
