@@ -1095,3 +1095,38 @@ def test_attention_small_elements_of_bf16_queries(ops, new, power):
                               P.kv_len, 2, new, o, None, 2, 1, 64, True, 0, scale)
     want, tol = ref_attention(P, q.double(), 2, True, 0, scale)
     check_rows(o, None, want, tol, 2, 64, P.rows)
+
+
+def check_long_sums(ops, heads, kvh, hd, n, new, kv, causal=False):
+    """All values are 1 under weights that differ, over many keys: the result is 1, seen to float32 by
+    the scale of int8 output.  Returns the largest error.
+
+    What it may be: each weight's rounding to f16, at most 2^-11 of it and of either sign, so at most
+    2^-11 sqrt(2 ln(2 / P) sum w^2) but with probability P (the squares of weights e^x, x normal
+    of deviation s: e^(s^2) / keys): 1e-5 at P = 1e-12, s = 0.8 and 500000 keys.  Sums of a
+    thread over an eighth of the keys, 2^-25 an add of either sign: 4e-5 likewise.  What the tensor cores
+    cut in a running sum over 8192 keys: below 2^-24 of it for each of 16 terms and the sum itself, of
+    512 products, half of it since it grows: 2.6e-4."""
+    page = 4096
+    mp = -(-kv // page)
+    k = torch.randint(-127, 128, (mp, page, kvh * hd), device="cuda", generator=gen(1),
+                      dtype=torch.int8)
+    v = torch.full_like(k, 100)
+    ks = torch.full((mp, page, kvh), 0.01, device="cuda")
+    vs = torch.full_like(ks, 0.01)
+    tables = torch.arange(mp, device="cuda").to(torch.int16).expand(n, -1).contiguous()
+    cache = ops.paged_kv(k, v, ks, vs, tables, kvh, hd, page)
+    row0 = torch.arange(0, n * new + 1, new, dtype=torch.int32, device="cuda")
+    kv_len = torch.full((n,), kv, dtype=torch.int32, device="cuda")
+    q = torch.randn(n * new, heads * hd, device="cuda", generator=gen(2)).half()
+    o = torch.empty(n * new, heads * hd, dtype=torch.int8, device="cuda")
+    os = torch.empty(n * new, heads, device="cuda")
+    ops.attention_chunk_batch(q, None, cache, mp, tables, mp, row0, kv_len, n, new, o, os, heads, kvh,
+                              hd, causal, 0, hd ** -0.5)
+    assert (o == 127).all()
+    return float((os.double() * 127 / (100 * vs[0, 0, 0].double()) - 1).abs().max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_long_sums_few_rows(ops, hd):
+    assert check_long_sums(ops, 8, 8, hd, 444, 1, 500000) <= 2.0 ** -11
