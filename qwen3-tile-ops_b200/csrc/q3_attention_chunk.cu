@@ -814,7 +814,9 @@ static Plan make_plan(uint32_t rows, uint32_t n_seqs, uint32_t max_rows, uint32_
     c.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   }
   const size_t parts = c.splits > 1 ? static_cast<size_t>(c.splits) * c.tiles * kv_heads * TC_ROWS : 0;
-  c.bytes = (c.few_slots + parts) * (head_dim + 2) * 4;
+  const bool fold = c.tiles && c.splits == 1 && max_kv > FOLD_KEYS;
+  c.bytes = (c.few_slots + parts) * (head_dim + 2) * 4 +
+            (fold ? static_cast<size_t>(rows) * heads * head_dim * 4 : 0);
   return c;
 }
 

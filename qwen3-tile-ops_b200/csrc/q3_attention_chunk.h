@@ -28,7 +28,8 @@ struct Args {
   int whole;                     // it takes a sequence's keys as a whole
   int page_shift;                // log2 of page_tokens, or -1
   int whole_blocks;              // a 32-key block lies in one page
-  float *part_o, *part_ml;       // parts: sums [..][hd], and their (maximum, sum of weights)
+  float *part_o, *part_ml;       // parts: sums [..][hd], and their (maximum, sum of weights); of one part: the
+                                 // sums of row r and head h at (r heads + h) hd
 };
 
 // Rows of sequence s as the device sees them; ok = false: nothing to do
@@ -173,6 +174,10 @@ __device__ __forceinline__ int find_unit(int n_seqs, long unit, int lane, long &
 // Many rows (q3_attention_chunk_tc.cu): sequences with more than few_rows packed rows.  `tiles` is the
 // number of 256-row tiles that the batch can have.
 constexpr int TC_ROWS = 256, TC_KEYS = 128;
+// Its sums of values run over at most FOLD_TILES key tiles in the tensor cores, which cut the bits that a
+// running sum cannot hold, always towards zero (3.3e-3 of it over 500000 keys); then they are added to
+// float32 sums in the workspace.
+constexpr int FOLD_TILES = 64, FOLD_KEYS = FOLD_TILES * TC_KEYS;
 __device__ __forceinline__ long tiles_of(const Args &p, int s, unsigned *err) {
   const Seq q = load_seq(p, s, err);
   const int packed = q.n * p.group;

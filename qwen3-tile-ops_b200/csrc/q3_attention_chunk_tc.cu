@@ -60,7 +60,7 @@ struct TcSmem {
   // 8 + 2 t4, 8 + 2 t4 + 1]
   alignas(16) float ks[INFO][TC_KEYS], lv[INFO][TC_KEYS], rv[INFO][TC_KEYS];
   long long place[INFO][TC_KEYS];                  // byte offset of a key's row in the pool, or -1
-  float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS];
+  float a[TC_ROWS], l[TC_ROWS], m[TC_ROWS], fold_m[TC_ROWS];
   unsigned long long full[RING], empty[RING], place_full[INFO], info_full[INFO], info_empty[INFO];
   unsigned long long s_full[2][2], p_full[2][2], o_full;   // [row tile][half & 1]
   uint32_t tmem;
@@ -316,6 +316,47 @@ __device__ __forceinline__ void rows16(const float *ks, const float *lv, const f
   l[1] = __fadd_rn(l[1], __fadd_rn(u, v));
 }
 
+// The sums at `ot` of 16 rows of a warp (a thread: rows e = 0, 1, as in rows16) to the float32 sums of
+// these rows, `to`, which are relative to the reference *from; first: there are none yet.  `next`, par: as
+// there.  The products after it start from zero.
+template <int HD>
+__device__ __forceinline__ void fold16(uint32_t ot, float *const (&to)[2], float *const (&from)[2], bool first,
+                                       unsigned long long *next, int par, int *abort,
+                                       const float (&mref)[2]) {
+  wait_bar(next, par, abort);
+  __syncwarp();
+  fence_after();
+  float f[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float was = first ? kNegInf : *from[e];
+    f[e] = was == kNegInf ? 0.0f : ex2(__fsub_rn(was, mref[e]));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 2; ++e) *from[e] = mref[e];   // (four lanes, the same value)
+#pragma unroll 1
+  for (int c = 0; c < HD / 32; ++c) {
+    float o[16];
+    float2 x[8];                                     // all loads before the stores
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {                    // (no such row: null)
+      x[i] = make_float2(0.0f, 0.0f);
+      if (!first && to[i & 1]) x[i] = *reinterpret_cast<const float2 *>(to[i & 1] + c * 32 + (i >> 1) * 8);
+    }
+    __syncwarp();
+    tm_ld(ot + c * 32, o);
+    tmem_wait_ld();
+    landed(o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = __fmaf_rn(x[i].x, f[i & 1], o[2 * i]), b = __fmaf_rn(x[i].y, f[i & 1], o[2 * i + 1]);
+      if (to[i & 1]) *reinterpret_cast<float2 *>(to[i & 1] + c * 32 + (i >> 1) * 8) = make_float2(a, b);
+    }
+    __syncwarp();
+  }
+}
+
 __device__ __forceinline__ bool elect_one() {   // one lane of the converged warp
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
@@ -496,36 +537,54 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     const int pmax = q.pos0 + token(min(rb + 15, rows - 1), unused);
     const int mine = t ? ht[1] : ht[0];
     const uint32_t st = tmem + (static_cast<uint32_t>(qd * 32 + ps * 16) << 16) + t * 128;
-    for (int j = 0; j < nj; ++j) {
-      const int in = j % INFO;
-      wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
-      const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int h = 2 * j + b;
-        if (h < mine) {
-          wait_bar(&sm.s_full[t][b], j & 1, &sm.abort);
-          __syncwarp();
-          fence_after();
-          const int key0 = z0 * TC_KEYS + h * 64, at = b * 64, par = h ? ((h + 1) >> 1) & 1 : -1;
-          const bool masked = (p.causal && key0 + 63 > pmin) || (p.window > 0 && key0 <= pmax - p.window);
-          if (masked)
-            rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                    &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
-          else if (unit)
-            rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                    &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
-          else
-            rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                     &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
-          tmem_wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full[t][b]);
-        }
+    // float32 sums of packed row x of the tile
+    auto sums_of = [&](int x) -> float * {
+      int hx;
+      const long r = q.first + token(x, hx);
+      const long at = p.splits > 1 ? (static_cast<long>(blockIdx.x) * p.splits + blockIdx.z) * TC_ROWS + x
+                                   : r * p.heads + kvh * p.group + hx;
+      return p.part_o + at * HD;
+    };
+    for (int j0 = 0; j0 < nj; j0 += FOLD_TILES) {
+      if (j0 && 2 * j0 < mine) {
+        const int m = rb + g;
+        float *const to[2] = {m < rows ? sums_of(m) + t4 * 2 : nullptr,
+                              m + 8 < rows ? sums_of(m + 8) + t4 * 2 : nullptr};
+        float *const from[2] = {sm.fold_m + m, sm.fold_m + m + 8};
+        fold16<HD>(st + TMEM_O, to, from, j0 == FOLD_TILES, &sm.s_full[t][1], j0 & 1, &sm.abort, mref);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.info_empty[in]);
+#pragma unroll 1
+      for (int j = j0; j < min(nj, j0 + FOLD_TILES); ++j) {
+        const int in = j % INFO;
+        wait_bar(&sm.info_full[in], (j / INFO) & 1, &sm.abort);
+        const float *ks = sm.ks[in] + t4 * 4, *lv = sm.lv[in] + t4 * 4, *rv = sm.rv[in] + t4 * 4;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int h = 2 * j + b;
+          if (h < mine) {
+            wait_bar(&sm.s_full[t][b], j & 1, &sm.abort);
+            __syncwarp();
+            fence_after();
+            const int key0 = z0 * TC_KEYS + h * 64, at = b * 64, par = h ? ((h + 1) >> 1) & 1 : -1;
+            const bool masked = (p.causal && key0 + 63 > pmin) || (p.window > 0 && key0 <= pmax - p.window);
+            if (masked)
+              rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                      &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+            else if (unit)
+              rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                      &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+            else
+              rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
+                                       &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[t][b]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.info_empty[in]);
+      }
     }
     // ---- sums of the rows; then each thread half the columns of its own row
 #pragma unroll
@@ -539,6 +598,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
       }
     }
     asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");   // the eight warps of the tile
+    // (the float32 sums of other warps' threads are visible behind it, too)
     if (nj > 0) wait_bar(&sm.o_full, 0, &sm.abort);
     fence_after();
     const int m = t * 128 + qd * 32 + lane;
@@ -548,6 +608,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
     const int h = kvh * p.group + hg;
     const uint32_t src = tmem + (static_cast<uint32_t>(qd * 32) << 16) + TMEM_O + t * 128;
     const float lsum = sm.l[m];
+    // 32 columns of this lane's row
+    const bool folded = mine > 2 * FOLD_TILES && have;
+    const float ff = !folded || sm.fold_m[m] == kNegInf ? 0.0f : ex2(__fsub_rn(sm.fold_m[m], sm.m[m]));
+    auto sums = [&](int c, float (&o)[32]) {
+      tm_ld_row(src + c * 32, o);
+      tmem_wait_ld();
+      landed(o);
+      if (folded) {
+        const float4 *at = reinterpret_cast<const float4 *>(sums_of(m) + c * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float4 x;   // (one at a time: 32 more registers are not there)
+          asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];"
+                       : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                       : "l"(at + i)
+                       : "memory");
+          o[4 * i] = __fmaf_rn(x.x, ff, o[4 * i]);
+          o[4 * i + 1] = __fmaf_rn(x.y, ff, o[4 * i + 1]);
+          o[4 * i + 2] = __fmaf_rn(x.z, ff, o[4 * i + 2]);
+          o[4 * i + 3] = __fmaf_rn(x.w, ff, o[4 * i + 3]);
+        }
+      }
+      __syncwarp();
+    };
     // this warp's columns, 32 at a time (its chunks ps * OC ..), go through its part of the query
     // tile, which the products no longer read: a row's pieces then leave as whole lines
     constexpr int OC = HD / 64;
@@ -576,9 +660,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
 #pragma unroll 1
         for (int c = ps * OC; c < ps * OC + OC; ++c) {
           Elems<float, 32> o;
-          tm_ld_row(src + c * 32, o.e);
-          tmem_wait_ld();
-          landed(o.e);
+          sums(c, o.e);
 #pragma unroll
           for (int i = 0; i < 8; ++i) put(128, i, o.v[i]);
           flush(128, reinterpret_cast<char *>(p.part_o + at * HD + c * 32));
@@ -599,9 +681,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           float o[32];
-          tm_ld_row(src + c * 32, o);
-          tmem_wait_ld();
-          landed(o);
+          sums(c, o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(__fmul_rn(o[i], inv)));
         }
@@ -611,9 +691,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
 #pragma unroll 1
       for (int c = 0; c < OC; ++c) {
         float o[32];
-        tm_ld_row(src + (ps * OC + c) * 32, o);
-        tmem_wait_ld();
-        landed(o);
+        sums(ps * OC + c, o);
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = __fmul_rn(o[i], inv);
         if (i8) {
@@ -795,7 +873,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           mma_ts(tmem + TMEM_O + t * 128, tmem + t * 128 + (h & 1) * 64 + k * 8, b + k * (2048 / 16),
-                 ID_O, h > 0 || k > 0);
+                 ID_O, h % (2 * FOLD_TILES) > 0 || k > 0);
       };
       auto ready = [&](int item) {
         wait_bar(&sm.full[item % RING], (item / RING) & 1, &sm.abort);

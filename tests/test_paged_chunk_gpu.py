@@ -1130,3 +1130,24 @@ def check_long_sums(ops, heads, kvh, hd, n, new, kv, causal=False):
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_long_sums_few_rows(ops, hd):
     assert check_long_sums(ops, 8, 8, hd, 444, 1, 500000) <= 2.0 ** -11
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_long_sums_many_rows(ops, hd):
+    assert check_long_sums(ops, 32, 8, hd, 1, 1024, 500000) <= 2.0 ** -11        # one part
+    assert check_long_sums(ops, 4, 2, hd, 1, 130, 500000) <= 2.0 ** -11          # several
+
+
+@pytest.mark.parametrize("heads,kvh,hd,lens,window,otype", [
+    (16, 4, 128, [(900, 20000), (300, 8193), (20, 30000), (257, 17000)], 0, "f16"),
+    (32, 8, 64, [(600, 8192 + 600), (40, 40000)], 0, "i8"),
+    (24, 8, 64, [(500, 33000)], 20000, "bf16"),
+    (2, 1, 128, [(300, 300000)], 0, "f16"), (3, 1, 64, [(200, 200000), (1, 9)], 0, "i8")])
+def test_attention_folded_sums(ops, heads, kvh, hd, lens, window, otype):
+    """Key ranges over a fold, in one part and in several, of tiles that end at other key tiles than
+    their CTA, whose references grow late (a few keys have far larger scales)."""
+    P = Pool(ops, lens, kvh, hd, page=64, seed=33)
+    P.ks.mul_(0.2)
+    far = torch.rand(P.ks.shape, device="cuda", generator=gen(8)) < 2e-4
+    P.ks.mul_(1.0 + 19.0 * far)
+    run_attention(ops, P, heads, "f16", otype, True, window, seed=2)
