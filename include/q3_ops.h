@@ -334,9 +334,9 @@ int q3_rope_tables(const q3_rope_spec *spec, uint32_t pos0, const q3_view *cos,
  * inv_hd = 1/head_dim), then rotation of the first rot = 2*cos->cols columns
  * (a multiple of 16) by row pos[r] of the tables: pairs (i, i + rot/2), or
  * (2i, 2i + 1) with interleaved.  x: f32, f16 or bf16.  out: f32, f16, bf16
- * (rounded once; may be x itself), or int8 with one scale per head in `scale`
- * (rows x heads f32), the codes of the norm-rope-quant epilogue of
- * q3_gemm_nt_group_store bit for bit.  A row whose position is not in the tables
+ * (rounded once; may be x itself, and must not overlap it otherwise), or int8
+ * with one scale per head in `scale` (rows x heads f32), the codes of the
+ * norm-rope-quant epilogue of q3_gemm_nt_group_store bit for bit.  A row whose position is not in the tables
  * is not written (status bit 4). */
 int q3_rope_rows(const q3_view *x, const q3_view *nw, const int32_t *pos, const q3_view *cos,
                  const q3_view *sin, const q3_view *out, const q3_view *scale, uint32_t heads,
@@ -367,8 +367,9 @@ int q3_paged_kv_append_batch(const q3_view *k, const q3_view *v, const q3_view *
  * of kv_heads, at most 16 times it.  max_rows: no sequence has more new rows;
  * one that has sets status bit 5 and is skipped.  The workspace of
  * q3_attention_chunk_workspace_bytes (the call's own sizes: the bytes need not
- * grow with each; max_kv = max_pages * page_tokens, at most 2^31 - 256) is written
- * by the call; calls that may overlap on the GPU need one each. */
+ * grow with each; max_kv = max_pages * page_tokens, at most 2^31 - 256, and n_seqs *
+ * max_kv below 2^35) is written by the call; calls that may overlap on the GPU
+ * need one each. */
 size_t q3_attention_chunk_workspace_bytes(uint32_t rows, uint32_t n_seqs, uint32_t max_rows,
                                           uint32_t max_kv, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim);

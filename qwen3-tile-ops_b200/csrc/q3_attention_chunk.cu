@@ -43,10 +43,14 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // c += a b, the product by itself, then added in float32: in a running sum the tensor cores cut the bits that
-// it cannot hold, always towards zero (over 500000 keys 3.3e-3 of the sum; an add costs 0.3 us of 54)
+// it cannot hold, always towards zero (over 500000 keys 3.3e-3 of the sum; the adds cost 0.2 us of 54, 0.4 of 18)
 __device__ __forceinline__ void add_product(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  mma_16816(x, a, b[0], b[1]);
+  float x[4];
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.0f));
   // two at once
 #pragma unroll
   for (int i = 0; i < 4; i += 2)
@@ -94,6 +98,9 @@ constexpr int ALONE_UNITS = 2, BESIDE_UNITS = 8;
 // Most packed rows of a sequence of this kernel, in tiles that read the keys again.  Alone: 2 sequences of
 // 48 packed rows over 1000 tokens 15.1 us, in the many-row kernel 20.4; 64 over 2000 177 and 181; 8 of 64
 // rows over 4000 63 and 54.  Beside the many-row kernel: 16 ragged sequences 62.8 us, with 32 rows 64.0.
+// That batch has few sequences between the two bounds; with many the step down costs: 63 of 20 packed
+// rows over 2000 tokens take 113 us alone, 176 where max_rows allows more than 48 packed ones, and 209
+// with a chunk of 1000 rows (itself 55).
 constexpr int ALONE_ROWS = 48, BESIDE_ROWS = 16;
 constexpr uint32_t WHOLE_KEYS = 256;               // most keys of a sequence that one warp takes (make_plan)
 

@@ -16,7 +16,8 @@
 // way (the tensor cores take no f16 x int8); rows of pages of any length then need
 // no tile shape of their own.
 //
-// 2 x 4096 rows behind 4096 tokens, 16 heads over 8: 503 us, 820 TFLOP/s (mma.sync for the same rows: 5.4 ms).
+// 2 x 4096 rows behind 4096 tokens, 16 heads over 8: 503 us, 820 TFLOP/s, four sets of inputs (over L2) in turn
+// in a graph (mma.sync for the same rows: 5.4 ms); with int8 output 514, not causal 691.
 // A key tile takes 2.8 us for the 256 rows, of which the tensor cores need 1.5: the row warps' issue
 // slots and the widening are the bound (385 us with rows that do nothing), and a CTA takes about
 // 10 us to start and end.  Sixteen row warps hold 64 keys of 16 rows each without spilling;
@@ -568,14 +569,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const Args p) {
             const int key0 = z0 * TC_KEYS + h * 64, at = b * 64, par = h ? ((h + 1) >> 1) & 1 : -1;
             const bool masked = (p.causal && key0 + 63 > pmin) || (p.window > 0 && key0 <= pmax - p.window);
             if (masked)
-              rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                      &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+              rows16<HD, true, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O,
+                                      &sm.s_full[t][b ^ 1], par, &sm.abort, a, mref, l, pos,
+                                      key0 + t4 * 2, p.causal, p.window);
             else if (unit)
-              rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                      &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+              rows16<HD, false, true>(ks + at, lv + at, rv + at, st + at, st + TMEM_O,
+                                      &sm.s_full[t][b ^ 1], par, &sm.abort, a, mref, l, pos,
+                                      key0 + t4 * 2, p.causal, p.window);
             else
-              rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O, &sm.s_full[t][b ^ 1], par,
-                                       &sm.abort, a, mref, l, pos, key0 + t4 * 2, p.causal, p.window);
+              rows16<HD, false, false>(ks + at, lv + at, rv + at, st + at, st + TMEM_O,
+                                       &sm.s_full[t][b ^ 1], par, &sm.abort, a, mref, l, pos,
+                                       key0 + t4 * 2, p.causal, p.window);
             tmem_wait_st();
             fence_before();
             __syncwarp();

@@ -1,8 +1,8 @@
 // Rotary positions and the append to the paged int8 cache: tables of cos and
 // sin with scaled positions, rotation of row heads (with the head norm before
 // and the int8 codes after it), and the same on the way of new K/V rows into
-// their pages.  Tables and rows are bound by HBM for many rows, the append by its
-// load latency for few.
+// their pages.  Tables and rows are bound by HBM when they are many, the append by its
+// look-ups; few of any by launch and load latency.
 #include <math.h>
 
 #include "q3_paged.cuh"
@@ -239,6 +239,8 @@ __device__ __forceinline__ float head_int8(const float (&x)[N], void *codes, boo
 // and one root for U heads brought 24.3 and 20.7 us (5.7 and 5.0 TB/s), 8192 bf16 rows of 32 heads
 // with norm 42.7 -> 33.3.  Registers are held to what 8 CTAs an SM leave (9 for f32; 7 and 5 for
 // heads in a whole warp): without the limit 23 us, at 10 CTAs 39 for the bf16 rows with norm.
+// (The limit spills in the 16-bit forms, 12 to 24 bytes a thread.)  int8 codes out take 27.3 us for the
+// 8192 rows and 27.2 for the 5003, bound by the instructions of the codes; a decode batch 2.8, floats 2.4.
 // ---------------------------------------------------------------------------
 struct RowArgs {
   const char *x;
@@ -306,8 +308,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? (GL == 32 ? 7 : 8) : N =
 
 // ---------------------------------------------------------------------------
 // append.  A warp takes U KV heads of K or of V of one row; the row's data is
-// requested before the dependent lookups (row -> sequence -> position -> page).  Bound by those
-// for few rows (64 rows of 8 KV heads: about 4 us), by HBM for many.
+// requested before the dependent lookups (row -> sequence -> position -> page -> table row), which are the
+// bound: 64 rows of 8 KV heads 3.5 us, 3472 of them, 21.5 MB, 9.8 us at 2.2 TB/s.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const char *k, *v;
