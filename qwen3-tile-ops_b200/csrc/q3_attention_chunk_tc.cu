@@ -20,8 +20,8 @@
 // in a graph (mma.sync for the same rows: 5.4 ms); with int8 output 514, not causal 691.
 // A key tile takes 2.8 us for the 256 rows, of which the tensor cores need 1.5: the row warps' issue
 // slots and the widening are the bound (385 us with rows that do nothing), and a CTA takes about
-// 10 us to start and end.  Sixteen row warps hold 64 keys of 16 rows each without spilling;
-// 256 rows share one widening of K and V.
+// 10 us to start and end.  Sixteen row warps hold 64 keys of 16 rows each in registers (4 bytes a thread
+// spill since the sums are folded); 256 rows share one widening of K and V.
 #include <atomic>
 
 #include "q3_attention_chunk.h"
